@@ -1,0 +1,228 @@
+// attn_api.cu -- the lk_attn_* C ABI (include/loki_attn.h): context, workspaces, argument checks and launches.
+#include <cstdio>
+#include <cstdarg>
+#include <new>
+#include "attn_internal.h"
+
+using namespace lk;
+
+struct LkAttnCtx {
+    LkAttnConfig cfg;
+    int device = 0, nsm = 0;
+    int* err = nullptr;
+    int* n_moves = nullptr; int* moves = nullptr; int64_t moves_cap = 0;      // eviction: [2][n_seqs][region]
+    char msg[256] = {0};
+};
+
+static int set_err(LkAttnCtx* c, int code, const char* fmt, ...) {
+    if (c) { va_list ap; va_start(ap, fmt); vsnprintf(c->msg, sizeof(c->msg), fmt, ap); va_end(ap); }
+    return code;
+}
+#define LK_CU(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) \
+    return set_err(c, LK_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); } while (0)
+
+namespace {
+// the context's device for the length of a call; the caller's is put back
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(int device) { if (cudaGetDevice(&prev) == cudaSuccess && prev != device) cudaSetDevice(device); else prev = -1; }
+    ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
+};
+}
+
+static bool is16(const void* p) { return p && !((uintptr_t)p & 15); }
+
+// the cache's fields, and what the kernels see of it
+static int check_cache(LkAttnCtx* c, const LkKvCache* k, KvView* v) {
+    if (!k) return set_err(c, LK_ERR_ARG, "null cache");
+    if (k->dtype != LK_DT_F16 && k->dtype != LK_DT_BF16) return set_err(c, LK_ERR_UNSUPPORTED, "cache dtype %d: fp16 (1) or bf16 (2)", k->dtype);
+    if (!is16(k->rows)) return set_err(c, LK_ERR_ARG, "cache rows null or not 16-byte aligned");
+    if (k->row_stride < AT_ROW || k->row_stride % 8) return set_err(c, LK_ERR_ARG, "row stride %lld: at least 576 and a multiple of 8", (long long)k->row_stride);
+    int shift = 4;
+    while (shift < 8 && (1 << shift) != k->page_size) ++shift;
+    if ((1 << shift) != k->page_size) return set_err(c, LK_ERR_UNSUPPORTED, "page size %d: 16, 32, 64, 128 or 256", k->page_size);
+    if (k->n_pages < 1 || (int64_t)k->n_pages * k->page_size > 0x7fffffff) return set_err(c, LK_ERR_ARG, "%d pages of %d rows", k->n_pages, k->page_size);
+    if (k->n_seqs < 1 || k->n_seqs > c->cfg.max_seqs) return set_err(c, LK_ERR_CAPACITY, "%d sequences, context capacity %d", k->n_seqs, c->cfg.max_seqs);
+    if (!k->block_table || !k->lens) return set_err(c, LK_ERR_ARG, "null block table or lens");
+    if (k->table_stride < 1 || (int64_t)k->table_stride * k->page_size > 0x7fffff00) return set_err(c, LK_ERR_ARG, "table stride %d", k->table_stride);
+    *v = KvView{ k->rows, k->row_stride, k->page_size, shift, k->n_pages, k->table_stride, k->n_seqs, k->block_table, k->lens, k->mass, k->pos };
+    return LK_OK;
+}
+
+static int check_rows(LkAttnCtx* c, const char* name, const void* p, int64_t token, int64_t head) {
+    if (!is16(p)) return set_err(c, LK_ERR_ARG, "%s null or not 16-byte aligned", name);
+    if (token % 8 || head % 8) return set_err(c, LK_ERR_ARG, "%s strides must be multiples of 8", name);
+    return LK_OK;
+}
+
+extern "C" {
+
+int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
+    if (!cfg || !out) return LK_ERR_ARG;
+    *out = nullptr;
+    if (cfg->max_seqs < 1 || cfg->max_seqs > LK_ATTN_MAX_SEQS || cfg->max_tokens < 1 || cfg->max_tokens > LK_ATTN_MAX_SEQS * LK_ATTN_MAX_NODES)
+        return LK_ERR_UNSUPPORTED;
+    LkAttnCtx* c = new (std::nothrow) LkAttnCtx();
+    if (!c) return LK_ERR_CAPACITY;
+    c->cfg = *cfg;
+    c->device = device;
+    int prev = 0;
+    cudaError_t e = cudaGetDevice(&prev);
+    if (e == cudaSuccess) e = cudaSetDevice(device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&c->nsm, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&c->err, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(c->err, 0, sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc((void**)&c->n_moves, (size_t)cfg->max_seqs * sizeof(int));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    cudaSetDevice(prev);
+    if (e != cudaSuccess) { lk_attn_destroy(c); return LK_ERR_CUDA; }
+    *out = c;
+    return LK_OK;
+}
+
+void lk_attn_destroy(LkAttnCtx* c) {
+    if (!c) return;
+    OnDevice on(c->device);
+    void* ptrs[] = { c->err, c->n_moves, c->moves };
+    for (void* p : ptrs) if (p) cudaFree(p);
+    delete c;
+}
+
+int lk_attn_get_error(LkAttnCtx* c, lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    OnDevice on(c->device);
+    LK_CU(cudaStreamSynchronize((cudaStream_t)stream));
+    int e = 0;
+    LK_CU(cudaMemcpy(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost));
+    if (!e) return LK_OK;
+    LK_CU(cudaMemset(c->err, 0, sizeof(int)));
+    const char* what = e == ATT_ERR_PAGE ? "a page id outside the pool" : e == ATT_ERR_POS ? "a position outside the rope table"
+                     : e == ATT_ERR_LEN ? "a length outside its pages" : e == ATT_ERR_TREE ? "token ranges out of order or too long"
+                     : "a bounded wait ran out";
+    return set_err(c, LK_ERR_DEVICE, "device error code %d: %s", e, what);
+}
+
+const char* lk_attn_last_error(LkAttnCtx* c) { return c ? c->msg : "null context"; }
+
+int lk_attn_rope_table(LkAttnCtx* c, const LkRopeConfig* cfg, int max_pos, float* table, lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    if (!cfg || !table || ((uintptr_t)table & 7)) return set_err(c, LK_ERR_ARG, "null config, or table null or not 8-byte aligned");
+    if (cfg->rot_dim < 2 || cfg->rot_dim % 2 || cfg->rot_dim > 4096 || max_pos < 1 || max_pos > (1 << 26)) return set_err(c, LK_ERR_ARG, "rot_dim %d, max_pos %d", cfg->rot_dim, max_pos);
+    if (!(cfg->base > 1.0) || !(cfg->factor >= 1.0) || !(cfg->mscale > 0.0)) return set_err(c, LK_ERR_ARG, "base must exceed 1, factor be at least 1, mscale positive");
+    if (cfg->factor > 1.0 && (cfg->orig_ctx < 1 || !(cfg->beta_slow > 0.0) || !(cfg->beta_fast >= cfg->beta_slow)))
+        return set_err(c, LK_ERR_ARG, "a stretched context needs orig_ctx and beta_fast >= beta_slow > 0");
+    OnDevice on(c->device);
+    LK_CU(launch_rope_table(*cfg, max_pos, (float2*)table, (cudaStream_t)stream));
+    return LK_OK;
+}
+
+int lk_attn_rope(LkAttnCtx* c, int dtype, const void* x, int64_t x_token, int64_t x_head, void* y, int64_t y_token, int64_t y_head,
+                 int T, int H, int head_dim, int rot_offset, int rot_dim, int layout, int grad, const int* pos, const float* table,
+                 int max_pos, lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    if (dtype < LK_DT_F32 || dtype > LK_DT_BF16 || layout < LK_ROPE_INTERLEAVED || layout > LK_ROPE_HALF)
+        return set_err(c, LK_ERR_UNSUPPORTED, "dtype %d, layout %d", dtype, layout);
+    if (T < 0 || H < 1 || H > 65536 || head_dim < 1 || head_dim > 65536 || rot_dim < 2 || rot_dim % 2 || rot_offset < 0 || rot_offset > head_dim - rot_dim || max_pos < 1)
+        return set_err(c, LK_ERR_ARG, "T %d, H %d, head_dim %d, rotated part [%d, %d)", T, H, head_dim, rot_offset, rot_offset + rot_dim);
+    if (T == 0) return LK_OK;
+    const int es = dtype == LK_DT_F32 ? 4 : 2;
+    if (!x || !y || !pos || !table || ((uintptr_t)x | (uintptr_t)y) % es || ((uintptr_t)table & 7)) return set_err(c, LK_ERR_ARG, "null or misaligned pointer");
+    if (x == y && (x_token != y_token || x_head != y_head)) return set_err(c, LK_ERR_ARG, "in place needs equal strides");
+    if ((int64_t)T * (((int64_t)H * head_dim + 31) / 32) > 0x7fffffff) return set_err(c, LK_ERR_CAPACITY, "T %d x H %d x %d", T, H, head_dim);
+    OnDevice on(c->device);
+    RopeParams p{ x, x_token, x_head, y, y_token, y_head, T, H, head_dim, rot_offset, rot_dim, grad != 0, x != y, pos, (const float2*)table, max_pos, c->err };
+    LK_CU(launch_rope(p, dtype, layout, (cudaStream_t)stream));
+    return LK_OK;
+}
+
+int lk_attn_append(LkAttnCtx* c, const LkKvCache* cache, int in_dtype, const void* latent, int64_t latent_ld, const void* k_rope,
+                   int64_t rope_ld, int T, const int* starts, const int* pos, const float* table, int max_pos, int layout,
+                   lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    AppendParams p{};
+    if (int rc = check_cache(c, cache, &p.kv)) return rc;
+    if (in_dtype != LK_DT_F32 && in_dtype != cache->dtype) return set_err(c, LK_ERR_UNSUPPORTED, "input dtype %d: fp32 or the cache's", in_dtype);
+    if (layout < LK_ROPE_INTERLEAVED || layout > LK_ROPE_HALF) return set_err(c, LK_ERR_UNSUPPORTED, "layout %d", layout);
+    if (T < 0 || T > 0x7fffffff / 256 || max_pos < 1) return set_err(c, LK_ERR_ARG, "T %d, max_pos %d", T, max_pos);
+    if (T == 0) return LK_OK;
+    if (int rc = check_rows(c, "latent", latent, latent_ld, 0)) return rc;
+    if (int rc = check_rows(c, "k_rope", k_rope, rope_ld, 0)) return rc;
+    if (!starts || !pos || !table || ((uintptr_t)table & 7)) return set_err(c, LK_ERR_ARG, "null or misaligned pointer");
+    OnDevice on(c->device);
+    p.latent = latent; p.latent_ld = latent_ld; p.k_rope = k_rope; p.rope_ld = rope_ld; p.T = T; p.starts = starts; p.pos = pos;
+    p.table = (const float2*)table; p.max_pos = max_pos; p.err = c->err;
+    LK_CU(launch_append(p, in_dtype, cache->dtype, layout, (cudaStream_t)stream));
+    return LK_OK;
+}
+
+// what lk_attn_tree and lk_attn_mass check alike
+static int tree_params(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H,
+                       const int* starts, const uint64_t* tree, float scale, TreeParams* p) {
+    if (int rc = check_cache(c, cache, &p->kv)) return rc;
+    if (T < 0 || H < 1 || H > LK_ATTN_MAX_HEADS) return set_err(c, LK_ERR_ARG, "T %d, H %d (at most %d heads)", T, H, LK_ATTN_MAX_HEADS);
+    if (T > c->cfg.max_tokens) return set_err(c, LK_ERR_CAPACITY, "T %d > capacity %d", T, c->cfg.max_tokens);
+    if (!(scale > 0.0f) || scale > 3.0e38f) return set_err(c, LK_ERR_ARG, "scale must be positive and finite");
+    if (T == 0) return LK_OK;
+    if (int rc = check_rows(c, "q", q, q_token, q_head)) return rc;
+    if (!starts || ((uintptr_t)tree & 7)) return set_err(c, LK_ERR_ARG, "null starts or misaligned tree");
+    p->q = q; p->q_token = q_token; p->q_head = q_head; p->T = T; p->H = H; p->starts = starts; p->tree = tree; p->scale = scale;
+    p->err = c->err;
+    return LK_OK;
+}
+
+int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H, const int* starts,
+                 const uint64_t* tree, float scale, void* out, int64_t out_token, int64_t out_head, float* lse, lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    TreeParams p{};
+    if (int rc = tree_params(c, cache, q, q_token, q_head, T, H, starts, tree, scale, &p)) return rc;
+    if (T == 0) return LK_OK;
+    if (int rc = check_rows(c, "out", out, out_token, out_head)) return rc;
+    OnDevice on(c->device);
+    p.out = out; p.out_token = out_token; p.out_head = out_head; p.lse = lse;
+    LK_CU(launch_tree(p, cache->dtype, c->nsm, (cudaStream_t)stream));
+    return LK_OK;
+}
+
+int lk_attn_mass(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H, const int* starts,
+                 const uint64_t* tree, float scale, const float* lse, const float* weight, float decay, lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    TreeParams p{};
+    if (int rc = tree_params(c, cache, q, q_token, q_head, T, H, starts, tree, scale, &p)) return rc;
+    if (!p.kv.mass) return set_err(c, LK_ERR_ARG, "the cache has no mass array");
+    if (!(decay >= 0.0f && decay <= 1.0f)) return set_err(c, LK_ERR_ARG, "decay must be in [0, 1]");
+    if (T == 0) return LK_OK;
+    if (!lse) return set_err(c, LK_ERR_ARG, "null lse");
+    OnDevice on(c->device);
+    p.lse = const_cast<float*>(lse); p.weight = weight; p.decay = decay;
+    LK_CU(launch_mass(p, cache->dtype, c->nsm, (cudaStream_t)stream));
+    return LK_OK;
+}
+
+int lk_attn_evict(LkAttnCtx* c, const LkKvCache* cache, int budget, int sinks, int recent, const int* next_pos, int* new_lens,
+                  lk_stream_t stream) {
+    if (!c) return LK_ERR_ARG;
+    EvictParams p{};
+    if (int rc = check_cache(c, cache, &p.kv)) return rc;
+    if (!p.kv.mass || !p.kv.pos) return set_err(c, LK_ERR_ARG, "eviction needs the cache's mass and pos");
+    if (budget < 1 || sinks < 0 || recent < 0) return set_err(c, LK_ERR_ARG, "budget %d, sinks %d, recent %d", budget, sinks, recent);
+    if (!next_pos || !new_lens) return set_err(c, LK_ERR_ARG, "null next_pos or new_lens");
+    OnDevice on(c->device);
+    const int64_t cap = (int64_t)p.kv.table_stride * p.kv.page_size;
+    p.region = cap > budget ? (cap - budget < budget ? cap - budget : budget) : 0;      // most rows that one sequence can move
+    const int64_t need = 2 * p.region * p.kv.n_seqs;
+    if (need > c->moves_cap) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        LK_CU(cudaStreamIsCapturing((cudaStream_t)stream, &cs));
+        if (cs != cudaStreamCaptureStatusNone) return set_err(c, LK_ERR_CAPACITY, "the move list grows on first use: call once before the capture");
+        LK_CU(cudaFree(c->moves));
+        c->moves = nullptr; c->moves_cap = 0;
+        LK_CU(cudaMalloc((void**)&c->moves, need * sizeof(int)));
+        c->moves_cap = need;
+    }
+    p.budget = budget; p.sinks = sinks; p.recent = recent; p.next_pos = next_pos; p.new_lens = new_lens;
+    p.src = c->moves; p.dst = c->moves + p.region * p.kv.n_seqs; p.n_moves = c->n_moves; p.err = c->err;
+    LK_CU(launch_evict(p, c->nsm, (cudaStream_t)stream));
+    return LK_OK;
+}
+
+}  // extern "C"

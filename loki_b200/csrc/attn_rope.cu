@@ -1,0 +1,201 @@
+// attn_rope.cu -- rotary positions on part of a head, and the rotate-and-append of new rows to the paged latent cache.
+//
+// y_a = m (cos t x_a - sin t x_b), y_b = m (sin t x_a + cos t x_b) for the pair (a, b) = (2i, 2i+1) (interleaved) or
+// (i, i + R/2) (half), t = pos * f_i; the transpose (the gradient) negates sin.  Both only move data: 3 operations
+// per rotated value against one load and one store, so HBM (or, for a decode step's few KB, the launch) bounds them.
+// cos and sin come from a table made once in 64 bits: an fp32 product pos * f_i is off by half an ulp of the angle,
+// 4e-3 at position 1e5, and sin/cos in the kernel would cost more than the rotation.
+#include <math.h>
+#include "attn_internal.h"
+
+namespace lk {
+
+// N elements of T moved as one 4-, 8- or 16-byte access
+template <class T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+
+// ---------------------------------------------------------------- table
+__global__ void __launch_bounds__(256) k_rope_table(LkRopeConfig c, double lo, double hi, int max_pos, float2* __restrict__ table) {
+    const int half = c.rot_dim / 2;
+    const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (idx >= (int64_t)max_pos * half) return;
+    const int i = (int)(idx % half);
+    double f = pow(c.base, -2.0 * i / c.rot_dim);
+    if (c.factor > 1.0) {
+        const double r = fmin(fmax((i - lo) / fmax(hi - lo, 1e-3), 0.0), 1.0);
+        f = f * (1.0 - r) + f / c.factor * r;
+    }
+    double s, co;
+    sincos((double)(idx / half) * f, &s, &co);
+    table[idx] = make_float2((float)(co * c.mscale), (float)(s * c.mscale));
+}
+
+cudaError_t launch_rope_table(const LkRopeConfig& c, int max_pos, float2* table, cudaStream_t st) {
+    double lo = 0, hi = 0;
+    if (c.factor > 1.0) {       // the (real) frequency index that makes `turns` turns over the original context
+        auto at = [&](double turns) { return c.rot_dim * log(c.orig_ctx / (turns * 2 * M_PI)) / (2 * log(c.base)); };
+        lo = fmax(0.0, floor(at(c.beta_fast)));
+        hi = fmin(c.rot_dim - 1.0, ceil(at(c.beta_slow)));
+    }
+    const int64_t n = (int64_t)max_pos * (c.rot_dim / 2);
+    k_rope_table<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(c, lo, hi, max_pos, table);
+    return cudaGetLastError();
+}
+
+__device__ __forceinline__ int checked_pos(int pos, int max_pos, int* err) {
+    if ((unsigned)pos < (unsigned)max_pos) return pos;
+    att_error(err, ATT_ERR_POS);
+    return pos < 0 ? 0 : max_pos - 1;
+}
+
+// V pairs: interleaved, a holds the first V elements of 2V consecutive ones and b the rest; half, a and b are the
+// pairs' two sides
+template <int V, int LAYOUT>
+__device__ __forceinline__ void rotate(float (&a)[V], float (&b)[V], const float2* __restrict__ cs, float sign) {
+    #pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float2 t = __ldg(cs + i);
+        const float s = sign * t.y;
+        if (LAYOUT == LK_ROPE_HALF) {
+            const float x = a[i], y = b[i];
+            a[i] = t.x * x - s * y;
+            b[i] = s * x + t.x * y;
+        } else {
+            float& p = 2 * i < V ? a[2 * i] : b[2 * i - V];
+            float& q = 2 * i + 1 < V ? a[2 * i + 1] : b[2 * i + 1 - V];
+            const float x = p, y = q;
+            p = t.x * x - s * y;
+            q = s * x + t.x * y;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- rope
+// A unit is V pairs of the rotated part, or V copied elements; V elements are one 16-byte access (V = 1 where the
+// head's geometry, a stride or a pointer is not a multiple of that).
+template <class T, int V, int LAYOUT>
+__global__ void __launch_bounds__(256) k_rope(RopeParams p, int units, int blocks_per_token) {
+    const int t = blockIdx.x / blocks_per_token;
+    const int idx = (blockIdx.x % blocks_per_token) * blockDim.x + threadIdx.x;
+    if (idx >= p.H * units) return;
+    const int h = idx / units, u = idx % units, rot_units = p.rot / 2 / V;
+    using Vt = Vec<T, V>;
+    const T* x = (const T*)p.x + t * p.x_token + h * p.x_head;
+    T* y = (T*)p.y + t * p.y_token + h * p.y_head;
+    if (u >= rot_units) {
+        int e = (u - rot_units) * V;
+        if (e >= p.off) e += p.rot;
+        *(Vt*)(y + e) = *(const Vt*)(x + e);
+        return;
+    }
+    const int ea = p.off + (LAYOUT == LK_ROPE_HALF ? u * V : 2 * u * V);
+    const int eb = ea + (LAYOUT == LK_ROPE_HALF ? p.rot / 2 : V);
+    const float2* cs = p.table + (int64_t)checked_pos(p.pos[t], p.max_pos, p.err) * (p.rot / 2) + u * V;
+    Vt va = *(const Vt*)(x + ea), vb = *(const Vt*)(x + eb);
+    float a[V], b[V];
+    #pragma unroll
+    for (int i = 0; i < V; ++i) { a[i] = to_f<T>(va.v[i]); b[i] = to_f<T>(vb.v[i]); }
+    rotate<V, LAYOUT>(a, b, cs, p.grad ? -1.0f : 1.0f);
+    #pragma unroll
+    for (int i = 0; i < V; ++i) { va.v[i] = from_f<T>(a[i]); vb.v[i] = from_f<T>(b[i]); }
+    *(Vt*)(y + ea) = va;
+    *(Vt*)(y + eb) = vb;
+}
+
+template <class T, int V>
+static cudaError_t rope_go(const RopeParams& p, int layout, cudaStream_t st) {
+    const int units = p.rot / 2 / V + (p.copy ? (p.head_dim - p.rot) / V : 0);
+    const int threads = p.H * units >= 256 ? 256 : (p.H * units + 31) / 32 * 32;
+    const int bpt = (p.H * units + threads - 1) / threads;
+    if (layout == LK_ROPE_HALF) k_rope<T, V, LK_ROPE_HALF><<<(unsigned)(p.T * bpt), threads, 0, st>>>(p, units, bpt);
+    else k_rope<T, V, LK_ROPE_INTERLEAVED><<<(unsigned)(p.T * bpt), threads, 0, st>>>(p, units, bpt);
+    return cudaGetLastError();
+}
+
+template <class T>
+static cudaError_t rope_type(const RopeParams& p, int layout, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = p.off % V == 0 && p.rot % (2 * V) == 0 && p.head_dim % V == 0 && p.x_token % V == 0 && p.x_head % V == 0 &&
+                      p.y_token % V == 0 && p.y_head % V == 0 && !(((uintptr_t)p.x | (uintptr_t)p.y) & 15);
+    return wide ? rope_go<T, V>(p, layout, st) : rope_go<T, 1>(p, layout, st);
+}
+
+cudaError_t launch_rope(const RopeParams& p, int dtype, int layout, cudaStream_t st) {
+    switch (dtype) {
+        case LK_DT_F32: return rope_type<float>(p, layout, st);
+        case LK_DT_F16: return rope_type<__half>(p, layout, st);
+        default: return rope_type<__nv_bfloat16>(p, layout, st);
+    }
+}
+
+// ---------------------------------------------------------------- append
+// One thread per 8 latent values (64 of them) or 8 rotated pairs (4): 68 units a token.
+constexpr int AP_UNITS = AT_LATENT / 8 + AT_ROPE / 16;
+
+template <class T> __device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
+    constexpr int N = 16 / sizeof(T);
+    #pragma unroll
+    for (int k = 0; k < 8 / N; ++k) {
+        const Vec<T, N> w = *(const Vec<T, N>*)(src + k * N);
+        #pragma unroll
+        for (int i = 0; i < N; ++i) v[k * N + i] = to_f<T>(w.v[i]);
+    }
+}
+template <class T> __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
+    Vec<T, 8> w;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) w.v[i] = from_f<T>(v[i]);
+    *(Vec<T, 8>*)dst = w;
+}
+
+template <class TI, class TO, int LAYOUT>
+__global__ void __launch_bounds__(256) k_append(AppendParams p) {
+    const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int t = (int)(idx / AP_UNITS), u = (int)(idx % AP_UNITS);
+    if (t >= p.T) return;
+    int b = 0;                                   // the sequence: last b with starts[b] <= t
+    for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
+        const int mid = (lo + hi) >> 1;
+        if (p.starts[mid] <= t) { b = mid; lo = mid + 1; } else hi = mid - 1;
+    }
+    const int i = t - p.starts[b];
+    if (i < 0 || t >= p.starts[b + 1]) { if (u == 0) att_error(p.err, ATT_ERR_TREE); return; }
+    const int slot = kv_slot(p.kv, b, kv_len(p.kv, b, p.err) + i, p.err);
+    if (slot < 0) return;
+    TO* row = (TO*)p.kv.rows + (int64_t)slot * p.kv.row_stride;
+    if (u < AT_LATENT / 8) {
+        float v[8];
+        load8<TI>((const TI*)p.latent + t * p.latent_ld + u * 8, v);
+        store8<TO>(row + u * 8, v);
+        if (u == 0) {
+            if (p.kv.pos) p.kv.pos[slot] = p.pos[t];
+            if (p.kv.mass) p.kv.mass[slot] = 0.0f;
+        }
+        return;
+    }
+    const int r = u - AT_LATENT / 8;
+    const int ea = LAYOUT == LK_ROPE_HALF ? 8 * r : 16 * r, eb = ea + (LAYOUT == LK_ROPE_HALF ? AT_ROPE / 2 : 8);
+    const TI* k = (const TI*)p.k_rope + t * p.rope_ld;
+    float a[8], c[8];
+    load8<TI>(k + ea, a);
+    load8<TI>(k + eb, c);
+    rotate<8, LAYOUT>(a, c, p.table + (int64_t)checked_pos(p.pos[t], p.max_pos, p.err) * (AT_ROPE / 2) + 8 * r, 1.0f);
+    store8<TO>(row + AT_LATENT + ea, a);
+    store8<TO>(row + AT_LATENT + eb, c);
+}
+
+template <class TI, class TO>
+static cudaError_t append_go(const AppendParams& p, int layout, cudaStream_t st) {
+    const unsigned grid = (unsigned)(((int64_t)p.T * AP_UNITS + 255) / 256);
+    if (layout == LK_ROPE_HALF) k_append<TI, TO, LK_ROPE_HALF><<<grid, 256, 0, st>>>(p);
+    else k_append<TI, TO, LK_ROPE_INTERLEAVED><<<grid, 256, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_append(const AppendParams& p, int in_dtype, int kv_dtype, int layout, cudaStream_t st) {
+    if (kv_dtype == LK_DT_F16)
+        return in_dtype == LK_DT_F32 ? append_go<float, __half>(p, layout, st) : append_go<__half, __half>(p, layout, st);
+    return in_dtype == LK_DT_F32 ? append_go<float, __nv_bfloat16>(p, layout, st)
+                                 : append_go<__nv_bfloat16, __nv_bfloat16>(p, layout, st);
+}
+
+}  // namespace lk

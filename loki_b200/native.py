@@ -1,4 +1,4 @@
-"""ctypes binding of libloki_moe.so (include/loki_moe.h, include/loki_fused_moe.h, include/loki_ep.h).
+"""ctypes binding of libloki_moe.so (include/loki_moe.h, include/loki_fused_moe.h, include/loki_ep.h, include/loki_attn.h).
 
 The library is the product: every call here goes straight to the CUDA kernels.  There is no CPU or
 PyTorch fallback; a missing library raises at first use.
@@ -27,6 +27,10 @@ GU_MATRIX_BYTES = {f: MOE_INTER * (HIDDEN // QK) * b for f, b in BLOCK_BYTES.ite
 EP_ROW_HDR_BYTES = 64
 EP_ROW_BYTES = EP_ROW_HDR_BYTES + HIDDEN + HIDDEN // 32 * 4   # 8 128: header, q8 codes, fp32 scales
 EP_MAX_RANKS = 8
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ATTN_LATENT, ATTN_ROPE, ATTN_ROW = 512, 64, 576
+ATTN_MAX_HEADS, ATTN_MAX_NODES, ATTN_MAX_SEQS = 128, 64, 1024
 EP_COMM_ID_BYTES = 128
 EP_IPC_HANDLE_BYTES = 64
 
@@ -53,6 +57,21 @@ class FLOut(ctypes.Structure):
 class FLMoeW(ctypes.Structure):
     _fields_ = [("gate_inp", ctypes.c_void_p), ("gate_f16", ctypes.c_int), ("probs_b", ctypes.c_void_p),
                 ("sh_gate", ctypes.c_void_p), ("sh_up", ctypes.c_void_p), ("sh_down", ctypes.c_void_p), ("sh_fmt", ctypes.c_int)]
+
+
+class LkAttnConfig(ctypes.Structure):
+    _fields_ = [("max_seqs", ctypes.c_int), ("max_tokens", ctypes.c_int)]
+
+
+class LkRopeConfig(ctypes.Structure):
+    _fields_ = [("rot_dim", ctypes.c_int), ("base", ctypes.c_double), ("factor", ctypes.c_double), ("orig_ctx", ctypes.c_int),
+                ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double), ("mscale", ctypes.c_double)]
+
+
+class LkKvCache(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("dtype", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("n_seqs", ctypes.c_int), ("lens", ctypes.c_void_p), ("mass", ctypes.c_void_p), ("pos", ctypes.c_void_p)]
 
 
 # exported symbol -> (restype, argtypes)
@@ -93,6 +112,16 @@ SIGNATURES = {
     "lk_ep_p2p_experts": (_I, [_P, _P, _P, _I, _I, _P, _P, _P]),
     "lk_ep_p2p_combine_entries": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P]),
     "lk_ep_p2p_route_dispatch": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "lk_attn_create": (_I, [ctypes.POINTER(LkAttnConfig), _I, ctypes.POINTER(_P)]),
+    "lk_attn_destroy": (None, [_P]),
+    "lk_attn_get_error": (_I, [_P, _P]),
+    "lk_attn_last_error": (ctypes.c_char_p, [_P]),
+    "lk_attn_rope_table": (_I, [_P, ctypes.POINTER(LkRopeConfig), _I, _P, _P]),
+    "lk_attn_rope": (_I, [_P, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P]),
+    "lk_attn_append": (_I, [_P, ctypes.POINTER(LkKvCache), _I, _P, _I64, _P, _I64, _I, _P, _P, _P, _I, _I, _P]),
+    "lk_attn_tree": (_I, [_P, ctypes.POINTER(LkKvCache), _P, _I64, _I64, _I, _I, _P, _P, _F, _P, _I64, _I64, _P, _P]),
+    "lk_attn_mass": (_I, [_P, ctypes.POINTER(LkKvCache), _P, _I64, _I64, _I, _I, _P, _P, _F, _P, _P, _F, _P]),
+    "lk_attn_evict": (_I, [_P, ctypes.POINTER(LkKvCache), _I, _I, _I, _P, _P, _P]),
     "fl_init": (_P, [_I, _I]),
     "fl_wide_init": (_I, [_P, _I, _I]),
     "fl_wide_moe": (None, [_P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I]),
@@ -142,10 +171,10 @@ def lib():
     return _lib
 
 
-def check(rc, ctx=None):
+def check(rc, ctx=None, last_error="lk_moe_last_error"):
     if rc != LK_OK:
         msg = lib().lk_moe_strerror(rc).decode()
         if ctx is not None:
-            msg += ": " + lib().lk_moe_last_error(ctx).decode()
+            msg += ": " + getattr(lib(), last_error)(ctx).decode()
         raise NativeError("loki_moe error %d (%s)" % (rc, msg))
     return rc
