@@ -73,7 +73,8 @@ LK_API int  lk_attn_get_error(LkAttnCtx* ctx, lk_stream_t stream);
 LK_API const char* lk_attn_last_error(LkAttnCtx* ctx);
 
 /* cos and sin of positions 0 .. max_pos-1 into table [max_pos][rot_dim/2][2] fp32; the angles are computed in 64
- * bits (an fp32 angle at position 1e5 is off by 4e-3) and reduced there */
+ * bits (an fp32 angle at position 1e5 is off by 4e-3) and reduced there.  On the current device; ctx may be null (it
+ * only takes the message of a refusal) */
 LK_API int lk_attn_rope_table(LkAttnCtx* ctx, const LkRopeConfig* cfg, int max_pos, float* table, lk_stream_t stream);
 
 /* y = x [T][H][head_dim] with elements [rot_offset, rot_offset + rot_dim) of every head rotated to position
@@ -103,7 +104,7 @@ LK_API int lk_attn_tree(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, i
                         float* lse, lk_stream_t stream);
 
 /* cache->mass[row k] = decay * mass + sum_t weight[t] * sum_h exp(scale * q . row_k - lse[t][h]) for every row of every
- * sequence (context and drafted), over the tokens that see it: the attention weight that lk_attn_tree gave it.  weight
+ * sequence (context and drafted), over the tokens that see it: the attention weight that lk_attn_tree gave it (sequences without tokens keep theirs).  weight
  * [T] (null: all 1; 0 for rejected drafts).  One owner adds each row's terms in a fixed order, so results repeat. */
 LK_API int lk_attn_mass(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H,
                         const int* starts, const uint64_t* tree, float scale, const float* lse, const float* weight,

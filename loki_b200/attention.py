@@ -50,10 +50,10 @@ class RopeTable:
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.max_pos, self.rot_dim = max_pos, rot_dim
-        ctx = AttnContext(device, 1, 1)
         self.table = torch.empty(max(max_pos, 0), max(rot_dim, 0) // 2, 2, device=device)
         cfg = N.LkRopeConfig(rot_dim, base, factor, orig_ctx, beta_fast, beta_slow, mscale)
-        ctx._check(lib().lk_attn_rope_table(ctx.ctx, ctypes.byref(cfg), max_pos, _ptr(self.table), _stream(stream)))
+        with torch.cuda.device(device):
+            check(lib().lk_attn_rope_table(None, ctypes.byref(cfg), max_pos, _ptr(self.table), _stream(stream)))
 
 
 class KvCache:

@@ -21,7 +21,7 @@ REPLAY_SRC = os.path.join(CSRC, "fl_replay.cpp")
 REPLAY_LIB = os.path.join(HERE, "libloki_replay.so")
 SOURCES = ["expert_gemv.cu", "expert_gemv1.cu", "aux_kernels.cu", "router.cu", "dispatch.cu", "prefill_gemm.cu", "gate_up_q8.cu", "moe_api.cu", "fl_abi.cu", "noalloc.cu", "ep.cu", "ep_comm.cu", "slot_mma.cu", "ep_p2p.cu", "expert_kq.cu", "shared_kq.cu", "shared_gemm.cu", "kq_mma.cu",
            "attn_api.cu", "attn_rope.cu", "attn_tree.cu", "attn_mass.cu", "attn_evict.cu"]
-HEADERS = ["moe_format.h", "moe_device.cuh", "moe_internal.h", "attn_internal.h", "ep_device.cuh", "tcgen05.cuh", "iq2_tc.cuh", "iq2_grid.inc",
+HEADERS = ["moe_format.h", "moe_device.cuh", "moe_internal.h", "attn_internal.h", "attn_sched.cuh", "attn_tc.cuh", "ep_device.cuh", "tcgen05.cuh", "iq2_tc.cuh", "iq2_grid.inc",
            os.path.join("..", "..", "include", "loki_moe.h"), os.path.join("..", "..", "include", "loki_fused_moe.h"),
            os.path.join("..", "..", "include", "loki_ep.h"), os.path.join("..", "..", "include", "loki_attn.h")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -3,6 +3,7 @@
 #include <cstdarg>
 #include <new>
 #include "attn_internal.h"
+#include "attn_sched.cuh"
 
 using namespace lk;
 
@@ -11,6 +12,7 @@ struct LkAttnCtx {
     int device = 0, nsm = 0;
     int* err = nullptr;
     int* n_moves = nullptr; int* moves = nullptr; int64_t moves_cap = 0;      // eviction: [2][n_seqs][region]
+    TreeWork work{};                                                          // lk_attn_tree: parts of split items
     char msg[256] = {0};
 };
 
@@ -31,6 +33,32 @@ struct OnDevice {
 }
 
 static bool is16(const void* p) { return p && !((uintptr_t)p & 15); }
+
+// the cache's rows as a tensor map: boxes of 64 values x up to 64 rows of one page, 128-byte swizzle
+static int encode_map(LkAttnCtx* c, const LkKvCache* k, CUtensorMap* map) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return ok ? (Encode)f : nullptr;
+    }();
+    if (!encode) return set_err(c, LK_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = { AT_ROW, (cuuint64_t)k->n_pages * k->page_size }, strides[1] = { (cuuint64_t)k->row_stride * 2 };
+    const cuuint32_t box[2] = { 64, (cuuint32_t)(k->page_size < 64 ? k->page_size : 64) }, step[2] = { 1, 1 };
+    const CUresult r = encode(map, k->dtype == LK_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, k->rows, dims, strides,
+                              box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? LK_OK : set_err(c, LK_ERR_CUDA, "cuTensorMapEncodeTiled: %d", (int)r);
+}
+
+// a workspace that is made on the first call that needs it; not inside a stream capture
+static int may_allocate(LkAttnCtx* c, cudaStream_t st) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    LK_CU(cudaStreamIsCapturing(st, &cs));
+    return cs == cudaStreamCaptureStatusNone ? LK_OK : set_err(c, LK_ERR_CAPACITY, "the first call makes its workspace: call once before the capture");
+}
 
 // the cache's fields, and what the kernels see of it
 static int check_cache(LkAttnCtx* c, const LkKvCache* k, KvView* v) {
@@ -83,7 +111,7 @@ int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
 void lk_attn_destroy(LkAttnCtx* c) {
     if (!c) return;
     OnDevice on(c->device);
-    void* ptrs[] = { c->err, c->n_moves, c->moves };
+    void* ptrs[] = { c->err, c->n_moves, c->moves, c->work.part };
     for (void* p : ptrs) if (p) cudaFree(p);
     delete c;
 }
@@ -105,13 +133,11 @@ int lk_attn_get_error(LkAttnCtx* c, lk_stream_t stream) {
 const char* lk_attn_last_error(LkAttnCtx* c) { return c ? c->msg : "null context"; }
 
 int lk_attn_rope_table(LkAttnCtx* c, const LkRopeConfig* cfg, int max_pos, float* table, lk_stream_t stream) {
-    if (!c) return LK_ERR_ARG;
     if (!cfg || !table || ((uintptr_t)table & 7)) return set_err(c, LK_ERR_ARG, "null config, or table null or not 8-byte aligned");
     if (cfg->rot_dim < 2 || cfg->rot_dim % 2 || cfg->rot_dim > 4096 || max_pos < 1 || max_pos > (1 << 26)) return set_err(c, LK_ERR_ARG, "rot_dim %d, max_pos %d", cfg->rot_dim, max_pos);
     if (!(cfg->base > 1.0) || !(cfg->factor >= 1.0) || !(cfg->mscale > 0.0)) return set_err(c, LK_ERR_ARG, "base must exceed 1, factor be at least 1, mscale positive");
     if (cfg->factor > 1.0 && (cfg->orig_ctx < 1 || !(cfg->beta_slow > 0.0) || !(cfg->beta_fast >= cfg->beta_slow)))
         return set_err(c, LK_ERR_ARG, "a stretched context needs orig_ctx and beta_fast >= beta_slow > 0");
-    OnDevice on(c->device);
     LK_CU(launch_rope_table(*cfg, max_pos, (float2*)table, (cudaStream_t)stream));
     return LK_OK;
 }
@@ -179,7 +205,16 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     if (int rc = check_rows(c, "out", out, out_token, out_head)) return rc;
     OnDevice on(c->device);
     p.out = out; p.out_token = out_token; p.out_head = out_head; p.lse = lse;
-    LK_CU(launch_tree(p, cache->dtype, c->nsm, (cudaStream_t)stream));
+    CUtensorMap map;
+    if (int rc = encode_map(c, cache, &map)) return rc;
+    if (!c->work.prefix) {                            // parts of at most two items per pair of SMs: 0.5 MB a pair
+        if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
+        const size_t slots = c->nsm / 2 * 2, part = slots * 128 * AT_LATENT * 4, ml = slots * 128 * 8, pre = (LK_ATTN_MAX_SEQS + 1) * 8;
+        void* w = nullptr;
+        LK_CU(cudaMalloc(&w, part + ml + pre));
+        c->work = TreeWork{ (float4*)w, (float2*)((char*)w + part), (int64_t*)((char*)w + part + ml) };
+    }
+    LK_CU(launch_tree(p, cache->dtype, map, c->work, c->nsm, (cudaStream_t)stream));
     return LK_OK;
 }
 
@@ -211,9 +246,7 @@ int lk_attn_evict(LkAttnCtx* c, const LkKvCache* cache, int budget, int sinks, i
     p.region = cap > budget ? (cap - budget < budget ? cap - budget : budget) : 0;      // most rows that one sequence can move
     const int64_t need = 2 * p.region * p.kv.n_seqs;
     if (need > c->moves_cap) {
-        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        LK_CU(cudaStreamIsCapturing((cudaStream_t)stream, &cs));
-        if (cs != cudaStreamCaptureStatusNone) return set_err(c, LK_ERR_CAPACITY, "the move list grows on first use: call once before the capture");
+        if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
         LK_CU(cudaFree(c->moves));
         c->moves = nullptr; c->moves_cap = 0;
         LK_CU(cudaMalloc((void**)&c->moves, need * sizeof(int)));

@@ -1,5 +1,6 @@
 // attn_internal.h -- parameter blocks, launchers and device helpers of the latent-cache attention operators.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
@@ -51,7 +52,8 @@ struct TreeParams {
     const float* weight; float decay;              // mass
     int* err;
 };
-cudaError_t launch_tree(const TreeParams& p, int dtype, int nsm, cudaStream_t st);
+struct TreeWork;                                   // attn_sched.cuh
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st);
 cudaError_t launch_mass(const TreeParams& p, int dtype, int nsm, cudaStream_t st);
 
 struct EvictParams {

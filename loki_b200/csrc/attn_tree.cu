@@ -1,108 +1,467 @@
 // attn_tree.cu -- attention of drafted token trees over the paged latent cache.
 //
-// S = scale * Q K^T with K the 576-wide rows, P = softmax(S) over the rows a token sees, O = P C with C the first 512
-// values of the same rows.  One pass over the cache with a running maximum m and sum l per row: on a new tile
-// m' = max(m, max S), O and l scale by exp(m - m'), P = exp(S - m').
+// S = scale * Q K^T with K the 576-wide rows, P = softmax(S) over the rows that a token sees, O = P C with C the first
+// 512 values of the same rows.  One pass over the cache with a running reference m and sum l per row: P = 2^(S' - m + 7)
+// (S' in units of log 2), and where a tile's maximum exceeds m by more than 8, m moves there and O and l are scaled.
 //
-// One CTA per (token, 16 heads): the rows of one token share its cache rows and its mask.  Keys in tiles of 32.
-#include "attn_internal.h"
+// Work.  A row is one (token, head); 128 rows of one sequence are an item, 128 cached rows a tile, and (item, tile) a
+// unit of work: 35.7 M products, 147 KB of cache.  All units, numbered item by item, are cut into equal runs, one per
+// pair of CTAs, whatever the batch's lengths; an item that lies in several runs leaves partial O, m and l for k_merge.
+// Lengths are read on the device, so a captured call follows them.
+//
+// Why a pair.  fp32 O is 128 x 512: all of one SM's tensor memory.  A pair halves the rows (2-CTA tcgen05.mma, M = 128:
+// 64 rows of each CTA in all 128 lanes), so O takes 256 columns and two S buffers 128, and Q 72 KB of shared memory.  Each
+// CTA loads half of a tile's rows for S (64 x 576) and half of the latent columns of all of them for O (128 x 256).
+// Measured on a B200, 2-CTA M = 128 runs at the full 4096 products per cycle and SM for N = 128 and 256 (one CTA with
+// M = 128, N = 128 reaches 2925), so a unit costs 2176 cycles of tensor pipe; 45 bytes per cycle and SM from L2 into all
+// SMs at once makes the 136 KB a CTA loads for it about 3100, which bounds calls with many rows.  Few rows are bound by
+// HBM: 74 pairs at 3100 cycles ask for 6.7 TB/s.
+//
+// Roles (256 threads a CTA): warp 0 loads (TMA, ring of 7 x 16 KB), warp 1 of CTA 0 issues all MMAs, warps 2-3 repair
+// tail tiles, warps 4-7 do softmax, O's scaling and the output.  Order of the MMAs and of the ring: S(0), S(1), O(0),
+// S(2), O(1), ..: softmax j runs under S(j + 1).
+//
+// Rows that must not matter: a tile's rows beyond the drafts, and drafted rows that a token does not see, get P = 0; but
+// 0 * NaN is NaN, so warps 2-3 zero the former in the O operand, and every drafted row there that holds a non-finite
+// value (a token that does see it gets its NaN through S and P).
+#include <type_traits>
+#include "attn_tc.cuh"
+#include "attn_sched.cuh"
+#include "moe_internal.h"
 
 namespace lk {
 
-constexpr int TS_H = 16, TS_K = 32, TS_THREADS = 256;
-constexpr int TS_SMEM = TS_H * AT_ROW * 4 + TS_K * (AT_ROW + 2) * 4 + TS_H * (TS_K + 1) * 4 + 3 * TS_H * 4 + TS_K * 4;
+constexpr int TR_THREADS = 256, TR_STAGES = 7, TR_STAGE = 16384, TR_CHUNK = 8192;
+constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + 2 * TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
+constexpr int TR_XCH = TR_BARS + 40 * 8, TR_SCHED = TR_XCH + 128 * 4;
+constexpr int TR_SMEM = TR_SCHED + (LK_ATTN_MAX_SEQS + 1) * 8;
+static_assert(TR_SMEM <= 232448, "227 KB a CTA");
+constexpr uint32_t TR_S_COL = 256, TR_TMEM = 512;
+constexpr float TR_SHIFT = 7.0f, TR_JUMP = 8.0f;      // P <= 2^15 fits fp16; its smallest normal is 2^-21 of the reference
+
+struct TreeBars {
+    uint64_t full[TR_STAGES], empty[TR_STAGES], land[TR_STAGES];
+    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], q_full, drain;
+    uint32_t tmem;
+    int gave_up;
+};
+static_assert(sizeof(TreeBars) <= 40 * 8, "barrier block");
 
 template <class T>
-__global__ void __launch_bounds__(TS_THREADS) k_tree(TreeParams p) {
-    extern __shared__ float sm[];
-    float* Q = sm;                                   // [16][576]
-    float* K = Q + TS_H * AT_ROW;                    // [32][578]
-    float* P = K + TS_K * (AT_ROW + 2);              // [16][33]
-    float* M = P + TS_H * (TS_K + 1);                // running maximum, sum, and this tile's rescale
-    float* L = M + TS_H;
-    float* F = L + TS_H;
-    int* slot = (int*)(F + TS_H);
-    const int t = blockIdx.x, h0 = blockIdx.y * TS_H, tid = threadIdx.x;
-    int b = -1, len = 0, j = 0, n = 0;
-    for (int s = 0; s < p.kv.n_seqs; ++s) {
-        if (t < p.starts[s] || t >= p.starts[s + 1]) continue;
-        len = kv_len(p.kv, s, p.err);
-        const int2 sp = seq_tokens(p.starts, s, p.T, len, p.kv, p.err);
-        if (sp.y) { b = s; j = t - sp.x; n = sp.y; }
-        break;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TR_THREADS, 1)
+k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, TreeWork wk) {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    TreeBars& B = *(TreeBars*)(sm + TR_BARS);
+    float* xch = (float*)(sm + TR_XCH);
+    int64_t* prefix = (int64_t*)(sm + TR_SCHED);
+    volatile int* gave_up = &B.gave_up;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+
+    if (tid == 0) {
+        B.gave_up = 0;
+        for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], 1); mbar_init(&B.land[s], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 8); mbar_init(&B.p_full[i], 8); mbar_init(&B.o_done[i], 1); }
+        mbar_init(&B.q_full, 8);
+        mbar_init(&B.drain, 1);
+        fence_mbar_init();
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
-    if (b < 0 && tid == 0) att_error(p.err, ATT_ERR_TREE);
-    const uint64_t mask = b >= 0 ? node_mask(p.tree, t, j, n) : 0;
-    const int total = b >= 0 ? len + n : 0;
-    for (int i = tid; i < TS_H * AT_ROW; i += TS_THREADS) {
-        const int h = h0 + i / AT_ROW;
-        Q[i] = h < p.H ? to_f<T>(((const T*)p.q)[t * p.q_token + h * p.q_head + i % AT_ROW]) : 0.0f;
-    }
-    if (tid < TS_H) { M[tid] = -INFINITY; L[tid] = 0.0f; }
-    float o[TS_H][2];
-    #pragma unroll
-    for (int h = 0; h < TS_H; ++h) o[h][0] = o[h][1] = 0.0f;
-    for (int k0 = 0; k0 < total; k0 += TS_K) {
-        __syncthreads();
-        if (tid < TS_K) {
-            const int i = k0 + tid;
-            const bool see = i < len || (i < total && ((mask >> (i - len)) & 1));
-            slot[tid] = see ? kv_slot(p.kv, b, i, p.err) : -1;
-        }
-        __syncthreads();
-        for (int i = tid; i < TS_K * AT_ROW; i += TS_THREADS) {
-            const int r = i / AT_ROW, c = i % AT_ROW;
-            K[r * (AT_ROW + 2) + c] = slot[r] < 0 ? 0.0f : to_f<T>(((const T*)p.kv.rows)[(int64_t)slot[r] * p.kv.row_stride + c]);
-        }
-        __syncthreads();
-        for (int i = tid; i < TS_H * TS_K; i += TS_THREADS) {
-            const int h = i / TS_K, r = i % TS_K;
-            float s = 0.0f;
-            for (int c = 0; c < AT_ROW; ++c) s += Q[h * AT_ROW + c] * K[r * (AT_ROW + 2) + c];
-            P[h * (TS_K + 1) + r] = slot[r] < 0 ? -INFINITY : s * p.scale;
-        }
-        __syncthreads();
-        if (tid < TS_H) {
-            float m = M[tid];
-            for (int r = 0; r < TS_K; ++r) m = fmaxf(m, P[tid * (TS_K + 1) + r]);
-            const float f = m == -INFINITY ? 1.0f : expf(M[tid] - m);
-            float l = L[tid] * f;
-            for (int r = 0; r < TS_K; ++r) {
-                const float s = P[tid * (TS_K + 1) + r], e = s == -INFINITY ? 0.0f : expf(s - m);
-                P[tid * (TS_K + 1) + r] = e;
-                l += e;
-            }
-            M[tid] = m; L[tid] = l; F[tid] = f;
-        }
-        __syncthreads();
-        #pragma unroll
-        for (int h = 0; h < TS_H; ++h) { o[h][0] *= F[h]; o[h][1] *= F[h]; }
-        for (int r = 0; r < TS_K; ++r) {
-            const float c0 = K[r * (AT_ROW + 2) + 2 * tid], c1 = K[r * (AT_ROW + 2) + 2 * tid + 1];
-            #pragma unroll
-            for (int h = 0; h < TS_H; ++h) { o[h][0] += P[h * (TS_K + 1) + r] * c0; o[h][1] += P[h * (TS_K + 1) + r] * c1; }
-        }
-    }
+    if (warp == 2) tmem_alloc2(&B.tmem, TR_TMEM);
+    sched_prefix<ATT_TILE>(p, prefix, tid, TR_THREADS);
+    tc_fence_before();
     __syncthreads();
-    for (int h = 0; h < TS_H && h0 + h < p.H; ++h) {
-        const float l = L[h], inv = l == 0.0f ? 0.0f : 1.0f / l;
-        T* out = (T*)p.out + t * p.out_token + (h0 + h) * p.out_head;
-        out[2 * tid] = from_f<T>(o[h][0] * inv);
-        out[2 * tid + 1] = from_f<T>(o[h][1] * inv);
-        if (tid == 0 && p.lse) p.lse[(int64_t)t * p.H + h0 + h] = l == 0.0f ? -INFINITY : M[h] + logf(l);
+    cluster_sync();
+    tc_fence_after();
+    pdl_trigger();
+    const uint32_t tmem = B.tmem;
+    const int64_t W = prefix[p.kv.n_seqs];
+    if (blockIdx.x == 0) for (int i = tid; i <= p.kv.n_seqs; i += TR_THREADS) wk.prefix[i] = prefix[i];
+    const int used = sched_pairs(W, pairs);
+    const int64_t u_end = pair < used ? W * (pair + 1) / used : 0;
+    int64_t u = pair < used ? W * pair / used : 0;
+    const uint32_t smb = smem_u32(sm);
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- loads
+        const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0), land0 = smem_u32(&B.land[0]);
+        const int box = min(p.kv.page_size, 64), boxes = 64 / box;
+        uint32_t st = 0, ph = 1;                          // empty barriers start free
+        bool ok = true;
+        for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+            // pool row of 16-row group `lane` (of 8) of tile j; groups beyond the drafts read the last one's page again
+            auto rows_of = [&](int j) {
+                const int i = min(j * ATT_TILE + (lane & 7) * 16, (g.total - 1) & ~15);
+                const int slot = kv_slot(p.kv, g.b, i, p.err);
+                return slot < 0 ? 0 : slot;
+            };
+            auto acquire = [&]() { return wait_phase(&B.empty[st], ph, gave_up, p.err); };
+            auto advance = [&]() { if (++st == TR_STAGES) { st = 0; ph ^= 1; } };
+            int row_k = rows_of(g.t0), row_v = 0;
+            for (int j = g.t0; ok && j <= g.t1; ++j) {    // K of tile j, then V of tile j - 1
+                if (j < g.t1) {
+                    for (int s = 0; s < 5 && ok; ++s) {
+                        if (!(ok = acquire())) break;
+                        const int chunks = s < 4 ? 2 : 1;
+                        if (lane == 0) arrive_expect_at(full0 + 8 * st, chunks * TR_CHUNK);
+                        for (int c = 0; c < chunks; ++c)
+                            for (int x = 0; x < boxes; ++x) {
+                                const int row = __shfl_sync(0xffffffffu, row_k, (int)rank * 4 + x * (box / 16));
+                                if (lane == 0)
+                                    tma_2d_pair(smb + TR_RING + st * TR_STAGE + c * TR_CHUNK + x * box * 128, &kv_map, (2 * s + c) * 64, row, full0 + 8 * st);
+                            }
+                        advance();
+                    }
+                }
+                if (j > g.t0) {
+                    const bool tail = j * ATT_TILE > g.len;              // tile j - 1 reaches beyond the context
+                    for (int s = 0; s < 4 && ok; ++s) {                  // column group s / 2, row half s % 2
+                        if (!(ok = acquire())) break;
+                        const uint32_t bar = tail ? land0 + 8 * st : full0 + 8 * st;
+                        if (lane == 0) {
+                            if (tail) mbar_arrive_expect_tx(&B.land[st], TR_STAGE);
+                            else arrive_expect_at(bar, TR_STAGE);
+                        }
+                        for (int c = 0; c < 2; ++c)
+                            for (int x = 0; x < boxes; ++x) {
+                                const int row = __shfl_sync(0xffffffffu, row_v, (s & 1) * 4 + x * (box / 16));
+                                if (lane == 0)
+                                    tma_2d_pair(smb + TR_RING + st * TR_STAGE + c * TR_CHUNK + x * box * 128, &kv_map,
+                                                (s >> 1) * 256 + (int)rank * 128 + c * 64, row, bar);
+                            }
+                        advance();
+                    }
+                }
+                row_v = row_k;
+                if (j + 1 < g.t1) row_k = rows_of(j + 1);
+            }
+        }
+        if (!ok) __nanosleep(1000000);                    // given up: the loads in flight land before the CTA ends
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both
+        if (rank == 0) {
+            constexpr uint32_t id_s = att_idesc(128, 128, BF, false), id_o = att_idesc(128, 256, BF, true);
+            uint32_t st = 0, ph = 0, n_s = 0, n_o = 0, n_q = 0;          // stages, S tiles, O tiles and segments so far
+            bool ok = true, any = false;
+            auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_phase(bar, parity, gave_up, p.err)); tc_fence_after(); return ok; };
+            for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+                if (!wait(&B.q_full, n_q & 1)) break;
+                ++n_q;
+                for (int j = g.t0; ok && j <= g.t1; ++j) {
+                    if (j < g.t1) {
+                        const uint32_t buf = n_s & 1;
+                        if (!wait(&B.s_free[buf], ((n_s >> 1) & 1) ^ 1)) break;
+                        for (int s = 0; s < 5; ++s) {
+                            if (!wait(&B.full[st], ph)) break;
+                            const uint32_t kb = smb + TR_RING + st * TR_STAGE;
+                            for (int c = 0; c < (s < 4 ? 2 : 1); ++c)
+                                #pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    umma2_warp(tmem + TR_S_COL + buf * 64, sw128_desc(smb + TR_Q + (2 * s + c) * TR_CHUNK + k * 32, 16),
+                                               sw128_desc(kb + c * TR_CHUNK + k * 32, 16), id_s, (s | c | k) != 0);
+                            commit2_warp(&B.empty[st]);
+                            if (++st == TR_STAGES) { st = 0; ph ^= 1; }
+                        }
+                        any = true;
+                        if (!ok) break;
+                        commit2_warp(&B.s_full[buf]);
+                        ++n_s;
+                    }
+                    if (j > g.t0) {
+                        const uint32_t buf = n_o & 1;
+                        if (!wait(&B.p_full[buf], (n_o >> 1) & 1)) break;
+                        for (int s = 0; s < 4; ++s) {
+                            if (!wait(&B.full[st], ph)) break;
+                            const uint32_t vb = smb + TR_RING + st * TR_STAGE, pb = smb + TR_P + buf * TR_STAGE + (s & 1) * TR_CHUNK;
+                            #pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                umma2_warp(tmem + (s >> 1) * 128, sw128_desc(pb + k * 32, 16), sw128_desc(vb + k * 2048, TR_CHUNK), id_o,
+                                           j - 1 > g.t0 || (s & 1) || k);
+                            commit2_warp(&B.empty[st]);
+                            if (++st == TR_STAGES) { st = 0; ph ^= 1; }
+                        }
+                        if (!ok) break;
+                        commit2_warp(&B.o_done[buf]);
+                        ++n_o;
+                    }
+                }
+            }
+            if (!ok && any) { commit2_warp(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
+        }
+    } else if (warp < 4) {
+        // ---------------------------------------------------------------- repair of the O operand's tail tiles
+        const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
+        const int ft = tid - 64;
+        uint32_t st = 0, uses = 0;                        // bit s: parity of the uses of land[s]
+        bool ok = true;
+        auto advance = [&](int n) { st = (st + n) % TR_STAGES; };
+        for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+            for (int j = g.t0; ok && j <= g.t1; ++j) {
+                if (j < g.t1) advance(5);
+                if (j == g.t0) continue;
+                if (j * ATT_TILE <= g.len) { advance(4); continue; }
+                for (int s = 0; s < 4; ++s) {
+                    ok = !named_bar_or(2, 64, !wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err));
+                    if (!ok) break;
+                    uses ^= 1u << st;
+                    // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each; one thread per row
+                    const int i = (j - 1) * ATT_TILE + (s & 1) * 64 + ft;
+                    if (i >= g.len) {
+                        uint4* r = (uint4*)(sm + TR_RING + st * TR_STAGE + ft * 128);
+                        bool bad = i >= g.total;
+                        if (!bad) {
+                            uint32_t hit = 0;             // a 16-bit value whose exponent bits are all ones
+                            #pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                const uint4 v = r[(c >> 3) * (TR_CHUNK / 16) + ((c + ft) & 7)];
+                                hit |= nonfinite2<T>(v.x) | nonfinite2<T>(v.y) | nonfinite2<T>(v.z) | nonfinite2<T>(v.w);
+                            }
+                            bad = hit != 0;
+                        }
+                        // a row's two blocks and its two column groups are judged each by itself: all that matters is
+                        // that nothing non-finite is multiplied by 0
+                        if (bad)
+                            #pragma unroll
+                            for (int c = 0; c < 16; ++c) r[(c >> 3) * (TR_CHUNK / 16) + ((c + ft) & 7)] = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async_smem();
+                    named_bar_sync(2, 64);
+                    if (ft == 0) arrive_at(full0 + 8 * st);
+                    advance(1);
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax, O's scaling, output
+        const int L = tid - 128, row = L & 63, half = L >> 6;
+        const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_free0 = peer_addr(smem_u32(&B.s_free[0]), 0), p_full0 = peer_addr(smem_u32(&B.p_full[0]), 0),
+                       q_full0 = peer_addr(smem_u32(&B.q_full), 0);
+        const float scale2 = p.scale * 1.4426950408889634f;
+        uint32_t n = 0;                                   // tiles so far
+        bool ok = true, first_seg = true;
+        // every thread of the group gets the same answer
+        auto wait = [&](uint64_t* bar, uint32_t parity) { ok = !named_bar_or(1, 128, !wait_phase(bar, parity, gave_up, p.err)); tc_fence_after(); return ok; };
+        for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+            // ---- Q: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values
+            const int r0 = g.rt * 128 + (int)rank * 64, rows = g.n * p.H;
+            for (int i = L; i < 64 * 72; i += 128) {
+                const int r = i / 72, c = i % 72, gr = r0 + r;
+                const uint32_t dst = smb + TR_Q + (c >> 3) * TR_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                const int tj = gr < rows ? gr / p.H : 0;
+                const T* src = (const T*)p.q + (int64_t)(g.first + tj) * p.q_token + (int64_t)(gr < rows ? gr - tj * p.H : 0) * p.q_head + c * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(gr < rows ? 16 : 0) : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_at(q_full0);
+            const int gr = r0 + row, tj = gr / p.H;
+            const bool live = gr < rows;
+            const uint64_t mask = live ? node_mask(p.tree, g.first + tj, tj, g.n) : 0;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = g.t0; j < g.t1; ++j, ++n) {
+                const uint32_t buf = n & 1;
+                if (!wait(&B.s_full[buf], (n >> 1) & 1)) break;
+                float s[64];
+                {
+                    uint32_t a[32], b[32];
+                    tmem_ld32(tmem + lane_base + TR_S_COL + buf * 64, a);
+                    tmem_ld32(tmem + lane_base + TR_S_COL + buf * 64 + 32, b);
+                    tmem_wait_ld();
+                    #pragma unroll
+                    for (int i = 0; i < 32; ++i) { s[i] = __uint_as_float(a[i]); s[32 + i] = __uint_as_float(b[i]); }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_at(s_free0 + 8 * buf);
+                const int base = j * ATT_TILE + half * 64 - g.len;        // drafted node of the first column
+                if (base > -64) {
+                    const uint64_t see = base >= 64 ? 0 : base >= 0 ? mask >> base : (mask << -base) | ((1ull << -base) - 1);
+                    #pragma unroll
+                    for (int i = 0; i < 64; ++i) if (!((see >> i) & 1)) s[i] = -INFINITY;
+                }
+                float mx[4] = { s[0], s[1], s[2], s[3] };
+                #pragma unroll
+                for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                if (named_bar_or(1, 128, top > m + TR_JUMP)) {
+                    xch[L] = top;
+                    named_bar_sync(1, 128);
+                    const float m1 = fmaxf(m, fmaxf(top, xch[L ^ 64]));
+                    const float f = m1 == m ? 1.0f : exp2_approx(m - m1);  // m = -inf: 0
+                    l *= f;
+                    m = m1;
+                    if (j > g.t0) {                       // O(j - 1) is complete: scale its 256 columns of this lane
+                        if (!wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
+                        for (int c = 0; c < 256; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(tmem + lane_base + c, o);
+                            tmem_wait_ld();
+                            #pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(tmem + lane_base + c, o);
+                        }
+                        tmem_wait_st();
+                        tc_fence_before();
+                    }
+                    named_bar_sync(1, 128);               // xch is free again
+                }
+                const float ref = (m == -INFINITY ? 0.0f : m) - TR_SHIFT;
+                if (j >= g.t0 + 2 && !wait(&B.o_done[buf], ((n - 2) >> 1) & 1)) break;      // O(j - 2) has read this P buffer
+                uint8_t* pr = sm + TR_P + buf * TR_STAGE + half * TR_CHUNK + row * 128;
+                float sum[4] = { 0, 0, 0, 0 };
+                #pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float e[8];
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) { e[i] = exp2_approx(fmaf(s[8 * c + i], scale2, -ref)); sum[i & 3] += e[i]; }
+                    *(uint4*)(pr + ((c ^ (row & 7)) << 4)) =
+                        make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive_at(p_full0 + 8 * buf);
+            }
+            if (!ok) break;
+            // ---- output: all of O, then the row's two half sums
+            if (!wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
+            xch[L] = l;
+            named_bar_sync(1, 128);
+            l += xch[L ^ 64];
+            named_bar_sync(1, 128);
+            if (g.whole) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int h = gr - tj * p.H, t = g.first + tj;
+                T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + half * 128;
+                for (int c = 0; c < 256; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem + lane_base + c, o);
+                    tmem_wait_ld();
+                    if (live)
+                        #pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 v;
+                            v.x = pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                            v.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                            v.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                            v.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                            *(uint4*)(out + (c & 128) * 2 + (c & 127) + i) = v;
+                        }
+                }
+                if (live && half == 0 && p.lse)
+                    p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+            } else {
+                const int slot = 2 * pair + !first_seg, pr = (int)rank * 64 + row;
+                float4* part = wk.part + (int64_t)slot * (128 * 128) + half * 32 * 128 + pr;
+                for (int c = 0; c < 256; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem + lane_base + c, o);
+                    tmem_wait_ld();
+                    if (live)
+                        #pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            part[((c & 128) / 2 + (c & 127) / 4 + i / 4) * 128] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                                                                                        __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                }
+                if (live && half == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
+            }
+            tc_fence_before();
+            first_seg = false;
+        }
     }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 2) { tc_fence_after(); tmem_dealloc2(tmem, TR_TMEM); }
+}
+
+// ---------------------------------------------------------------- joining split items
+// A CTA takes 4 rows of one token-and-head run x 64 latent values; 4 groups of 64 threads take every fourth part and their
+// sums are added in order.  Items that one pair finished were written by k_tree.
+constexpr int MG_ROWS = 4, MG_C4 = 16, MG_GROUPS = 4;
+
+template <class T>
+__global__ void __launch_bounds__(MG_ROWS * MG_C4 * MG_GROUPS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk, int pairs) {
+    __shared__ float4 acc[MG_GROUPS][MG_C4][MG_ROWS];
+    __shared__ float ls[MG_GROUPS][MG_ROWS];
+    pdl_wait();
+    const int64_t W = wk.prefix[p.kv.n_seqs];
+    if (W == 0) return;
+    const int used = sched_pairs(W, pairs);
+    const int rr = threadIdx.x % MG_ROWS, c4 = threadIdx.x / MG_ROWS % MG_C4, grp = threadIdx.x / (MG_ROWS * MG_C4);
+    const int64_t flat = (int64_t)blockIdx.x * MG_ROWS + rr;         // row t * H + h of the call
+    const int t = (int)(flat / p.H), h = (int)(flat % p.H), cg = blockIdx.y * MG_C4 + c4;
+    int p0 = 0, p1 = -1, pr = 0;
+    int64_t u0 = 0;
+    if (t < p.T) {
+        int b = 0;                                                   // last b with starts[b] <= t
+        for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
+            const int mid = (lo + hi) >> 1;
+            if (p.starts[mid] <= t) { b = mid; lo = mid + 1; } else hi = mid - 1;
+        }
+        const int64_t w = wk.prefix[b + 1] - wk.prefix[b];
+        const int n = p.starts[b + 1] - p.starts[b];
+        const int row = (t - p.starts[b]) * p.H + h;
+        if (w > 0 && row >= 0 && t < p.starts[b + 1]) {
+            const int tiles = (int)(w / ((n * p.H + 127) / 128));
+            u0 = wk.prefix[b] + (int64_t)(row / 128) * tiles;
+            p0 = sched_owner(u0, W, used);
+            p1 = sched_owner(u0 + tiles - 1, W, used);
+            pr = row % 128;
+        }
+    }
+    const bool split = p1 > p0;
+    if (!__syncthreads_or(split)) return;
+    float m = -INFINITY;
+    if (split) for (int q = p0; q <= p1; ++q) m = fmaxf(m, wk.ml[sched_slot(q, u0, W, used) * 128 + pr].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 a = make_float4(0, 0, 0, 0);
+    if (split) {
+        #pragma unroll 4
+        for (int q = p0 + grp; q <= p1; q += MG_GROUPS) {
+            const int slot = sched_slot(q, u0, W, used);
+            const float2 ml = wk.ml[slot * 128 + pr];
+            const float4 v = wk.part[(int64_t)slot * (128 * 128) + cg * 128 + pr];
+            // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
+            const float f = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - ref);
+            if (f != 0.0f) { l += f * ml.y; a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w; }
+        }
+    }
+    acc[grp][c4][rr] = a;
+    if (c4 == 0) ls[grp][rr] = l;
+    __syncthreads();
+    if (grp || !split) return;
+    l = 0.0f;
+    a = make_float4(0, 0, 0, 0);
+    #pragma unroll
+    for (int q = 0; q < MG_GROUPS; ++q) {
+        const float4 v = acc[q][c4][rr];
+        l += ls[q][rr]; a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + cg * 4;
+    *(uint2*)out = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+    if (cg == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
 }
 
 template <class T>
-static cudaError_t tree_go(const TreeParams& p, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TS_SMEM);
+static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
     if (e != cudaSuccess) return e;
-    k_tree<T><<<dim3(p.T, (p.H + TS_H - 1) / TS_H), TS_THREADS, TS_SMEM, st>>>(p);
-    return cudaGetLastError();
+    const int pairs = nsm / 2;
+    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const int64_t rows = (int64_t)p.T * p.H;
+    return launch_pdl_n(k_merge<T>, dim3((unsigned)((rows + MG_ROWS - 1) / MG_ROWS), AT_LATENT / 4 / MG_C4), dim3(MG_ROWS * MG_C4 * MG_GROUPS), 0, st, p, wk, pairs);
 }
 
-cudaError_t launch_tree(const TreeParams& p, int dtype, int, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? tree_go<__half>(p, st) : tree_go<__nv_bfloat16>(p, st);
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, wk, nsm, st) : tree_go<__nv_bfloat16>(p, map, wk, nsm, st);
 }
 
 }  // namespace lk
