@@ -18,23 +18,20 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Arrivals and waits have CTA scope: what they order is this CTA's shared memory, handed to the tensor core by
+// fence.proxy.async, or tensor memory, ordered by the tcgen05 fences.  With cluster scope each arrival cost ~700 cycles
+// and each wait ~150 on a B200 (a unit of work of k_tree 15 000 cycles).
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ void arrive_expect_at(uint32_t cluster_bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" :: "r"(cluster_bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return ok != 0;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" :: "r"(cluster_bar), "r"(bytes) : "memory");
 }
 // wait for the phase of `parity`; false once WAIT_LIMIT_NS passes (recorded) or another role has given up
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* err) {
-    for (int i = 0; i < 64; ++i) if (try_wait_cluster(bar, parity)) return true;
+    for (int i = 0; i < 64; ++i) if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long t0 = globaltimer_ns();
-    while (!try_wait_cluster(bar, parity)) {
+    while (!mbar_try_wait(bar, parity)) {
         if (*gave_up) return false;
         if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) { att_error(err, DEV_ERR_TIMEOUT_FULL); *gave_up = 1; return false; }
     }
@@ -50,24 +47,39 @@ __device__ __forceinline__ void tmem_alloc2(uint32_t* dst_smem, uint32_t ncols) 
 __device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(ncols) : "memory");
 }
-// whole warp, one elected lane issues
-__device__ __forceinline__ void umma2_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-// arrive on this barrier in both CTAs when every tcgen05.mma issued so far has completed
-__device__ __forceinline__ void commit2_warp(uint64_t* bar) {
-    asm volatile("{\n\t.reg .pred e;\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
-                 :: "r"(smem_u32(bar)) : "memory");
-}
-// operand tile of 128-byte rows with the 128-byte swizzle (8-row groups of 1 KB; 16-byte column c of row r at c ^ (r % 8)).
+// Operand tiles of 128-byte rows with the 128-byte swizzle (8-row groups of 1 KB; 16-byte column c of row r at c ^ (r % 8)).
 // K-major: row = M/N index, 64 16-bit values of K; a 16-deep K step is +32 bytes.
 // MN-major: row = K index, 64 values of M/N; blocks of 64 M/N values `lbo` bytes apart; a 16-deep K step is +2048 bytes.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr, uint32_t lbo) {
-    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
+// Descriptor: low word start >> 4 and lbo >> 4, high word 8-row stride, version and swizzle.
+constexpr uint32_t SW128_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t smem_addr, uint32_t lbo) { return ((smem_addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); }
+// true in one lane of a converged warp.  The single-thread roles branch on this: behind an ordinary lane test the compiler
+// cannot know that one thread is active and serialises every TMA and MMA over the possible ones (~200 cycles each).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e = 0;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t@p mov.u32 %0, 1;\n\t}" : "+r"(e));
+    return e != 0;
+}
+// four 16-deep K steps of D[tmem] (+)= A x B^T, A_STEP and B_STEP bytes apart; the first overwrites D where !accumulate
+template <uint32_t IDESC, uint32_t A_STEP, uint32_t B_STEP>
+__device__ __forceinline__ void umma2_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\t"
+                 "setp.ne.b32 p, %3, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+                 "mov.b64 ad, {%1, %4};\n\tmov.b64 bd, {%2, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, p;\n\t"
+                 "add.u32 al, %1, %6;\n\tadd.u32 bl, %2, %7;\n\tmov.b64 ad, {al, %4};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t"
+                 "add.u32 al, al, %6;\n\tadd.u32 bl, bl, %7;\n\tmov.b64 ad, {al, %4};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t"
+                 "add.u32 al, al, %6;\n\tadd.u32 bl, bl, %7;\n\tmov.b64 ad, {al, %4};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t}"
+                 :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(accumulate), "n"(SW128_HI), "n"(IDESC), "n"(A_STEP >> 4), "n"(B_STEP >> 4) : "memory");
+}
+// arrive on this barrier in both CTAs when every tcgen05.mma issued so far has completed
+__device__ __forceinline__ void commit2(uint64_t* bar) {
+    asm volatile("{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+                 "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
+                 :: "r"(smem_u32(bar)) : "memory");
 }
 __host__ __device__ constexpr uint32_t att_idesc(int M, int N, bool bf16, bool b_mn_major) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |

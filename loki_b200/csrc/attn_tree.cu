@@ -47,6 +47,66 @@ struct TreeBars {
 };
 static_assert(sizeof(TreeBars) <= 40 * 8, "barrier block");
 
+// the load role of one CTA, one thread: boxes of BOX rows x 64 values.  Its instructions are the loop's length (a loaded
+// stage feeds 512 cycles of MMAs), so the page lookups are made a tile ahead and nothing is computed per box.
+template <int BOX>
+__device__ __forceinline__ bool tree_load(const TreeParams& p, const int64_t* prefix, int64_t u, int64_t u_end, const CUtensorMap* map,
+                                          TreeBars& B, uint32_t smb, uint32_t rank) {
+    constexpr int NB = 64 / BOX;                          // boxes of 64 rows
+    const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
+    uint32_t st = 0, ph = 1, dst = smb + TR_RING, bar = full0;
+    auto advance = [&]() {
+        dst += TR_STAGE; bar += 8;
+        if (++st == TR_STAGES) { st = 0; ph ^= 1; dst = smb + TR_RING; bar = full0; }
+    };
+    for (Segment g; sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+        int next[2 * NB], k[2 * NB], v[2 * NB];           // pool rows of the boxes of tiles j + 1, j and j - 1
+        // boxes beyond the drafts read the last 16 rows' page again
+        auto rows_of = [&](int j) {
+            #pragma unroll
+            for (int x = 0; x < 2 * NB; ++x) next[x] = max(0, kv_slot(p.kv, g.b, min(j * ATT_TILE + x * BOX, (g.total - 1) & ~15), p.err));
+        };
+        rows_of(g.t0);
+        for (int j = g.t0; j <= g.t1; ++j) {              // K of tile j, then V of tile j - 1
+            #pragma unroll
+            for (int x = 0; x < 2 * NB; ++x) { v[x] = k[x]; k[x] = next[x]; }
+            if (j + 1 < g.t1) rows_of(j + 1);
+            if (j < g.t1) {
+                int mine[NB];
+                #pragma unroll
+                for (int x = 0; x < NB; ++x) mine[x] = rank ? k[NB + x] : k[x];
+                #pragma unroll
+                for (int s = 0; s < 5; ++s) {
+                    if (!wait_phase(&B.empty[st], ph, &B.gave_up, p.err)) return false;
+                    arrive_expect_at(bar, (s < 4 ? 2 : 1) * TR_CHUNK);
+                    #pragma unroll
+                    for (int c = 0; c < (s < 4 ? 2 : 1); ++c)
+                        #pragma unroll
+                        for (int x = 0; x < NB; ++x) tma_2d_pair(dst + c * TR_CHUNK + x * BOX * 128, map, (2 * s + c) * 64, mine[x], bar);
+                    advance();
+                }
+            }
+            if (j > g.t0) {
+                const bool tail = j * ATT_TILE > g.len;   // tile j - 1 reaches beyond the context: warps 2-3 pass it on
+                #pragma unroll
+                for (int s = 0; s < 4; ++s) {             // column group s / 2, row half s % 2
+                    if (!wait_phase(&B.empty[st], ph, &B.gave_up, p.err)) return false;
+                    uint32_t to = bar;
+                    if (tail) { to = smem_u32(&B.land[st]); mbar_arrive_expect_tx(&B.land[st], TR_STAGE); }
+                    else arrive_expect_at(bar, TR_STAGE);
+                    const int col = (s >> 1) * 256 + (int)rank * 128;
+                    #pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        #pragma unroll
+                        for (int x = 0; x < NB; ++x) tma_2d_pair(dst + c * TR_CHUNK + x * BOX * 128, map, col + c * 64, v[(s & 1) * NB + x], to);
+                    advance();
+                }
+            }
+        }
+    }
+    return true;
+}
+
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TR_THREADS, 1)
 k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, TreeWork wk) {
@@ -86,66 +146,19 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 
     if (warp == 0) {
         // ---------------------------------------------------------------- loads
-        const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0), land0 = smem_u32(&B.land[0]);
-        const int box = min(p.kv.page_size, 64), boxes = 64 / box;
-        uint32_t st = 0, ph = 1;                          // empty barriers start free
-        bool ok = true;
-        for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
-            // pool row of 16-row group `lane` (of 8) of tile j; groups beyond the drafts read the last one's page again
-            auto rows_of = [&](int j) {
-                const int i = min(j * ATT_TILE + (lane & 7) * 16, (g.total - 1) & ~15);
-                const int slot = kv_slot(p.kv, g.b, i, p.err);
-                return slot < 0 ? 0 : slot;
-            };
-            auto acquire = [&]() { return wait_phase(&B.empty[st], ph, gave_up, p.err); };
-            auto advance = [&]() { if (++st == TR_STAGES) { st = 0; ph ^= 1; } };
-            int row_k = rows_of(g.t0), row_v = 0;
-            for (int j = g.t0; ok && j <= g.t1; ++j) {    // K of tile j, then V of tile j - 1
-                if (j < g.t1) {
-                    for (int s = 0; s < 5 && ok; ++s) {
-                        if (!(ok = acquire())) break;
-                        const int chunks = s < 4 ? 2 : 1;
-                        if (lane == 0) arrive_expect_at(full0 + 8 * st, chunks * TR_CHUNK);
-                        for (int c = 0; c < chunks; ++c)
-                            for (int x = 0; x < boxes; ++x) {
-                                const int row = __shfl_sync(0xffffffffu, row_k, (int)rank * 4 + x * (box / 16));
-                                if (lane == 0)
-                                    tma_2d_pair(smb + TR_RING + st * TR_STAGE + c * TR_CHUNK + x * box * 128, &kv_map, (2 * s + c) * 64, row, full0 + 8 * st);
-                            }
-                        advance();
-                    }
-                }
-                if (j > g.t0) {
-                    const bool tail = j * ATT_TILE > g.len;              // tile j - 1 reaches beyond the context
-                    for (int s = 0; s < 4 && ok; ++s) {                  // column group s / 2, row half s % 2
-                        if (!(ok = acquire())) break;
-                        const uint32_t bar = tail ? land0 + 8 * st : full0 + 8 * st;
-                        if (lane == 0) {
-                            if (tail) mbar_arrive_expect_tx(&B.land[st], TR_STAGE);
-                            else arrive_expect_at(bar, TR_STAGE);
-                        }
-                        for (int c = 0; c < 2; ++c)
-                            for (int x = 0; x < boxes; ++x) {
-                                const int row = __shfl_sync(0xffffffffu, row_v, (s & 1) * 4 + x * (box / 16));
-                                if (lane == 0)
-                                    tma_2d_pair(smb + TR_RING + st * TR_STAGE + c * TR_CHUNK + x * box * 128, &kv_map,
-                                                (s >> 1) * 256 + (int)rank * 128 + c * 64, row, bar);
-                            }
-                        advance();
-                    }
-                }
-                row_v = row_k;
-                if (j + 1 < g.t1) row_k = rows_of(j + 1);
-            }
+        if (elect_one()) {
+            const bool ok = p.kv.page_size >= 64 ? tree_load<64>(p, prefix, u, u_end, &kv_map, B, smb, rank)
+                          : p.kv.page_size == 32 ? tree_load<32>(p, prefix, u, u_end, &kv_map, B, smb, rank)
+                                                 : tree_load<16>(p, prefix, u, u_end, &kv_map, B, smb, rank);
+            if (!ok) __nanosleep(1000000);                // given up: the loads in flight land before the CTA ends
         }
-        if (!ok) __nanosleep(1000000);                    // given up: the loads in flight land before the CTA ends
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both
-        if (rank == 0) {
+        if (rank == 0 && elect_one()) {
             constexpr uint32_t id_s = att_idesc(128, 128, BF, false), id_o = att_idesc(128, 256, BF, true);
             uint32_t st = 0, ph = 0, n_s = 0, n_o = 0, n_q = 0;          // stages, S tiles, O tiles and segments so far
             bool ok = true, any = false;
-            auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_phase(bar, parity, gave_up, p.err)); tc_fence_after(); return ok; };
+            auto wait = [&](uint64_t* bar, uint32_t parity) { ok = wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); return ok; };
             for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
                 if (!wait(&B.q_full, n_q & 1)) break;
                 ++n_q;
@@ -156,17 +169,15 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                         for (int s = 0; s < 5; ++s) {
                             if (!wait(&B.full[st], ph)) break;
                             const uint32_t kb = smb + TR_RING + st * TR_STAGE;
-                            for (int c = 0; c < (s < 4 ? 2 : 1); ++c)
-                                #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    umma2_warp(tmem + TR_S_COL + buf * 64, sw128_desc(smb + TR_Q + (2 * s + c) * TR_CHUNK + k * 32, 16),
-                                               sw128_desc(kb + c * TR_CHUNK + k * 32, 16), id_s, (s | c | k) != 0);
-                            commit2_warp(&B.empty[st]);
+                            const uint32_t qb = smb + TR_Q + 2 * s * TR_CHUNK, d = tmem + TR_S_COL + buf * 64;
+                            umma2_x4<id_s, 32, 32>(d, sw128_lo(qb, 16), sw128_lo(kb, 16), s != 0);
+                            if (s < 4) umma2_x4<id_s, 32, 32>(d, sw128_lo(qb + TR_CHUNK, 16), sw128_lo(kb + TR_CHUNK, 16), 1);
+                            commit2(&B.empty[st]);
                             if (++st == TR_STAGES) { st = 0; ph ^= 1; }
                         }
                         any = true;
                         if (!ok) break;
-                        commit2_warp(&B.s_full[buf]);
+                        commit2(&B.s_full[buf]);
                         ++n_s;
                     }
                     if (j > g.t0) {
@@ -175,20 +186,17 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                         for (int s = 0; s < 4; ++s) {
                             if (!wait(&B.full[st], ph)) break;
                             const uint32_t vb = smb + TR_RING + st * TR_STAGE, pb = smb + TR_P + buf * TR_STAGE + (s & 1) * TR_CHUNK;
-                            #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                umma2_warp(tmem + (s >> 1) * 128, sw128_desc(pb + k * 32, 16), sw128_desc(vb + k * 2048, TR_CHUNK), id_o,
-                                           j - 1 > g.t0 || (s & 1) || k);
-                            commit2_warp(&B.empty[st]);
+                            umma2_x4<id_o, 32, 2048>(tmem + (s >> 1) * 128, sw128_lo(pb, 16), sw128_lo(vb, TR_CHUNK), j - 1 > g.t0 || (s & 1));
+                            commit2(&B.empty[st]);
                             if (++st == TR_STAGES) { st = 0; ph ^= 1; }
                         }
                         if (!ok) break;
-                        commit2_warp(&B.o_done[buf]);
+                        commit2(&B.o_done[buf]);
                         ++n_o;
                     }
                 }
             }
-            if (!ok && any) { commit2_warp(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
+            if (!ok && any) { commit2(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
         }
     } else if (warp < 4) {
         // ---------------------------------------------------------------- repair of the O operand's tail tiles
@@ -245,22 +253,27 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         // every thread of the group gets the same answer
         auto wait = [&](uint64_t* bar, uint32_t parity) { ok = !named_bar_or(1, 128, !wait_phase(bar, parity, gave_up, p.err)); tc_fence_after(); return ok; };
         for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
-            // ---- Q: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values
-            const int r0 = g.rt * 128 + (int)rank * 64, rows = g.n * p.H;
-            for (int i = L; i < 64 * 72; i += 128) {
-                const int r = i / 72, c = i % 72, gr = r0 + r;
-                const uint32_t dst = smb + TR_Q + (c >> 3) * TR_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                const int tj = gr < rows ? gr / p.H : 0;
-                const T* src = (const T*)p.q + (int64_t)(g.first + tj) * p.q_token + (int64_t)(gr < rows ? gr - tj * p.H : 0) * p.q_head + c * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(gr < rows ? 16 : 0) : "memory");
+            // ---- Q: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 16 rows a warp, whose places in q the
+            // lanes that own the rows below know
+            const int gr = g.rt * 128 + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
+            const bool live = gr < g.n * p.H;
+            const int64_t q_at = live ? t * p.q_token + h * p.q_head : -1;
+            const int w4 = warp & 3;
+            #pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const int64_t at = __shfl_sync(0xffffffffu, q_at, (w4 >> 1) * 16 + i);
+                const int r = (w4 & 1) * 32 + (w4 >> 1) * 16 + i;
+                const T* src = (const T*)p.q + max(at, (int64_t)0);
+                #pragma unroll
+                for (int c = lane; c < 72; c += 32)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 :: "r"(smb + TR_Q + (c >> 3) * TR_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4)), "l"(src + c * 8), "r"(at < 0 ? 0 : 16) : "memory");
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
             __syncwarp();
             if (lane == 0) arrive_at(q_full0);
-            const int gr = r0 + row, tj = gr / p.H;
-            const bool live = gr < rows;
-            const uint64_t mask = live ? node_mask(p.tree, g.first + tj, tj, g.n) : 0;
+            const uint64_t mask = live ? node_mask(p.tree, t, tj, g.n) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int j = g.t0; j < g.t1; ++j, ++n) {
                 const uint32_t buf = n & 1;
@@ -335,7 +348,6 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             named_bar_sync(1, 128);
             if (g.whole) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int h = gr - tj * p.H, t = g.first + tj;
                 T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + half * 128;
                 for (int c = 0; c < 256; c += 32) {
                     uint32_t o[32];
