@@ -70,11 +70,9 @@ __device__ __forceinline__ bool sched_next(const TreeParams& p, const int64_t* p
 
 // runs that a call is cut into
 __host__ __device__ __forceinline__ int sched_pairs(int64_t W, int pairs) { return W < pairs ? (int)W : pairs; }
-// the run that has unit u: the last q with W q / used <= u
+// the run that has unit u: the last q with W q / used <= u.  A run leaves a part of its first item in slot 2 q and of its
+// last in 2 q + 1, so an item that starts inside run q has its first part in 2 q + 1 and the others in even slots
 __device__ __forceinline__ int sched_owner(int64_t u, int64_t W, int used) { return (int)(((u + 1) * used + W - 1) / W) - 1; }
-// where run q left its part of the item that starts at unit u0
-__device__ __forceinline__ int sched_slot(int q, int64_t u0, int64_t W, int used) { return 2 * q + (W * q / used < u0); }
-
 template <class T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t v);
 template <> __device__ __forceinline__ uint32_t nonfinite2<__half>(uint32_t v) { return (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u; }
 template <> __device__ __forceinline__ uint32_t nonfinite2<__nv_bfloat16>(uint32_t v) { return (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u; }

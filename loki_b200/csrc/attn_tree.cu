@@ -392,84 +392,103 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 }
 
 // ---------------------------------------------------------------- joining split items
-// A CTA takes 4 rows of one token-and-head run x 64 latent values; 4 groups of 64 threads take every fourth part and their
-// sums are added in order.  Items that one pair finished were written by k_tree.
-constexpr int MG_ROWS = 4, MG_C4 = 16, MG_GROUPS = 4;
+// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q.  A CTA takes 4 rows x 64 latent
+// values: the parts' factors once into shared memory, then 4 groups of 64 threads take every fourth part, added in order.
+// Items that one pair finished were written by k_tree.
+constexpr int MG_ROWS = 4, MG_C4 = 16, MG_GROUPS = 4, MG_THREADS = MG_ROWS * MG_C4 * MG_GROUPS, MG_PARTS = 128;
 
 template <class T>
-__global__ void __launch_bounds__(MG_ROWS * MG_C4 * MG_GROUPS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk, int pairs) {
+__global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk, int pairs) {
     __shared__ float4 acc[MG_GROUPS][MG_C4][MG_ROWS];
-    __shared__ float ls[MG_GROUPS][MG_ROWS];
+    __shared__ float f[MG_PARTS][MG_ROWS];
+    __shared__ int first[MG_ROWS], parts[MG_ROWS], at[MG_ROWS];      // slot of a row's first part (the others: even, 2 apart)
+    __shared__ float ref[MG_ROWS], sum[MG_ROWS];
     pdl_wait();
-    const int64_t W = wk.prefix[p.kv.n_seqs];
-    if (W == 0) return;
-    const int used = sched_pairs(W, pairs);
-    const int rr = threadIdx.x % MG_ROWS, c4 = threadIdx.x / MG_ROWS % MG_C4, grp = threadIdx.x / (MG_ROWS * MG_C4);
+    const int tid = threadIdx.x, rr = tid % MG_ROWS, c4 = tid / MG_ROWS % MG_C4, grp = tid / (MG_ROWS * MG_C4);
     const int64_t flat = (int64_t)blockIdx.x * MG_ROWS + rr;         // row t * H + h of the call
-    const int t = (int)(flat / p.H), h = (int)(flat % p.H), cg = blockIdx.y * MG_C4 + c4;
-    int p0 = 0, p1 = -1, pr = 0;
-    int64_t u0 = 0;
-    if (t < p.T) {
-        int b = 0;                                                   // last b with starts[b] <= t
-        for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
-            const int mid = (lo + hi) >> 1;
-            if (p.starts[mid] <= t) { b = mid; lo = mid + 1; } else hi = mid - 1;
+    const int t = (int)(flat / p.H), h = (int)(flat - (int64_t)t * p.H);
+    if (tid < MG_ROWS) {
+        int n = 0;
+        const int64_t W = wk.prefix[p.kv.n_seqs];
+        if (t < p.T && W > 0) {
+            int b = 0;                                               // last b with starts[b] <= t
+            for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
+                const int mid = (lo + hi) >> 1;
+                if (p.starts[mid] <= t) { b = mid; lo = mid + 1; } else hi = mid - 1;
+            }
+            const int64_t u_b = wk.prefix[b], w = wk.prefix[b + 1] - u_b;
+            const int t0 = p.starts[b], t1 = p.starts[b + 1], row = (t - t0) * p.H + h;
+            if (w > 0 && t >= t0 && t < t1) {
+                const int used = sched_pairs(W, pairs), items = ((t1 - t0) * p.H + ATT_ITEM - 1) / ATT_ITEM;
+                const int64_t tiles = w / items, u0 = u_b + row / ATT_ITEM * tiles;
+                const int q0 = sched_owner(u0, W, used);
+                n = sched_owner(u0 + tiles - 1, W, used) - q0 + 1;
+                first[rr] = 2 * q0 + (W * q0 / used < u0);
+                at[rr] = row % ATT_ITEM;
+            }
         }
-        const int64_t w = wk.prefix[b + 1] - wk.prefix[b];
-        const int n = p.starts[b + 1] - p.starts[b];
-        const int row = (t - p.starts[b]) * p.H + h;
-        if (w > 0 && row >= 0 && t < p.starts[b + 1]) {
-            const int tiles = (int)(w / ((n * p.H + 127) / 128));
-            u0 = wk.prefix[b] + (int64_t)(row / 128) * tiles;
-            p0 = sched_owner(u0, W, used);
-            p1 = sched_owner(u0 + tiles - 1, W, used);
-            pr = row % 128;
+        parts[rr] = n > 1 ? n : 0;
+    }
+    __syncthreads();
+    const int n = parts[rr];
+    if (!__syncthreads_or(n > 0)) return;
+    const int s0 = n ? first[rr] : 0, s1 = (s0 & ~1) + 2, pr = n ? at[rr] : 0;      // part i > 0: slot s1 + 2 (i - 1)
+    // the parts' references and sums, then their factors: one row per warp of the first four
+    if (tid < 32 * MG_ROWS) {
+        const int r = tid >> 5, lane = tid & 31, nr = parts[r];
+        if (nr) {
+            const int a0 = first[r], a1 = (a0 & ~1) + 2;
+            float m = -INFINITY, l = 0.0f;
+            for (int i = lane; i < nr; i += 32) m = fmaxf(m, wk.ml[(i ? a1 + 2 * (i - 1) : a0) * 128 + at[r]].x);
+            #pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float rf = m == -INFINITY ? 0.0f : m;
+            for (int i = lane; i < nr; i += 32) {
+                const float2 ml = wk.ml[(i ? a1 + 2 * (i - 1) : a0) * 128 + at[r]];
+                // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
+                const float v = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
+                f[i][r] = v;
+                l += v == 0.0f ? 0.0f : v * ml.y;
+            }
+            #pragma unroll
+            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (lane == 0) { ref[r] = rf; sum[r] = l; }
         }
     }
-    const bool split = p1 > p0;
-    if (!__syncthreads_or(split)) return;
-    float m = -INFINITY;
-    if (split) for (int q = p0; q <= p1; ++q) m = fmaxf(m, wk.ml[sched_slot(q, u0, W, used) * 128 + pr].x);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
+    __syncthreads();
     float4 a = make_float4(0, 0, 0, 0);
-    if (split) {
-        #pragma unroll 4
-        for (int q = p0 + grp; q <= p1; q += MG_GROUPS) {
-            const int slot = sched_slot(q, u0, W, used);
-            const float2 ml = wk.ml[slot * 128 + pr];
-            const float4 v = wk.part[(int64_t)slot * (128 * 128) + cg * 128 + pr];
-            // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
-            const float f = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - ref);
-            if (f != 0.0f) { l += f * ml.y; a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w; }
-        }
+    const int cg = blockIdx.y * MG_C4 + c4;
+    const float4* src = wk.part + cg * 128 + pr;
+    #pragma unroll 8
+    for (int i = grp; i < n; i += MG_GROUPS) {
+        const float4 v = __ldcg(src + (int64_t)(i ? s1 + 2 * (i - 1) : s0) * (128 * 128));
+        const float g = f[i][rr];
+        if (g != 0.0f) { a.x += g * v.x; a.y += g * v.y; a.z += g * v.z; a.w += g * v.w; }
     }
     acc[grp][c4][rr] = a;
-    if (c4 == 0) ls[grp][rr] = l;
     __syncthreads();
-    if (grp || !split) return;
-    l = 0.0f;
+    if (grp || !n) return;
     a = make_float4(0, 0, 0, 0);
     #pragma unroll
     for (int q = 0; q < MG_GROUPS; ++q) {
         const float4 v = acc[q][c4][rr];
-        l += ls[q][rr]; a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float l = sum[rr], inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + cg * 4;
     *(uint2*)out = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-    if (cg == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+    if (cg == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[rr] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
 }
 
 template <class T>
 static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
     if (e != cudaSuccess) return e;
-    const int pairs = nsm / 2;
+    const int pairs = nsm / 2 < MG_PARTS ? nsm / 2 : MG_PARTS;
     k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const int64_t rows = (int64_t)p.T * p.H;
-    return launch_pdl_n(k_merge<T>, dim3((unsigned)((rows + MG_ROWS - 1) / MG_ROWS), AT_LATENT / 4 / MG_C4), dim3(MG_ROWS * MG_C4 * MG_GROUPS), 0, st, p, wk, pairs);
+    return launch_pdl_n(k_merge<T>, dim3((unsigned)((rows + MG_ROWS - 1) / MG_ROWS), AT_LATENT / 4 / MG_C4), dim3(MG_THREADS), 0, st, p, wk, pairs);
 }
 
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
