@@ -17,9 +17,10 @@
 // SMs at once makes the 136 KB a CTA loads for it about 3100, which bounds calls with many rows.  Few rows are bound by
 // HBM: 74 pairs at 3100 cycles ask for 6.7 TB/s.
 //
-// Roles (256 threads a CTA): warp 0 loads (TMA, ring of 7 x 16 KB), warp 1 of CTA 0 issues all MMAs, warps 2-3 repair
-// tail tiles, warps 4-7 do softmax, O's scaling and the output.  Order of the MMAs and of the ring: S(0), S(1), O(0),
-// S(2), O(1), ..: softmax j runs under S(j + 1).
+// Roles (288 threads a CTA): warp 0 loads (TMA, ring of 7 x 16 KB), warps 1 and 8 of CTA 0 issue the MMAs of S and of O,
+// warps 2-3 repair tail tiles, warps 4-7 do softmax, O's scaling and the output.  Order of the ring: K(0), K(1), V(0),
+// K(2), V(1), ..: softmax j runs under S(j + 1).  Two issuing threads because a satisfied barrier wait between two MMAs
+// leaves the tensor pipe empty for ~50 cycles, 11 times a unit: while one thread waits the other's MMAs run.
 //
 // Rows that must not matter: a tile's rows beyond the drafts, and drafted rows that a token does not see, get P = 0; but
 // 0 * NaN is NaN, so warps 2-3 zero the former in the O operand, and every drafted row there that holds a non-finite
@@ -31,7 +32,7 @@
 
 namespace lk {
 
-constexpr int TR_THREADS = 256, TR_STAGES = 7, TR_STAGE = 16384, TR_CHUNK = 8192;
+constexpr int TR_THREADS = 288, TR_STAGES = 7, TR_STAGE = 16384, TR_CHUNK = 8192;
 constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + 2 * TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
 constexpr int TR_XCH = TR_BARS + 40 * 8, TR_SCHED = TR_XCH + 128 * 4;
 constexpr int TR_SMEM = TR_SCHED + (LK_ATTN_MAX_SEQS + 1) * 8;
@@ -41,7 +42,7 @@ constexpr float TR_SHIFT = 7.0f, TR_JUMP = 8.0f;      // P <= 2^15 fits fp16; it
 
 struct TreeBars {
     uint64_t full[TR_STAGES], empty[TR_STAGES], land[TR_STAGES];
-    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], q_full, drain;
+    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], q_full, drain[2];
     uint32_t tmem;
     int gave_up;
 };
@@ -123,9 +124,8 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     if (tid == 0) {
         B.gave_up = 0;
         for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], 1); mbar_init(&B.land[s], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 8); mbar_init(&B.p_full[i], 8); mbar_init(&B.o_done[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 8); mbar_init(&B.p_full[i], 8); mbar_init(&B.o_done[i], 1); mbar_init(&B.drain[i], 1); }
         mbar_init(&B.q_full, 8);
-        mbar_init(&B.drain, 1);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
@@ -152,51 +152,60 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                                                  : tree_load<16>(p, prefix, u, u_end, &kv_map, B, smb, rank);
             if (!ok) __nanosleep(1000000);                // given up: the loads in flight land before the CTA ends
         }
-    } else if (warp == 1) {
-        // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both
+    } else if (warp == 1 || warp == 8) {
+        // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both: S and O by a thread each
         if (rank == 0 && elect_one()) {
             constexpr uint32_t id_s = att_idesc(128, 128, BF, false), id_o = att_idesc(128, 256, BF, true);
-            uint32_t st = 0, ph = 0, n_s = 0, n_o = 0, n_q = 0;          // stages, S tiles, O tiles and segments so far
-            bool ok = true, any = false;
-            auto wait = [&](uint64_t* bar, uint32_t parity) { ok = wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); return ok; };
-            for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
-                if (!wait(&B.q_full, n_q & 1)) break;
-                ++n_q;
-                for (int j = g.t0; ok && j <= g.t1; ++j) {
-                    if (j < g.t1) {
-                        const uint32_t buf = n_s & 1;
-                        if (!wait(&B.s_free[buf], ((n_s >> 1) & 1) ^ 1)) break;
+            uint32_t st = 0, ph = 0, n = 0, n_q = 0;      // ring place; tiles and segments so far
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = wait_phase(bar, parity, gave_up, p.err); };
+            auto advance = [&](uint32_t k) { st += k; if (st >= TR_STAGES) { st -= TR_STAGES; ph ^= 1; } };
+            if (warp == 1) {
+                for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+                    if (!wait(&B.q_full, n_q++ & 1)) break;
+                    for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
+                        const uint32_t buf = n & 1, d = tmem + TR_S_COL + buf * 64;
+                        if (!wait(&B.s_free[buf], ((n >> 1) & 1) ^ 1)) break;
+                        tc_fence_after();
                         for (int s = 0; s < 5; ++s) {
                             if (!wait(&B.full[st], ph)) break;
-                            const uint32_t kb = smb + TR_RING + st * TR_STAGE;
-                            const uint32_t qb = smb + TR_Q + 2 * s * TR_CHUNK, d = tmem + TR_S_COL + buf * 64;
+                            const uint32_t kb = smb + TR_RING + st * TR_STAGE, qb = smb + TR_Q + 2 * s * TR_CHUNK;
                             umma2_x4<id_s, 32, 32>(d, sw128_lo(qb, 16), sw128_lo(kb, 16), s != 0);
                             if (s < 4) umma2_x4<id_s, 32, 32>(d, sw128_lo(qb + TR_CHUNK, 16), sw128_lo(kb + TR_CHUNK, 16), 1);
                             commit2(&B.empty[st]);
-                            if (++st == TR_STAGES) { st = 0; ph ^= 1; }
+                            advance(1);
                         }
-                        any = true;
                         if (!ok) break;
                         commit2(&B.s_full[buf]);
-                        ++n_s;
+                        if (j > g.t0) advance(4);         // V of tile j - 1
                     }
-                    if (j > g.t0) {
-                        const uint32_t buf = n_o & 1;
-                        if (!wait(&B.p_full[buf], (n_o >> 1) & 1)) break;
+                    advance(4);                           // V of the last tile
+                }
+            } else {
+                for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+                    advance(5);                           // K of the first tile
+                    for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
+                        if (j + 1 < g.t1) advance(5);     // K of tile j + 1
+                        const uint32_t buf = n & 1;
+                        if (!wait(&B.p_full[buf], (n >> 1) & 1)) break;
+                        tc_fence_after();
                         for (int s = 0; s < 4; ++s) {
                             if (!wait(&B.full[st], ph)) break;
                             const uint32_t vb = smb + TR_RING + st * TR_STAGE, pb = smb + TR_P + buf * TR_STAGE + (s & 1) * TR_CHUNK;
-                            umma2_x4<id_o, 32, 2048>(tmem + (s >> 1) * 128, sw128_lo(pb, 16), sw128_lo(vb, TR_CHUNK), j - 1 > g.t0 || (s & 1));
+                            umma2_x4<id_o, 32, 2048>(tmem + (s >> 1) * 128, sw128_lo(pb, 16), sw128_lo(vb, TR_CHUNK), j > g.t0 || (s & 1));
                             commit2(&B.empty[st]);
-                            if (++st == TR_STAGES) { st = 0; ph ^= 1; }
+                            advance(1);
                         }
                         if (!ok) break;
                         commit2(&B.o_done[buf]);
-                        ++n_o;
                     }
                 }
             }
-            if (!ok && any) { commit2(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
+            if (!ok) {                                    // given up: this thread's MMAs complete before the CTA ends
+                uint64_t* drain = &B.drain[warp >> 3];
+                commit2(drain);
+                mbar_wait(drain, 0, nullptr, 0);
+            }
         }
     } else if (warp < 4) {
         // ---------------------------------------------------------------- repair of the O operand's tail tiles
@@ -483,6 +492,7 @@ __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ Tr
 template <class T>
 static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_merge<T>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     if (e != cudaSuccess) return e;
     const int pairs = nsm / 2 < MG_PARTS ? nsm / 2 : MG_PARTS;
     k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
