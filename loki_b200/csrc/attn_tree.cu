@@ -17,13 +17,14 @@
 // SMs at once makes the 136 KB a CTA loads for it about 3100, which bounds calls with many rows.  Few rows are bound by
 // HBM: 74 pairs at 3100 cycles ask for 6.7 TB/s.
 //
-// Roles (288 threads a CTA): warp 0 loads (TMA, ring of 7 x 16 KB), warps 1 and 8 of CTA 0 issue the MMAs of S and of O,
-// warps 2-3 repair tail tiles, warps 4-7 do softmax, O's scaling and the output.  Order of the ring: K(0), K(1), V(0),
+// Roles (384 threads a CTA): warp 0 loads (TMA, ring of 7 x 16 KB), warps 1 and 2 of CTA 0 issue the MMAs of S and of O,
+// warp 3 repairs tail tiles, warps 4-11 do softmax, O's scaling and the output (two threads per tensor-memory lane, four per
+// row: with one per lane V waits twice as long in the ring for P).  Order of the ring: K(0), K(1), V(0),
 // K(2), V(1), ..: softmax j runs under S(j + 1).  Two issuing threads because a satisfied barrier wait between two MMAs
 // leaves the tensor pipe empty for ~50 cycles, 11 times a unit: while one thread waits the other's MMAs run.
 //
 // Rows that must not matter: a tile's rows beyond the drafts, and drafted rows that a token does not see, get P = 0; but
-// 0 * NaN is NaN, so warps 2-3 zero the former in the O operand, and every drafted row there that holds a non-finite
+// 0 * NaN is NaN, so warp 3 zeroes the former in the O operand, and every drafted row there that holds a non-finite
 // value (a token that does see it gets its NaN through S and P).
 #include <type_traits>
 #include "attn_tc.cuh"
@@ -32,9 +33,9 @@
 
 namespace lk {
 
-constexpr int TR_THREADS = 288, TR_STAGES = 7, TR_STAGE = 16384, TR_CHUNK = 8192;
+constexpr int TR_THREADS = 384, TR_STAGES = 7, TR_STAGE = 16384, TR_CHUNK = 8192;
 constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + 2 * TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
-constexpr int TR_XCH = TR_BARS + 40 * 8, TR_SCHED = TR_XCH + 128 * 4;
+constexpr int TR_XCH = TR_BARS + 40 * 8, TR_SCHED = TR_XCH + 256 * 4;
 constexpr int TR_SMEM = TR_SCHED + (LK_ATTN_MAX_SEQS + 1) * 8;
 static_assert(TR_SMEM <= 232448, "227 KB a CTA");
 constexpr uint32_t TR_S_COL = 256, TR_TMEM = 512;
@@ -88,7 +89,7 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const int64_t* pr
                 }
             }
             if (j > g.t0) {
-                const bool tail = j * ATT_TILE > g.len;   // tile j - 1 reaches beyond the context: warps 2-3 pass it on
+                const bool tail = j * ATT_TILE > g.len;   // tile j - 1 reaches beyond the context: warp 3 passes it on
                 #pragma unroll
                 for (int s = 0; s < 4; ++s) {             // column group s / 2, row half s % 2
                     if (!wait_phase(&B.empty[st], ph, &B.gave_up, p.err)) return false;
@@ -124,12 +125,12 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     if (tid == 0) {
         B.gave_up = 0;
         for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], 1); mbar_init(&B.land[s], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 8); mbar_init(&B.p_full[i], 8); mbar_init(&B.o_done[i], 1); mbar_init(&B.drain[i], 1); }
-        mbar_init(&B.q_full, 8);
+        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 16); mbar_init(&B.p_full[i], 16); mbar_init(&B.o_done[i], 1); mbar_init(&B.drain[i], 1); }
+        mbar_init(&B.q_full, 16);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
-    if (warp == 2) tmem_alloc2(&B.tmem, TR_TMEM);
+    if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
     sched_prefix<ATT_TILE>(p, prefix, tid, TR_THREADS);
     tc_fence_before();
     __syncthreads();
@@ -152,7 +153,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                                                  : tree_load<16>(p, prefix, u, u_end, &kv_map, B, smb, rank);
             if (!ok) __nanosleep(1000000);                // given up: the loads in flight land before the CTA ends
         }
-    } else if (warp == 1 || warp == 8) {
+    } else if (warp < 3) {
         // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both: S and O by a thread each
         if (rank == 0 && elect_one()) {
             constexpr uint32_t id_s = att_idesc(128, 128, BF, false), id_o = att_idesc(128, 256, BF, true);
@@ -202,7 +203,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 }
             }
             if (!ok) {                                    // given up: this thread's MMAs complete before the CTA ends
-                uint64_t* drain = &B.drain[warp >> 3];
+                uint64_t* drain = &B.drain[warp - 1];
                 commit2(drain);
                 mbar_wait(drain, 0, nullptr, 0);
             }
@@ -210,68 +211,65 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     } else if (warp < 4) {
         // ---------------------------------------------------------------- repair of the O operand's tail tiles
         const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
-        const int ft = tid - 64;
         uint32_t st = 0, uses = 0;                        // bit s: parity of the uses of land[s]
-        bool ok = true;
         auto advance = [&](int n) { st = (st + n) % TR_STAGES; };
-        for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
-            for (int j = g.t0; ok && j <= g.t1; ++j) {
+        for (Segment g; sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+            for (int j = g.t0; j <= g.t1; ++j) {
                 if (j < g.t1) advance(5);
                 if (j == g.t0) continue;
                 if (j * ATT_TILE <= g.len) { advance(4); continue; }
-                for (int s = 0; s < 4; ++s) {
-                    ok = !named_bar_or(2, 64, !wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err));
-                    if (!ok) break;
+                for (int s = 0; s < 4; ++s, advance(1)) {
+                    wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err);
                     uses ^= 1u << st;
-                    // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each; one thread per row
-                    const int i = (j - 1) * ATT_TILE + (s & 1) * 64 + ft;
-                    if (i >= g.len) {
-                        uint4* r = (uint4*)(sm + TR_RING + st * TR_STAGE + ft * 128);
+                    // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each; two rows a lane.  Each row's part is judged by
+                    // itself: all that matters is that nothing non-finite is multiplied by 0
+                    for (int r = lane; r < 64; r += 32) {
+                        const int i = (j - 1) * ATT_TILE + (s & 1) * 64 + r;
+                        if (i < g.len) continue;
+                        uint4* v = (uint4*)(sm + TR_RING + st * TR_STAGE + r * 128);
                         bool bad = i >= g.total;
                         if (!bad) {
                             uint32_t hit = 0;             // a 16-bit value whose exponent bits are all ones
                             #pragma unroll
                             for (int c = 0; c < 16; ++c) {
-                                const uint4 v = r[(c >> 3) * (TR_CHUNK / 16) + ((c + ft) & 7)];
-                                hit |= nonfinite2<T>(v.x) | nonfinite2<T>(v.y) | nonfinite2<T>(v.z) | nonfinite2<T>(v.w);
+                                const uint4 w = v[(c >> 3) * (TR_CHUNK / 16) + ((c + r) & 7)];
+                                hit |= nonfinite2<T>(w.x) | nonfinite2<T>(w.y) | nonfinite2<T>(w.z) | nonfinite2<T>(w.w);
                             }
                             bad = hit != 0;
                         }
-                        // a row's two blocks and its two column groups are judged each by itself: all that matters is
-                        // that nothing non-finite is multiplied by 0
                         if (bad)
                             #pragma unroll
-                            for (int c = 0; c < 16; ++c) r[(c >> 3) * (TR_CHUNK / 16) + ((c + ft) & 7)] = make_uint4(0, 0, 0, 0);
+                            for (int c = 0; c < 16; ++c) v[(c >> 3) * (TR_CHUNK / 16) + ((c + r) & 7)] = make_uint4(0, 0, 0, 0);
                     }
                     fence_async_smem();
-                    named_bar_sync(2, 64);
-                    if (ft == 0) arrive_at(full0 + 8 * st);
-                    advance(1);
+                    __syncwarp();
+                    if (lane == 0) arrive_at(full0 + 8 * st);
                 }
             }
         }
     } else {
         // ---------------------------------------------------------------- softmax, O's scaling, output
-        const int L = tid - 128, row = L & 63, half = L >> 6;
-        const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+        // Thread (lane L, column half ch): row L % 64, keys 64 (L / 64) + 32 ch .. + 31 of a tile, O columns 128 ch .. + 127 of
+        // the lane.  A wait that gives up is not acted on here: every later one then returns at once, and the loops end.
+        const int L = (tid - 128) & 127, ch = (tid - 128) >> 7, row = L & 63, half = L >> 6, part = 2 * half + ch;
+        const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16, o_base = tmem + lane_base + ch * 128;
         const uint32_t s_free0 = peer_addr(smem_u32(&B.s_free[0]), 0), p_full0 = peer_addr(smem_u32(&B.p_full[0]), 0),
                        q_full0 = peer_addr(smem_u32(&B.q_full), 0);
         const float scale2 = p.scale * 1.4426950408889634f;
         uint32_t n = 0;                                   // tiles so far
-        bool ok = true, first_seg = true;
-        // every thread of the group gets the same answer
-        auto wait = [&](uint64_t* bar, uint32_t parity) { ok = !named_bar_or(1, 128, !wait_phase(bar, parity, gave_up, p.err)); tc_fence_after(); return ok; };
-        for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
-            // ---- Q: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 16 rows a warp, whose places in q the
+        bool first_seg = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); };
+        for (Segment g; sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+            // ---- Q: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 8 rows a warp, whose places in q the
             // lanes that own the rows below know
             const int gr = g.rt * 128 + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
             const bool live = gr < g.n * p.H;
             const int64_t q_at = live ? t * p.q_token + h * p.q_head : -1;
-            const int w4 = warp & 3;
+            const int w0 = ((warp - 4) >> 1) * 8;
             #pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                const int64_t at = __shfl_sync(0xffffffffu, q_at, (w4 >> 1) * 16 + i);
-                const int r = (w4 & 1) * 32 + (w4 >> 1) * 16 + i;
+            for (int i = 0; i < 8; ++i) {
+                const int64_t at = __shfl_sync(0xffffffffu, q_at, w0 + i);
+                const int r = (warp & 1) * 32 + w0 + i;
                 const T* src = (const T*)p.q + max(at, (int64_t)0);
                 #pragma unroll
                 for (int c = lane; c < 72; c += 32)
@@ -286,81 +284,83 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             float m = -INFINITY, l = 0.0f;
             for (int j = g.t0; j < g.t1; ++j, ++n) {
                 const uint32_t buf = n & 1;
-                if (!wait(&B.s_full[buf], (n >> 1) & 1)) break;
-                float s[64];
+                wait(&B.s_full[buf], (n >> 1) & 1);
+                float s[32];
                 {
-                    uint32_t a[32], b[32];
-                    tmem_ld32(tmem + lane_base + TR_S_COL + buf * 64, a);
-                    tmem_ld32(tmem + lane_base + TR_S_COL + buf * 64 + 32, b);
+                    uint32_t a[32];
+                    tmem_ld32(tmem + lane_base + TR_S_COL + buf * 64 + ch * 32, a);
                     tmem_wait_ld();
                     #pragma unroll
-                    for (int i = 0; i < 32; ++i) { s[i] = __uint_as_float(a[i]); s[32 + i] = __uint_as_float(b[i]); }
+                    for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(a[i]);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_at(s_free0 + 8 * buf);
-                const int base = j * ATT_TILE + half * 64 - g.len;        // drafted node of the first column
-                if (base > -64) {
-                    const uint64_t see = base >= 64 ? 0 : base >= 0 ? mask >> base : (mask << -base) | ((1ull << -base) - 1);
+                const int base = j * ATT_TILE + half * 64 + ch * 32 - g.len;        // drafted node of the first column
+                if (base > -32) {
+                    const uint32_t see = base >= 64 ? 0 : base >= 0 ? (uint32_t)(mask >> base) : (uint32_t)(mask << -base) | ((1u << -base) - 1);
                     #pragma unroll
-                    for (int i = 0; i < 64; ++i) if (!((see >> i) & 1)) s[i] = -INFINITY;
+                    for (int i = 0; i < 32; ++i) if (!((see >> i) & 1)) s[i] = -INFINITY;
                 }
                 float mx[4] = { s[0], s[1], s[2], s[3] };
                 #pragma unroll
-                for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-                if (named_bar_or(1, 128, top > m + TR_JUMP)) {
-                    xch[L] = top;
-                    named_bar_sync(1, 128);
-                    const float m1 = fmaxf(m, fmaxf(top, xch[L ^ 64]));
+                if (named_bar_or(1, 256, top > m + TR_JUMP)) {
+                    xch[part * 64 + row] = top;
+                    named_bar_sync(1, 256);
+                    const float m1 = fmaxf(fmaxf(m, fmaxf(xch[row], xch[64 + row])), fmaxf(xch[128 + row], xch[192 + row]));
                     const float f = m1 == m ? 1.0f : exp2_approx(m - m1);  // m = -inf: 0
                     l *= f;
                     m = m1;
-                    if (j > g.t0) {                       // O(j - 1) is complete: scale its 256 columns of this lane
-                        if (!wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
-                        for (int c = 0; c < 256; c += 32) {
+                    if (j > g.t0) {                       // O(j - 1) is complete: scale its columns
+                        wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+                        for (int c = 0; c < 128; c += 32) {
                             uint32_t o[32];
-                            tmem_ld32(tmem + lane_base + c, o);
+                            tmem_ld32(o_base + c, o);
                             tmem_wait_ld();
                             #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(tmem + lane_base + c, o);
+                            tmem_st32(o_base + c, o);
                         }
                         tmem_wait_st();
                         tc_fence_before();
                     }
-                    named_bar_sync(1, 128);               // xch is free again
+                    named_bar_sync(1, 256);               // xch is free again
                 }
                 const float ref = (m == -INFINITY ? 0.0f : m) - TR_SHIFT;
-                if (j >= g.t0 + 2 && !wait(&B.o_done[buf], ((n - 2) >> 1) & 1)) break;      // O(j - 2) has read this P buffer
-                uint8_t* pr = sm + TR_P + buf * TR_STAGE + half * TR_CHUNK + row * 128;
+                uint32_t e2[16];
                 float sum[4] = { 0, 0, 0, 0 };
                 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    float e[8];
-                    #pragma unroll
-                    for (int i = 0; i < 8; ++i) { e[i] = exp2_approx(fmaf(s[8 * c + i], scale2, -ref)); sum[i & 3] += e[i]; }
-                    *(uint4*)(pr + ((c ^ (row & 7)) << 4)) =
-                        make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
+                for (int i = 0; i < 32; i += 2) {
+                    const float e0 = exp2_approx(fmaf(s[i], scale2, -ref)), e1 = exp2_approx(fmaf(s[i + 1], scale2, -ref));
+                    sum[i & 2] += e0;
+                    sum[(i & 2) + 1] += e1;
+                    e2[i / 2] = pack2<T>(e0, e1);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (j >= g.t0 + 2) wait(&B.o_done[buf], ((n - 2) >> 1) & 1);       // O(j - 2) has read this P buffer
+                uint8_t* pr = sm + TR_P + buf * TR_STAGE + half * TR_CHUNK + row * 128;
+                #pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *(uint4*)(pr + (((4 * ch + c) ^ (row & 7)) << 4)) = make_uint4(e2[4 * c], e2[4 * c + 1], e2[4 * c + 2], e2[4 * c + 3]);
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) arrive_at(p_full0 + 8 * buf);
             }
-            if (!ok) break;
-            // ---- output: all of O, then the row's two half sums
-            if (!wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
-            xch[L] = l;
-            named_bar_sync(1, 128);
-            l += xch[L ^ 64];
-            named_bar_sync(1, 128);
+            // ---- output: all of O, then the row's four sums
+            wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+            xch[part * 64 + row] = l;
+            named_bar_sync(1, 256);
+            l = (xch[row] + xch[64 + row]) + (xch[128 + row] + xch[192 + row]);
+            named_bar_sync(1, 256);
+            const float ref = (m == -INFINITY ? 0.0f : m) - TR_SHIFT;
             if (g.whole) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + half * 128;
-                for (int c = 0; c < 256; c += 32) {
+                T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + ch * 256 + half * 128;
+                for (int c = 0; c < 128; c += 32) {
                     uint32_t o[32];
-                    tmem_ld32(tmem + lane_base + c, o);
+                    tmem_ld32(o_base + c, o);
                     tmem_wait_ld();
                     if (live)
                         #pragma unroll
@@ -370,25 +370,23 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                             v.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
                             v.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
                             v.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-                            *(uint4*)(out + (c & 128) * 2 + (c & 127) + i) = v;
+                            *(uint4*)(out + c + i) = v;
                         }
                 }
-                if (live && half == 0 && p.lse)
-                    p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+                if (live && part == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
             } else {
                 const int slot = 2 * pair + !first_seg, pr = (int)rank * 64 + row;
-                float4* part = wk.part + (int64_t)slot * (128 * 128) + half * 32 * 128 + pr;
-                for (int c = 0; c < 256; c += 32) {
+                float4* to = wk.part + (int64_t)slot * (128 * 128) + (ch * 64 + half * 32) * 128 + pr;
+                for (int c = 0; c < 128; c += 32) {
                     uint32_t o[32];
-                    tmem_ld32(tmem + lane_base + c, o);
+                    tmem_ld32(o_base + c, o);
                     tmem_wait_ld();
                     if (live)
                         #pragma unroll
                         for (int i = 0; i < 32; i += 4)
-                            part[((c & 128) / 2 + (c & 127) / 4 + i / 4) * 128] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                                                                                        __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                            to[(c + i) / 4 * 128] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                 }
-                if (live && half == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
+                if (live && part == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
             }
             tc_fence_before();
             first_seg = false;
@@ -397,7 +395,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     tc_fence_before();
     __syncthreads();
     cluster_sync();
-    if (warp == 2) { tc_fence_after(); tmem_dealloc2(tmem, TR_TMEM); }
+    if (warp == 3) { tc_fence_after(); tmem_dealloc2(tmem, TR_TMEM); }
 }
 
 // ---------------------------------------------------------------- joining split items
