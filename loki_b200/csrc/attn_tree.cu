@@ -17,7 +17,7 @@
 // SMs at once makes the 136 KB a CTA loads for it about 3100, which bounds calls with many rows.  Few rows are bound by
 // HBM: 74 pairs at 3100 cycles ask for 6.7 TB/s.
 //
-// Roles (384 threads a CTA): warp 0 loads (TMA, ring of 7 x 16 KB), warps 1 and 2 of CTA 0 issue the MMAs of S and of O,
+// Roles (384 threads a CTA): warp 0 loads (TMA, ring of 8 x 16 KB), warps 1 and 2 of CTA 0 issue the MMAs of S and of O,
 // warp 3 repairs tail tiles, warps 4-11 do softmax, O's scaling and the output (two threads per tensor-memory lane, four per
 // row: with one per lane V waits twice as long in the ring for P).  Order of the ring: K(0), K(1), V(0),
 // K(2), V(1), ..: softmax j runs under S(j + 1).  Two issuing threads because a satisfied barrier wait between two MMAs
@@ -33,8 +33,8 @@
 
 namespace lk {
 
-constexpr int TR_THREADS = 384, TR_STAGES = 7, TR_STAGE = 16384, TR_CHUNK = 8192;
-constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + 2 * TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
+constexpr int TR_THREADS = 384, TR_STAGES = 8, TR_STAGE = 16384, TR_CHUNK = 8192;
+constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
 constexpr int TR_XCH = TR_BARS + 40 * 8, TR_SCHED = TR_XCH + 256 * 4;
 constexpr int TR_SMEM = TR_SCHED + (LK_ATTN_MAX_SEQS + 1) * 8;
 static_assert(TR_SMEM <= 232448, "227 KB a CTA");
@@ -43,7 +43,7 @@ constexpr float TR_SHIFT = 7.0f, TR_JUMP = 8.0f;      // P <= 2^15 fits fp16; it
 
 struct TreeBars {
     uint64_t full[TR_STAGES], empty[TR_STAGES], land[TR_STAGES];
-    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], q_full, drain[2];
+    uint64_t s_full[2], s_free[2], p_full, o_done, q_full, drain[2];
     uint32_t tmem;
     int gave_up;
 };
@@ -125,8 +125,8 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     if (tid == 0) {
         B.gave_up = 0;
         for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], 1); mbar_init(&B.land[s], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 16); mbar_init(&B.p_full[i], 16); mbar_init(&B.o_done[i], 1); mbar_init(&B.drain[i], 1); }
-        mbar_init(&B.q_full, 16);
+        for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 16); mbar_init(&B.drain[i], 1); }
+        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, 16);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
@@ -187,18 +187,17 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     advance(5);                           // K of the first tile
                     for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
                         if (j + 1 < g.t1) advance(5);     // K of tile j + 1
-                        const uint32_t buf = n & 1;
-                        if (!wait(&B.p_full[buf], (n >> 1) & 1)) break;
+                        if (!wait(&B.p_full, n & 1)) break;
                         tc_fence_after();
                         for (int s = 0; s < 4; ++s) {
                             if (!wait(&B.full[st], ph)) break;
-                            const uint32_t vb = smb + TR_RING + st * TR_STAGE, pb = smb + TR_P + buf * TR_STAGE + (s & 1) * TR_CHUNK;
+                            const uint32_t vb = smb + TR_RING + st * TR_STAGE, pb = smb + TR_P + (s & 1) * TR_CHUNK;
                             umma2_x4<id_o, 32, 2048>(tmem + (s >> 1) * 128, sw128_lo(pb, 16), sw128_lo(vb, TR_CHUNK), j > g.t0 || (s & 1));
                             commit2(&B.empty[st]);
                             advance(1);
                         }
                         if (!ok) break;
-                        commit2(&B.o_done[buf]);
+                        commit2(&B.o_done);
                     }
                 }
             }
@@ -253,7 +252,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         // the lane.  A wait that gives up is not acted on here: every later one then returns at once, and the loops end.
         const int L = (tid - 128) & 127, ch = (tid - 128) >> 7, row = L & 63, half = L >> 6, part = 2 * half + ch;
         const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16, o_base = tmem + lane_base + ch * 128;
-        const uint32_t s_free0 = peer_addr(smem_u32(&B.s_free[0]), 0), p_full0 = peer_addr(smem_u32(&B.p_full[0]), 0),
+        const uint32_t s_free0 = peer_addr(smem_u32(&B.s_free[0]), 0), p_full0 = peer_addr(smem_u32(&B.p_full), 0),
                        q_full0 = peer_addr(smem_u32(&B.q_full), 0);
         const float scale2 = p.scale * 1.4426950408889634f;
         uint32_t n = 0;                                   // tiles so far
@@ -314,7 +313,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     l *= f;
                     m = m1;
                     if (j > g.t0) {                       // O(j - 1) is complete: scale its columns
-                        wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+                        wait(&B.o_done, (n - 1) & 1);
                         for (int c = 0; c < 128; c += 32) {
                             uint32_t o[32];
                             tmem_ld32(o_base + c, o);
@@ -339,17 +338,17 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     e2[i / 2] = pack2<T>(e0, e1);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (j >= g.t0 + 2) wait(&B.o_done[buf], ((n - 2) >> 1) & 1);       // O(j - 2) has read this P buffer
-                uint8_t* pr = sm + TR_P + buf * TR_STAGE + half * TR_CHUNK + row * 128;
+                if (j > g.t0) wait(&B.o_done, (n - 1) & 1);        // O(j - 1) has read P
+                uint8_t* pr = sm + TR_P + half * TR_CHUNK + row * 128;
                 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     *(uint4*)(pr + (((4 * ch + c) ^ (row & 7)) << 4)) = make_uint4(e2[4 * c], e2[4 * c + 1], e2[4 * c + 2], e2[4 * c + 3]);
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive_at(p_full0 + 8 * buf);
+                if (lane == 0) arrive_at(p_full0);
             }
             // ---- output: all of O, then the row's four sums
-            wait(&B.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+            wait(&B.o_done, (n - 1) & 1);
             xch[part * 64 + row] = l;
             named_bar_sync(1, 256);
             l = (xch[row] + xch[64 + row]) + (xch[128 + row] + xch[192 + row]);
