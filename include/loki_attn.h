@@ -26,7 +26,7 @@ extern "C" {
 #define LK_ATTN_ROW 576
 #define LK_ATTN_MAX_HEADS 128
 #define LK_ATTN_MAX_NODES 64       /* drafted tokens per sequence and call */
-#define LK_ATTN_MAX_SEQS 1024
+#define LK_ATTN_MAX_SEQS 512
 
 enum { LK_DT_F32 = 0, LK_DT_F16 = 1, LK_DT_BF16 = 2 };
 enum { LK_ROPE_INTERLEAVED = 0, LK_ROPE_HALF = 1 };     /* pairs (2i, 2i+1), or (i, i + rot_dim/2) */

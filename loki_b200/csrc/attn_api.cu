@@ -3,7 +3,6 @@
 #include <cstdarg>
 #include <new>
 #include "attn_internal.h"
-#include "attn_sched.cuh"
 
 using namespace lk;
 
@@ -12,7 +11,7 @@ struct LkAttnCtx {
     int device = 0, nsm = 0;
     int* err = nullptr;
     int* n_moves = nullptr; int* moves = nullptr; int64_t moves_cap = 0;      // eviction: [2][n_seqs][region]
-    TreeWork work{};                                                          // lk_attn_tree: parts of split items
+    TreeWork work{}; int pairs = 0;                                           // lk_attn_tree: parts of split items
     char msg[256] = {0};
 };
 
@@ -124,6 +123,7 @@ int lk_attn_get_error(LkAttnCtx* c, lk_stream_t stream) {
     LK_CU(cudaMemcpy(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost));
     if (!e) return LK_OK;
     LK_CU(cudaMemset(c->err, 0, sizeof(int)));
+    if (c->work.sync) LK_CU(cudaMemset(c->work.sync, 0, (size_t)c->pairs * 2 * sizeof(int)));      // a wait that ran out leaves its counts
     const char* what = e == ATT_ERR_PAGE ? "a page id outside the pool" : e == ATT_ERR_POS ? "a position outside the rope table"
                      : e == ATT_ERR_LEN ? "a length outside its pages" : e == ATT_ERR_TREE ? "token ranges out of order or too long"
                      : "a bounded wait ran out";
@@ -207,14 +207,17 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     p.out = out; p.out_token = out_token; p.out_head = out_head; p.lse = lse;
     CUtensorMap map;
     if (int rc = encode_map(c, cache, &map)) return rc;
-    if (!c->work.prefix) {                            // parts of at most two items per pair of SMs: 0.5 MB a pair
+    if (!c->work.part) {                              // parts of at most two items per pair of SMs: 0.5 MB a pair
         if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
-        const size_t slots = c->nsm / 2 * 2, part = slots * 128 * AT_LATENT * 4, ml = slots * 128 * 8, pre = (LK_ATTN_MAX_SEQS + 1) * 8;
-        void* w = nullptr;
-        LK_CU(cudaMalloc(&w, part + ml + pre));
-        c->work = TreeWork{ (float4*)w, (float2*)((char*)w + part), (int64_t*)((char*)w + part + ml) };
+        c->pairs = tree_pairs(c->nsm);
+        if (c->pairs < 1) return set_err(c, LK_ERR_UNSUPPORTED, "no room for a pair of CTAs on this device");
+        const size_t part = (size_t)c->pairs * 2 * 128 * AT_LATENT * 4, ml = (size_t)c->pairs * 2 * 128 * 8, sync = (size_t)c->pairs * 2 * sizeof(int);
+        char* w = nullptr;
+        LK_CU(cudaMalloc((void**)&w, part + ml + sync));
+        if (cudaMemsetAsync(w + part + ml, 0, sync, (cudaStream_t)stream) != cudaSuccess) { cudaFree(w); return set_err(c, LK_ERR_CUDA, "cudaMemsetAsync"); }
+        c->work = TreeWork{ (float4*)w, (float2*)(w + part), (int*)(w + part + ml) };
     }
-    LK_CU(launch_tree(p, cache->dtype, map, c->work, c->nsm, (cudaStream_t)stream));
+    LK_CU(launch_tree(p, cache->dtype, map, c->work, c->pairs, (cudaStream_t)stream));
     return LK_OK;
 }
 

@@ -52,8 +52,14 @@ struct TreeParams {
     const float* weight; float decay;              // mass
     int* err;
 };
-struct TreeWork;                                   // attn_sched.cuh
-cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st);
+// parts of items that more than one pair of CTAs works on (attn_tree.cu)
+struct TreeWork {
+    float4* part;              // [2 per pair][16 groups of 8 rows][512 / 4][8 rows]: O, not yet divided by the sum
+    float2* ml;                // [2 per pair][128 rows]: reference and sum
+    int* sync;                 // [2][pairs]: CTAs that have left their part of an item, and that have read all of them; zero between calls
+};
+int tree_pairs(int nsm);       // pairs of CTAs that run at once on the current device
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st);
 cudaError_t launch_mass(const TreeParams& p, int dtype, int nsm, cudaStream_t st);
 
 struct EvictParams {

@@ -1,7 +1,7 @@
 // attn_sched.cuh -- equal cuts of a ragged batch's work, made on the device from the lengths.
 //
-// Sequence b has ceil(n_b * H / rows per item) items of ceil((len_b + n_b) / TILE) tiles; (item, tile) units are numbered
-// sequence by sequence, item by item.  Run q of `used` takes units [W q / used, W (q + 1) / used).
+// Sequence b has ceil(n_b * H / 128) items of ceil((len_b + n_b) / TILE) tiles; (item, tile) units are numbered sequence by
+// sequence, item by item.  They are cut into `runs` of `base` or base + 1 units, the longer ones first.
 #pragma once
 #include "attn_internal.h"
 
@@ -9,70 +9,99 @@ namespace lk {
 
 constexpr int ATT_TILE = 128, ATT_ITEM = 128;
 
-struct TreeWork {
-    float4* part;              // [2 per run][512 / 4][128 rows]: O of a run's first and last item where it has only part of it
-    float2* ml;                // [2 per run][128 rows]: reference and sum
-    int64_t* prefix;           // [n_seqs + 1] units before each sequence
+// a call's sequences, in shared memory
+struct Sched {
+    int64_t prefix[LK_ATTN_MAX_SEQS + 1];      // units before each sequence, the last: all of them
+    int len[LK_ATTN_MAX_SEQS];                 // context rows
+    int start[LK_ATTN_MAX_SEQS + 1];           // drafted tokens
+    int64_t base; int more, runs;              // units of a run, runs of one unit more, all runs
+    __device__ __forceinline__ int64_t run_start(int q) const { return q * base + min(q, more); }
+    // the run that has unit u.  A run leaves a part of its first item in slot 2 q and of its last in 2 q + 1, so an item that
+    // starts inside run q has its first part in 2 q + 1 and the others in even slots
+    __device__ __forceinline__ int owner(int64_t u) const;
 };
+
+// 64-bit values that nearly always fit 32 bits, where a division takes a fifth of the instructions
+__device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+__device__ __forceinline__ int Sched::owner(int64_t u) const {
+    const int64_t longer = more * (base + 1);
+    return (int)(u < longer ? div_small(u, base + 1) : more + div_small(u - longer, base));
+}
 
 struct Segment {
-    int b, first, n, len, total;       // sequence, its first drafted token, drafted tokens, context, all rows
-    int rt, t0, t1;                    // item of the sequence, tiles
-    bool whole;                        // the item's every tile
+    int b, first, n, len, total;               // sequence, its first drafted token, drafted tokens, context, all rows
+    int rt, t0, t1, tiles;                     // item of the sequence, tiles [t0, t1) of its `tiles`
+    int64_t item;                              // the item's first unit
+    __device__ __forceinline__ bool whole() const { return t1 - t0 == tiles; }
 };
 
-// units before each sequence, prefix[n_seqs] all of them; every thread of the block calls it, the caller synchronises
+// the whole block calls it (one sequence: its first warp is enough), for at most `pairs` runs and no more than the longest
+// run's length needs; the caller synchronises before sched_next
 template <int TILE>
-__device__ __forceinline__ void sched_prefix(const TreeParams& p, int64_t* prefix, int tid, int threads) {
+__device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int tid, int threads, int pairs) {
     for (int b = tid; b < p.kv.n_seqs; b += threads) {
-        const int len = kv_len(p.kv, b, p.err), n = seq_tokens(p.starts, b, p.T, len, p.kv, p.err).y;
-        prefix[b + 1] = n ? (int64_t)((n * p.H + ATT_ITEM - 1) / ATT_ITEM) * ((len + n + TILE - 1) / TILE) : 0;
+        const int len0 = p.kv.lens[b], t0 = p.starts[b], t1 = p.starts[b + 1], cap = p.kv.table_stride << p.kv.page_shift;
+        const int len = min(max(len0, 0), cap), n = t1 - t0;
+        int64_t units = 0;
+        if (len != len0) att_error(p.err, ATT_ERR_LEN);
+        if (t0 < 0 || n < 0 || t1 > p.T || n > LK_ATTN_MAX_NODES) att_error(p.err, ATT_ERR_TREE);
+        else if (n > cap - len) att_error(p.err, ATT_ERR_LEN);
+        else if (n) units = (int64_t)((n * p.H + ATT_ITEM - 1) / ATT_ITEM) * ((len + n + TILE - 1) / TILE);
+        s.len[b] = len;
+        s.start[b] = t0;
+        if (b == p.kv.n_seqs - 1) s.start[b + 1] = t1;
+        s.prefix[b + 1] = units;
     }
-    __syncthreads();
+    if (tid == 0) s.prefix[0] = 0;
+    if (p.kv.n_seqs > 1) __syncthreads();
     if (tid < 32) {
+        __syncwarp();
         int64_t before = 0;
         for (int b0 = 0; b0 < p.kv.n_seqs; b0 += 32) {
-            int64_t v = b0 + tid < p.kv.n_seqs ? prefix[b0 + tid + 1] : 0;
+            int64_t v = b0 + tid < p.kv.n_seqs ? s.prefix[b0 + tid + 1] : 0;
             #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
                 if (tid >= o) v += w;
             }
-            if (b0 + tid < p.kv.n_seqs) prefix[b0 + tid + 1] = before + v;
+            if (b0 + tid < p.kv.n_seqs) s.prefix[b0 + tid + 1] = before + v;
             before += __shfl_sync(0xffffffffu, v, 31);
         }
-        if (tid == 0) prefix[0] = 0;
+        if (tid == 0) {
+            const int64_t per = div_small(before + pairs - 1, pairs);
+            s.runs = before ? (int)div_small(before + per - 1, per) : 0;
+            s.base = before ? div_small(before, s.runs) : 0;
+            s.more = (int)(before - s.runs * s.base);
+        }
     }
 }
 
 // the next segment of [u, u_end): consecutive tiles of one item
 template <int TILE>
-__device__ __forceinline__ bool sched_next(const TreeParams& p, const int64_t* prefix, int64_t& u, int64_t u_end, Segment& g) {
+__device__ __forceinline__ bool sched_next(const TreeParams& p, const Sched& s, int64_t& u, int64_t u_end, Segment& g) {
     if (u >= u_end) return false;
-    int lo = 0, hi = p.kv.n_seqs - 1;                    // the last sequence that starts at or before u and has units
+    int lo = 0, hi = p.kv.n_seqs - 1;                    // the last sequence that starts at or before u: it has units
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+        if (s.prefix[mid] <= u) lo = mid; else hi = mid - 1;
     }
     g.b = lo;
-    g.len = kv_len(p.kv, lo, nullptr);
-    const int2 sp = seq_tokens(p.starts, lo, p.T, g.len, p.kv, nullptr);
-    g.first = sp.x; g.n = sp.y; g.total = g.len + g.n;
-    const int tiles = (g.total + TILE - 1) / TILE;
-    const int64_t rem = u - prefix[lo];
-    g.rt = (int)(rem / tiles);
-    g.t0 = (int)(rem % tiles);
-    g.t1 = (int)min((int64_t)tiles, g.t0 + (u_end - u));
-    g.whole = g.t0 == 0 && g.t1 == tiles;
+    g.len = s.len[lo];
+    g.first = s.start[lo];
+    g.n = s.start[lo + 1] - g.first;
+    g.total = g.len + g.n;
+    g.tiles = (g.total + TILE - 1) / TILE;
+    const int64_t rem = u - s.prefix[lo];
+    g.rt = rem < g.tiles ? 0 : (int)div_small(rem, g.tiles);
+    g.t0 = (int)(rem - (int64_t)g.rt * g.tiles);
+    g.t1 = (int)min((int64_t)g.tiles, g.t0 + (u_end - u));
+    g.item = u - g.t0;
     u += g.t1 - g.t0;
     return true;
 }
 
-// runs that a call is cut into
-__host__ __device__ __forceinline__ int sched_pairs(int64_t W, int pairs) { return W < pairs ? (int)W : pairs; }
-// the run that has unit u: the last q with W q / used <= u.  A run leaves a part of its first item in slot 2 q and of its
-// last in 2 q + 1, so an item that starts inside run q has its first part in 2 q + 1 and the others in even slots
-__device__ __forceinline__ int sched_owner(int64_t u, int64_t W, int used) { return (int)(((u + 1) * used + W - 1) / W) - 1; }
 template <class T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t v);
 template <> __device__ __forceinline__ uint32_t nonfinite2<__half>(uint32_t v) { return (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u; }
 template <> __device__ __forceinline__ uint32_t nonfinite2<__nv_bfloat16>(uint32_t v) { return (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u; }

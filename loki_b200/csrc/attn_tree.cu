@@ -6,7 +6,7 @@
 //
 // Work.  A row is one (token, head); 128 rows of one sequence are an item, 128 cached rows a tile, and (item, tile) a
 // unit of work: 35.7 M products, 147 KB of cache.  All units, numbered item by item, are cut into equal runs, one per
-// pair of CTAs, whatever the batch's lengths; an item that lies in several runs leaves partial O, m and l for k_merge.
+// pair of CTAs, whatever the batch's lengths; of an item that lies in several runs each leaves its O, m and l, and joins a share of them.
 // Lengths are read on the device, so a captured call follows them.
 //
 // Why a pair.  fp32 O is 128 x 512: all of one SM's tensor memory.  A pair halves the rows (2-CTA tcgen05.mma, M = 128:
@@ -29,30 +29,109 @@
 #include <type_traits>
 #include "attn_tc.cuh"
 #include "attn_sched.cuh"
-#include "moe_internal.h"
 
 namespace lk {
 
 constexpr int TR_THREADS = 384, TR_STAGES = 8, TR_STAGE = 16384, TR_CHUNK = 8192;
 constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
-constexpr int TR_XCH = TR_BARS + 40 * 8, TR_SCHED = TR_XCH + 256 * 4;
-constexpr int TR_SMEM = TR_SCHED + (LK_ATTN_MAX_SEQS + 1) * 8;
+constexpr int TR_XCH = TR_BARS + 48 * 8, TR_SCHED = TR_XCH + 256 * 4;
+constexpr int TR_SMEM = TR_SCHED + (int)sizeof(Sched);
 static_assert(TR_SMEM <= 232448, "227 KB a CTA");
 constexpr uint32_t TR_S_COL = 256, TR_TMEM = 512;
 constexpr float TR_SHIFT = 7.0f, TR_JUMP = 8.0f;      // P <= 2^15 fits fp16; its smallest normal is 2^-21 of the reference
 
+// a split item that this CTA left a part of
+struct TreeJoin { int q0, parts, slot0, rows, row0, first; };       // first run, runs, the first part's slot, rows, first row, first token
+
 struct TreeBars {
     uint64_t full[TR_STAGES], empty[TR_STAGES], land[TR_STAGES];
-    uint64_t s_full[2], s_free[2], p_full, o_done, q_full, drain[2];
+    uint64_t s_full[2], s_free[2], p_full, o_done, q_full, joined, drain[2];
     uint32_t tmem;
     int gave_up;
+    TreeJoin join[2];
 };
-static_assert(sizeof(TreeBars) <= 40 * 8, "barrier block");
+static_assert(sizeof(TreeBars) <= 48 * 8, "barrier block");
+
+// ---------------------------------------------------------------- joining the parts of an item
+// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over the item's parts q.  Every CTA that left a part takes an
+// equal share of the item's (8-row group, 4 latent values, row) elements once all parts are there: 128 KB in all, whatever the
+// number of parts, fetched by one bulk copy a part into the memory that Q and the ring had.  They are added in the parts'
+// order, so the result does not depend on who was first.
+constexpr int JN_PARTS = 128, JN_STAGE = 8192;
+
+template <class T>
+__device__ __forceinline__ void tree_join(const TreeParams& p, const TreeWork& wk, const TreeJoin& jn, int cta, int pairs, uint8_t* sm, int tid,
+                                          uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    const int warp = tid >> 5, lane = tid & 31, n = jn.parts, ctas = 2 * n;
+    float* ref = (float*)sm; float* sum = ref + 128; float* f = sum + 128;      // of the share's rows; f [part][row]
+    const float4* stage = (const float4*)(sm + JN_STAGE);                       // [part][element]
+    auto slot = [&](int i) { return i ? (jn.slot0 & ~1) + 2 * i : jn.slot0; };
+    // this CTA's elements e: row group e / 1024, values 4 (e / 8 % 128), row e % 8
+    const int mine = cta - 2 * jn.q0, all = (jn.rows + 7) / 8 * 1024;
+    const int e0 = (int)((uint32_t)(all * mine) / (uint32_t)ctas), e1 = (int)((uint32_t)(all * (mine + 1)) / (uint32_t)ctas), ne = e1 - e0;
+    const int r0 = e0 >> 10 << 3, nr = ne ? min(jn.rows, ((e1 - 1) >> 10 << 3) + 8) - r0 : 0;
+    if (warp == 0) {
+        if (lane == 0) {
+            const unsigned long long t0 = globaltimer_ns();
+            int seen;
+            do {
+                asm volatile("ld.acquire.gpu.s32 %0, [%1];" : "=r"(seen) : "l"(wk.sync + jn.q0) : "memory");
+                if (seen < ctas && (*gave_up || globaltimer_ns() - t0 > WAIT_LIMIT_NS)) { att_error(p.err, DEV_ERR_TIMEOUT_FULL); *gave_up = 1; break; }
+            } while (seen < ctas);
+            asm volatile("fence.proxy.async;" ::: "memory");                    // the parts were written by ordinary stores
+            mbar_arrive_expect_tx(bar, (uint32_t)(n * ne) * 16);
+        }
+        __syncwarp();
+        if (ne) for (int i = lane; i < n; i += 32) bulk_g2s((void*)(stage + i * ne), wk.part + (int64_t)slot(i) * (128 * 128) + e0, ne * 16, bar);
+    }
+    named_bar_sync(1, 256);
+    for (int r = warp; r < nr; r += 8) {
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&wk.ml[slot(i) * 128 + r0 + r]).x);
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float rf = m == -INFINITY ? 0.0f : m;
+        for (int i = lane; i < n; i += 32) {
+            const float2 ml = __ldcg(&wk.ml[slot(i) * 128 + r0 + r]);
+            // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
+            const float v = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
+            f[i * nr + r] = v;
+            l += v == 0.0f ? 0.0f : v * ml.y;
+        }
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) { ref[r] = rf; sum[r] = l; }
+    }
+    named_bar_sync(1, 256);
+    wait_phase(bar, parity, gave_up, p.err);
+    for (int x = tid; x < ne; x += 256) {
+        const int e = e0 + x, r = (e >> 10 << 3) + (e & 7), c4 = (e >> 3) & 127;
+        if (r >= jn.rows) continue;
+        float4 s = make_float4(0, 0, 0, 0);
+        #pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float4 v = stage[i * ne + x];
+            const float w = f[i * nr + r - r0];
+            s.x += w == 0.0f ? 0.0f : w * v.x;
+            s.y += w == 0.0f ? 0.0f : w * v.y;
+            s.z += w == 0.0f ? 0.0f : w * v.z;
+            s.w += w == 0.0f ? 0.0f : w * v.w;
+        }
+        const int gr = jn.row0 + r, tj = gr / p.H, h = gr - tj * p.H, t = jn.first + tj;
+        const float l = sum[r - r0], inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *(uint2*)((T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + 4 * c4) =
+            make_uint2(pack2<T>(s.x * inv, s.y * inv), pack2<T>(s.z * inv, s.w * inv));
+        if (c4 == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[r - r0] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+    }
+    if (tid == 0 && atomicAdd(wk.sync + pairs + jn.q0, 1) == ctas - 1) { wk.sync[jn.q0] = 0; wk.sync[pairs + jn.q0] = 0; }
+    fence_async_smem();                                // the next join's copies come after these reads
+    named_bar_sync(1, 256);
+}
 
 // the load role of one CTA, one thread: boxes of BOX rows x 64 values.  Its instructions are the loop's length (a loaded
 // stage feeds 512 cycles of MMAs), so the page lookups are made a tile ahead and nothing is computed per box.
 template <int BOX>
-__device__ __forceinline__ bool tree_load(const TreeParams& p, const int64_t* prefix, int64_t u, int64_t u_end, const CUtensorMap* map,
+__device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sched, int64_t u, int64_t u_end, const CUtensorMap* map,
                                           TreeBars& B, uint32_t smb, uint32_t rank) {
     constexpr int NB = 64 / BOX;                          // boxes of 64 rows
     const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
@@ -61,7 +140,7 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const int64_t* pr
         dst += TR_STAGE; bar += 8;
         if (++st == TR_STAGES) { st = 0; ph ^= 1; dst = smb + TR_RING; bar = full0; }
     };
-    for (Segment g; sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+    for (Segment g; sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
         int next[2 * NB], k[2 * NB], v[2 * NB];           // pool rows of the boxes of tiles j + 1, j and j - 1
         // boxes beyond the drafts read the last 16 rows' page again
         auto rows_of = [&](int j) {
@@ -115,42 +194,38 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     extern __shared__ __align__(1024) uint8_t sm[];
     TreeBars& B = *(TreeBars*)(sm + TR_BARS);
     float* xch = (float*)(sm + TR_XCH);
-    int64_t* prefix = (int64_t*)(sm + TR_SCHED);
+    Sched& sched = *(Sched*)(sm + TR_SCHED);
     volatile int* gave_up = &B.gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
 
-    if (tid == 0) {
+    if (warp == 2 && lane == 0) {
         B.gave_up = 0;
         for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], 1); mbar_init(&B.land[s], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 16); mbar_init(&B.drain[i], 1); }
-        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, 16);
+        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, 16); mbar_init(&B.joined, 1);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
-    sched_prefix<ATT_TILE>(p, prefix, tid, TR_THREADS);
+    if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE>(p, sched, tid, TR_THREADS, pairs);
     tc_fence_before();
     __syncthreads();
     cluster_sync();
     tc_fence_after();
-    pdl_trigger();
     const uint32_t tmem = B.tmem;
-    const int64_t W = prefix[p.kv.n_seqs];
-    if (blockIdx.x == 0) for (int i = tid; i <= p.kv.n_seqs; i += TR_THREADS) wk.prefix[i] = prefix[i];
-    const int used = sched_pairs(W, pairs);
-    const int64_t u_end = pair < used ? W * (pair + 1) / used : 0;
-    int64_t u = pair < used ? W * pair / used : 0;
+    int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
+    const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
     const uint32_t smb = smem_u32(sm);
 
     if (warp == 0) {
         // ---------------------------------------------------------------- loads
         if (elect_one()) {
-            const bool ok = p.kv.page_size >= 64 ? tree_load<64>(p, prefix, u, u_end, &kv_map, B, smb, rank)
-                          : p.kv.page_size == 32 ? tree_load<32>(p, prefix, u, u_end, &kv_map, B, smb, rank)
-                                                 : tree_load<16>(p, prefix, u, u_end, &kv_map, B, smb, rank);
+            const bool ok = p.kv.page_size >= 64 ? tree_load<64>(p, sched, u, u_end, &kv_map, B, smb, rank)
+                          : p.kv.page_size == 32 ? tree_load<32>(p, sched, u, u_end, &kv_map, B, smb, rank)
+                                                 : tree_load<16>(p, sched, u, u_end, &kv_map, B, smb, rank);
             if (!ok) __nanosleep(1000000);                // given up: the loads in flight land before the CTA ends
         }
     } else if (warp < 3) {
@@ -162,7 +237,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = wait_phase(bar, parity, gave_up, p.err); };
             auto advance = [&](uint32_t k) { st += k; if (st >= TR_STAGES) { st -= TR_STAGES; ph ^= 1; } };
             if (warp == 1) {
-                for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+                for (Segment g; ok && sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
                     if (!wait(&B.q_full, n_q++ & 1)) break;
                     for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
                         const uint32_t buf = n & 1, d = tmem + TR_S_COL + buf * 64;
@@ -183,7 +258,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     advance(4);                           // V of the last tile
                 }
             } else {
-                for (Segment g; ok && sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+                for (Segment g; ok && sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
                     advance(5);                           // K of the first tile
                     for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
                         if (j + 1 < g.t1) advance(5);     // K of tile j + 1
@@ -212,7 +287,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
         uint32_t st = 0, uses = 0;                        // bit s: parity of the uses of land[s]
         auto advance = [&](int n) { st = (st + n) % TR_STAGES; };
-        for (Segment g; sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
+        for (Segment g; sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
             for (int j = g.t0; j <= g.t1; ++j) {
                 if (j < g.t1) advance(5);
                 if (j == g.t0) continue;
@@ -220,25 +295,21 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 for (int s = 0; s < 4; ++s, advance(1)) {
                     wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err);
                     uses ^= 1u << st;
-                    // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each; two rows a lane.  Each row's part is judged by
+                    // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each: eight lanes a row.  Each row's part is judged by
                     // itself: all that matters is that nothing non-finite is multiplied by 0
-                    for (int r = lane; r < 64; r += 32) {
-                        const int i = (j - 1) * ATT_TILE + (s & 1) * 64 + r;
-                        if (i < g.len) continue;
-                        uint4* v = (uint4*)(sm + TR_RING + st * TR_STAGE + r * 128);
+                    const int i0 = (j - 1) * ATT_TILE + (s & 1) * 64;
+                    for (int r = max(0, g.len - i0) & ~3; r < 64; r += 4) {
+                        const int i = i0 + r + (lane >> 3);
+                        uint4* v = (uint4*)(sm + TR_RING + st * TR_STAGE + (r + (lane >> 3)) * 128) + (lane & 7);
                         bool bad = i >= g.total;
-                        if (!bad) {
-                            uint32_t hit = 0;             // a 16-bit value whose exponent bits are all ones
-                            #pragma unroll
-                            for (int c = 0; c < 16; ++c) {
-                                const uint4 w = v[(c >> 3) * (TR_CHUNK / 16) + ((c + r) & 7)];
-                                hit |= nonfinite2<T>(w.x) | nonfinite2<T>(w.y) | nonfinite2<T>(w.z) | nonfinite2<T>(w.w);
-                            }
-                            bad = hit != 0;
+                        if (i0 + r < g.total) {           // a 16-bit value whose exponent bits are all ones
+                            const uint4 a = v[0], c = v[TR_CHUNK / 16];
+                            const uint32_t hit = nonfinite2<T>(a.x) | nonfinite2<T>(a.y) | nonfinite2<T>(a.z) | nonfinite2<T>(a.w) |
+                                                 nonfinite2<T>(c.x) | nonfinite2<T>(c.y) | nonfinite2<T>(c.z) | nonfinite2<T>(c.w);
+                            const uint32_t rows = __ballot_sync(0xffffffffu, hit);
+                            bad |= i >= g.len && ((rows >> (lane & 24)) & 0xff);
                         }
-                        if (bad)
-                            #pragma unroll
-                            for (int c = 0; c < 16; ++c) v[(c >> 3) * (TR_CHUNK / 16) + ((c + r) & 7)] = make_uint4(0, 0, 0, 0);
+                        if (bad) v[0] = v[TR_CHUNK / 16] = make_uint4(0, 0, 0, 0);
                     }
                     fence_async_smem();
                     __syncwarp();
@@ -256,16 +327,15 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                        q_full0 = peer_addr(smem_u32(&B.q_full), 0);
         const float scale2 = p.scale * 1.4426950408889634f;
         uint32_t n = 0;                                   // tiles so far
-        bool first_seg = true;
+        int parts = 0;                                    // split items so far
         auto wait = [&](uint64_t* bar, uint32_t parity) { wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); };
-        for (Segment g; sched_next<ATT_TILE>(p, prefix, u, u_end, g);) {
-            // ---- Q: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 8 rows a warp, whose places in q the
-            // lanes that own the rows below know
-            const int gr = g.rt * 128 + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
-            const bool live = gr < g.n * p.H;
-            const int64_t q_at = live ? t * p.q_token + h * p.q_head : -1;
+        // Q of a segment: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 8 rows a warp, whose places in q
+        // the lanes that own the rows know
+        auto start_q = [&](const Segment& g) {
+            const int gr = g.rt * ATT_ITEM + (int)rank * 64 + row, tj = gr / p.H;
+            const int64_t q_at = gr < g.n * p.H ? (g.first + tj) * p.q_token + (gr - tj * p.H) * p.q_head : -1;
             const int w0 = ((warp - 4) >> 1) * 8;
-            #pragma unroll 4
+            #pragma unroll 2
             for (int i = 0; i < 8; ++i) {
                 const int64_t at = __shfl_sync(0xffffffffu, q_at, w0 + i);
                 const int r = (warp & 1) * 32 + w0 + i;
@@ -275,10 +345,19 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                                  :: "r"(smb + TR_Q + (c >> 3) * TR_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4)), "l"(src + c * 8), "r"(at < 0 ? 0 : 16) : "memory");
             }
+        };
+        auto finish_q = [&]() {
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
             __syncwarp();
             if (lane == 0) arrive_at(q_full0);
+        };
+        Segment g, next;
+        bool more = sched_next<ATT_TILE>(p, sched, u, u_end, g);
+        if (more) { start_q(g); finish_q(); }
+        while (more) {
+            const int gr = g.rt * ATT_ITEM + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
+            const bool live = gr < g.n * p.H;
             const uint64_t mask = live ? node_mask(p.tree, t, tj, g.n) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int j = g.t0; j < g.t1; ++j, ++n) {
@@ -347,14 +426,17 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 __syncwarp();
                 if (lane == 0) arrive_at(p_full0);
             }
-            // ---- output: all of O, then the row's four sums
+            // ---- output: all of O, then the row's four sums; the next segment's Q and first S under them (this one's S are done)
+            more = sched_next<ATT_TILE>(p, sched, u, u_end, next);
+            if (more) start_q(next);
             wait(&B.o_done, (n - 1) & 1);
+            if (more) finish_q();
             xch[part * 64 + row] = l;
             named_bar_sync(1, 256);
             l = (xch[row] + xch[64 + row]) + (xch[128 + row] + xch[192 + row]);
             named_bar_sync(1, 256);
             const float ref = (m == -INFINITY ? 0.0f : m) - TR_SHIFT;
-            if (g.whole) {
+            if (g.whole()) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + ch * 256 + half * 128;
                 for (int c = 0; c < 128; c += 32) {
@@ -374,8 +456,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 }
                 if (live && part == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
             } else {
-                const int slot = 2 * pair + !first_seg, pr = (int)rank * 64 + row;
-                float4* to = wk.part + (int64_t)slot * (128 * 128) + (ch * 64 + half * 32) * 128 + pr;
+                // a part: 8-row groups of 128-byte lines
+                const int slot = 2 * pair + (g.item > sched.run_start(pair)), pr = (int)rank * 64 + row;
+                float4* to = wk.part + (int64_t)slot * (128 * 128) + (pr >> 3) * 1024 + (ch * 64 + half * 32) * 8 + (pr & 7);
                 for (int c = 0; c < 128; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(o_base + c, o);
@@ -383,13 +466,28 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     if (live)
                         #pragma unroll
                         for (int i = 0; i < 32; i += 4)
-                            to[(c + i) / 4 * 128] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                            to[(c + i) * 2] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                 }
                 if (live && part == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
+                const int q0 = sched.owner(g.item);
+                if (tid == 128) {
+                    TreeJoin& jn = B.join[parts];
+                    jn.q0 = q0;
+                    jn.parts = sched.owner(g.item + g.tiles - 1) - q0 + 1;
+                    jn.slot0 = 2 * q0 + (g.item > sched.run_start(q0));
+                    jn.rows = min(ATT_ITEM, g.n * p.H - g.rt * ATT_ITEM);
+                    jn.row0 = g.rt * ATT_ITEM;
+                    jn.first = g.first;
+                }
+                ++parts;
+                __threadfence();
+                named_bar_sync(1, 256);
+                if (tid == 128) atomicAdd(wk.sync + q0, 1);
             }
             tc_fence_before();
-            first_seg = false;
+            g = next;
         }
+        for (int i = 0; i < parts; ++i) tree_join<T>(p, wk, B.join[i], 2 * pair + (int)rank, pairs, sm, tid - 128, &B.joined, i, gave_up);
     }
     tc_fence_before();
     __syncthreads();
@@ -397,109 +495,33 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     if (warp == 3) { tc_fence_after(); tmem_dealloc2(tmem, TR_TMEM); }
 }
 
-// ---------------------------------------------------------------- joining split items
-// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q.  A CTA takes 4 rows x 64 latent
-// values: the parts' factors once into shared memory, then 4 groups of 64 threads take every fourth part, added in order.
-// Items that one pair finished were written by k_tree.
-constexpr int MG_ROWS = 4, MG_C4 = 16, MG_GROUPS = 4, MG_THREADS = MG_ROWS * MG_C4 * MG_GROUPS, MG_PARTS = 128;
-
-template <class T>
-__global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk, int pairs) {
-    __shared__ float4 acc[MG_GROUPS][MG_C4][MG_ROWS];
-    __shared__ float f[MG_PARTS][MG_ROWS];
-    __shared__ int first[MG_ROWS], parts[MG_ROWS], at[MG_ROWS];      // slot of a row's first part (the others: even, 2 apart)
-    __shared__ float ref[MG_ROWS], sum[MG_ROWS];
-    pdl_wait();
-    const int tid = threadIdx.x, rr = tid % MG_ROWS, c4 = tid / MG_ROWS % MG_C4, grp = tid / (MG_ROWS * MG_C4);
-    const int64_t flat = (int64_t)blockIdx.x * MG_ROWS + rr;         // row t * H + h of the call
-    const int t = (int)(flat / p.H), h = (int)(flat - (int64_t)t * p.H);
-    if (tid < MG_ROWS) {
-        int n = 0;
-        const int64_t W = wk.prefix[p.kv.n_seqs];
-        if (t < p.T && W > 0) {
-            int b = 0;                                               // last b with starts[b] <= t
-            for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
-                const int mid = (lo + hi) >> 1;
-                if (p.starts[mid] <= t) { b = mid; lo = mid + 1; } else hi = mid - 1;
-            }
-            const int64_t u_b = wk.prefix[b], w = wk.prefix[b + 1] - u_b;
-            const int t0 = p.starts[b], t1 = p.starts[b + 1], row = (t - t0) * p.H + h;
-            if (w > 0 && t >= t0 && t < t1) {
-                const int used = sched_pairs(W, pairs), items = ((t1 - t0) * p.H + ATT_ITEM - 1) / ATT_ITEM;
-                const int64_t tiles = w / items, u0 = u_b + row / ATT_ITEM * tiles;
-                const int q0 = sched_owner(u0, W, used);
-                n = sched_owner(u0 + tiles - 1, W, used) - q0 + 1;
-                first[rr] = 2 * q0 + (W * q0 / used < u0);
-                at[rr] = row % ATT_ITEM;
-            }
-        }
-        parts[rr] = n > 1 ? n : 0;
-    }
-    __syncthreads();
-    const int n = parts[rr];
-    if (!__syncthreads_or(n > 0)) return;
-    const int s0 = n ? first[rr] : 0, s1 = (s0 & ~1) + 2, pr = n ? at[rr] : 0;      // part i > 0: slot s1 + 2 (i - 1)
-    // the parts' references and sums, then their factors: one row per warp of the first four
-    if (tid < 32 * MG_ROWS) {
-        const int r = tid >> 5, lane = tid & 31, nr = parts[r];
-        if (nr) {
-            const int a0 = first[r], a1 = (a0 & ~1) + 2;
-            float m = -INFINITY, l = 0.0f;
-            for (int i = lane; i < nr; i += 32) m = fmaxf(m, wk.ml[(i ? a1 + 2 * (i - 1) : a0) * 128 + at[r]].x);
-            #pragma unroll
-            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float rf = m == -INFINITY ? 0.0f : m;
-            for (int i = lane; i < nr; i += 32) {
-                const float2 ml = wk.ml[(i ? a1 + 2 * (i - 1) : a0) * 128 + at[r]];
-                // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
-                const float v = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
-                f[i][r] = v;
-                l += v == 0.0f ? 0.0f : v * ml.y;
-            }
-            #pragma unroll
-            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane == 0) { ref[r] = rf; sum[r] = l; }
-        }
-    }
-    __syncthreads();
-    float4 a = make_float4(0, 0, 0, 0);
-    const int cg = blockIdx.y * MG_C4 + c4;
-    const float4* src = wk.part + cg * 128 + pr;
-    #pragma unroll 8
-    for (int i = grp; i < n; i += MG_GROUPS) {
-        const float4 v = __ldcg(src + (int64_t)(i ? s1 + 2 * (i - 1) : s0) * (128 * 128));
-        const float g = f[i][rr];
-        if (g != 0.0f) { a.x += g * v.x; a.y += g * v.y; a.z += g * v.z; a.w += g * v.w; }
-    }
-    acc[grp][c4][rr] = a;
-    __syncthreads();
-    if (grp || !n) return;
-    a = make_float4(0, 0, 0, 0);
-    #pragma unroll
-    for (int q = 0; q < MG_GROUPS; ++q) {
-        const float4 v = acc[q][c4][rr];
-        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-    }
-    const float l = sum[rr], inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = (T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + cg * 4;
-    *(uint2*)out = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-    if (cg == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[rr] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+int tree_pairs(int nsm) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = nsm / 2 * 2; cfg.blockDim = TR_THREADS; cfg.dynamicSmemBytes = TR_SMEM; cfg.attrs = attr; cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(k_tree<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_tree<__half>, &cfg) != cudaSuccess) { cudaGetLastError(); return 0; }
+    n = n < nsm / 2 ? n : nsm / 2;
+    return n < JN_PARTS ? n : JN_PARTS;
 }
 
 template <class T>
-static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
+static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_merge<T>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     if (e != cudaSuccess) return e;
-    const int pairs = nsm / 2 < MG_PARTS ? nsm / 2 : MG_PARTS;
-    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const int64_t rows = (int64_t)p.T * p.H;
-    return launch_pdl_n(k_merge<T>, dim3((unsigned)((rows + MG_ROWS - 1) / MG_ROWS), AT_LATENT / 4 / MG_C4), dim3(MG_THREADS), 0, st, p, wk, pairs);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;      // pairs wait for one another's parts: all of them run at once
+    attr[0].val.cooperative = 1;
+    cfg.gridDim = 2 * pairs; cfg.blockDim = TR_THREADS; cfg.dynamicSmemBytes = TR_SMEM; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_tree<T>, p, map, wk);
 }
 
-cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int nsm, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, wk, nsm, st) : tree_go<__nv_bfloat16>(p, map, wk, nsm, st);
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, wk, pairs, st) : tree_go<__nv_bfloat16>(p, map, wk, pairs, st);
 }
 
 }  // namespace lk

@@ -30,7 +30,7 @@ EP_MAX_RANKS = 8
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ATTN_LATENT, ATTN_ROPE, ATTN_ROW = 512, 64, 576
-ATTN_MAX_HEADS, ATTN_MAX_NODES, ATTN_MAX_SEQS = 128, 64, 1024
+ATTN_MAX_HEADS, ATTN_MAX_NODES, ATTN_MAX_SEQS = 128, 64, 512
 EP_COMM_ID_BYTES = 128
 EP_IPC_HANDLE_BYTES = 64
 
