@@ -123,7 +123,6 @@ int lk_attn_get_error(LkAttnCtx* c, lk_stream_t stream) {
     LK_CU(cudaMemcpy(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost));
     if (!e) return LK_OK;
     LK_CU(cudaMemset(c->err, 0, sizeof(int)));
-    if (c->work.sync) LK_CU(cudaMemset(c->work.sync, 0, (size_t)c->pairs * 2 * sizeof(int)));      // a wait that ran out leaves its counts
     const char* what = e == ATT_ERR_PAGE ? "a page id outside the pool" : e == ATT_ERR_POS ? "a position outside the rope table"
                      : e == ATT_ERR_LEN ? "a length outside its pages" : e == ATT_ERR_TREE ? "token ranges out of order or too long"
                      : "a bounded wait ran out";
@@ -210,12 +209,10 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     if (!c->work.part) {                              // parts of at most two items per pair of SMs: 0.5 MB a pair
         if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
         c->pairs = tree_pairs(c->nsm);
-        if (c->pairs < 1) return set_err(c, LK_ERR_UNSUPPORTED, "no room for a pair of CTAs on this device");
-        const size_t part = (size_t)c->pairs * 2 * 128 * AT_LATENT * 4, ml = (size_t)c->pairs * 2 * 128 * 8, sync = (size_t)c->pairs * 2 * sizeof(int);
+        const size_t part = (size_t)c->pairs * 2 * 128 * AT_LATENT * 4, ml = (size_t)c->pairs * 2 * 128 * 8;
         char* w = nullptr;
-        LK_CU(cudaMalloc((void**)&w, part + ml + sync));
-        if (cudaMemsetAsync(w + part + ml, 0, sync, (cudaStream_t)stream) != cudaSuccess) { cudaFree(w); return set_err(c, LK_ERR_CUDA, "cudaMemsetAsync"); }
-        c->work = TreeWork{ (float4*)w, (float2*)(w + part), (int*)(w + part + ml) };
+        LK_CU(cudaMalloc((void**)&w, part + ml + tree_sched_bytes()));
+        c->work = TreeWork{ (float4*)w, (float2*)(w + part), (Sched*)(w + part + ml) };
     }
     LK_CU(launch_tree(p, cache->dtype, map, c->work, c->pairs, (cudaStream_t)stream));
     return LK_OK;

@@ -52,13 +52,15 @@ struct TreeParams {
     const float* weight; float decay;              // mass
     int* err;
 };
-// parts of items that more than one pair of CTAs works on (attn_tree.cu)
+// parts of items that more than one pair of CTAs works on, and the call's cuts (attn_tree.cu)
+struct Sched;
 struct TreeWork {
     float4* part;              // [2 per pair][16 groups of 8 rows][512 / 4][8 rows]: O, not yet divided by the sum
     float2* ml;                // [2 per pair][128 rows]: reference and sum
-    int* sync;                 // [2][pairs]: CTAs that have left their part of an item, and that have read all of them; zero between calls
+    Sched* sched;
 };
-int tree_pairs(int nsm);       // pairs of CTAs that run at once on the current device
+int tree_pairs(int nsm);       // pairs of CTAs of a launch
+size_t tree_sched_bytes();
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st);
 cudaError_t launch_mass(const TreeParams& p, int dtype, int nsm, cudaStream_t st);
 

@@ -9,7 +9,10 @@
 namespace lk {
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+// The .aligned forms below (barriers, tensor-memory loads and stores) are undefined in a diverged warp, and a warp may
+// leave a polling loop (wait_phase) lane by lane: each is preceded by __syncwarp().
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // the shared::cluster address of the same shared variable in CTA `rank` of the cluster
@@ -27,7 +30,7 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
 __device__ __forceinline__ void arrive_expect_at(uint32_t cluster_bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" :: "r"(cluster_bar), "r"(bytes) : "memory");
 }
-// wait for the phase of `parity`; false once WAIT_LIMIT_NS passes (recorded) or another role has given up
+// one thread waits for the phase of `parity`; false once WAIT_LIMIT_NS passes (recorded) or another role has given up
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* err) {
     for (int i = 0; i < 64; ++i) if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long t0 = globaltimer_ns();
@@ -38,13 +41,26 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
     return true;
 }
 
+// the same by a whole warp, converged again afterwards
+__device__ __forceinline__ bool warp_wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* err) {
+    const bool ok = wait_phase(bar, parity, gave_up, err);
+    __syncwarp();
+    return ok;
+}
+
+// barrier 1 of 256 threads, and the same with the OR of a predicate
+__device__ __forceinline__ void group_sync() { __syncwarp(); named_bar_sync(1, 256); }
+__device__ __forceinline__ bool group_or(bool pred) { __syncwarp(); return named_bar_or(1, 256, pred); }
+
 // ---- 2-CTA tcgen05: M = 128 rows are 64 of each CTA, N columns half of each.  The accumulator of a CTA's 64 rows uses
 // all 128 lanes: row i, column n is lane i + 64 * (n >= N/2), column n % (N/2).
 __device__ __forceinline__ void tmem_alloc2(uint32_t* dst_smem, uint32_t ncols) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(dst_smem)), "r"(ncols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+    __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(ncols) : "memory");
 }
 // Operand tiles of 128-byte rows with the 128-byte swizzle (8-row groups of 1 KB; 16-byte column c of row r at c ^ (r % 8)).
@@ -93,6 +109,7 @@ __device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map
 
 // ---- 32 lanes x 32 columns
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    __syncwarp();
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -101,14 +118,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                  : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    __syncwarp();
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
                  :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
                    "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { __syncwarp(); asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);

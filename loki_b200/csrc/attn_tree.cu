@@ -6,7 +6,7 @@
 //
 // Work.  A row is one (token, head); 128 rows of one sequence are an item, 128 cached rows a tile, and (item, tile) a
 // unit of work: 35.7 M products, 147 KB of cache.  All units, numbered item by item, are cut into equal runs, one per
-// pair of CTAs, whatever the batch's lengths; of an item that lies in several runs each leaves its O, m and l, and joins a share of them.
+// pair of CTAs, whatever the batch's lengths; an item that lies in several runs leaves partial O, m and l for k_merge.
 // Lengths are read on the device, so a captured call follows them.
 //
 // Why a pair.  fp32 O is 128 x 512: all of one SM's tensor memory.  A pair halves the rows (2-CTA tcgen05.mma, M = 128:
@@ -21,7 +21,9 @@
 // warp 3 repairs tail tiles, warps 4-11 do softmax, O's scaling and the output (two threads per tensor-memory lane, four per
 // row: with one per lane V waits twice as long in the ring for P).  Order of the ring: K(0), K(1), V(0),
 // K(2), V(1), ..: softmax j runs under S(j + 1).  Two issuing threads because a satisfied barrier wait between two MMAs
-// leaves the tensor pipe empty for ~50 cycles, 11 times a unit: while one thread waits the other's MMAs run.
+// leaves the tensor pipe empty for ~50 cycles, 11 times a unit: while one thread waits the other's MMAs run.  A stage has one
+// "full" barrier for K and one for V: a parity wait is only right for a barrier's next phase, and with a shared one the thread
+// of O, which can reach a stage while the K before it is still on its way (V is in L2 by then), would take that phase for its own.
 //
 // Rows that must not matter: a tile's rows beyond the drafts, and drafted rows that a token does not see, get P = 0; but
 // 0 * NaN is NaN, so warp 3 zeroes the former in the O operand, and every drafted row there that holds a non-finite
@@ -29,104 +31,25 @@
 #include <type_traits>
 #include "attn_tc.cuh"
 #include "attn_sched.cuh"
+#include "moe_internal.h"
 
 namespace lk {
 
 constexpr int TR_THREADS = 384, TR_STAGES = 8, TR_STAGE = 16384, TR_CHUNK = 8192;
 constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + TR_STAGE, TR_BARS = TR_RING + TR_STAGES * TR_STAGE;
-constexpr int TR_XCH = TR_BARS + 48 * 8, TR_SCHED = TR_XCH + 256 * 4;
+constexpr int TR_XCH = TR_BARS + 44 * 8, TR_SCHED = TR_XCH + 256 * 4;
 constexpr int TR_SMEM = TR_SCHED + (int)sizeof(Sched);
 static_assert(TR_SMEM <= 232448, "227 KB a CTA");
 constexpr uint32_t TR_S_COL = 256, TR_TMEM = 512;
 constexpr float TR_SHIFT = 7.0f, TR_JUMP = 8.0f;      // P <= 2^15 fits fp16; its smallest normal is 2^-21 of the reference
 
-// a split item that this CTA left a part of
-struct TreeJoin { int q0, parts, slot0, rows, row0, first; };       // first run, runs, the first part's slot, rows, first row, first token
-
 struct TreeBars {
-    uint64_t full[TR_STAGES], empty[TR_STAGES], land[TR_STAGES];
-    uint64_t s_full[2], s_free[2], p_full, o_done, q_full, joined, drain[2];
+    uint64_t k_full[TR_STAGES], v_full[TR_STAGES], land[TR_STAGES], empty[TR_STAGES];
+    uint64_t s_full[2], s_free[2], p_full, o_done, q_full, drain[2];
     uint32_t tmem;
     int gave_up;
-    TreeJoin join[2];
 };
-static_assert(sizeof(TreeBars) <= 48 * 8, "barrier block");
-
-// ---------------------------------------------------------------- joining the parts of an item
-// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over the item's parts q.  Every CTA that left a part takes an
-// equal share of the item's (8-row group, 4 latent values, row) elements once all parts are there: 128 KB in all, whatever the
-// number of parts, fetched by one bulk copy a part into the memory that Q and the ring had.  They are added in the parts'
-// order, so the result does not depend on who was first.
-constexpr int JN_PARTS = 128, JN_STAGE = 8192;
-
-template <class T>
-__device__ __forceinline__ void tree_join(const TreeParams& p, const TreeWork& wk, const TreeJoin& jn, int cta, int pairs, uint8_t* sm, int tid,
-                                          uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-    const int warp = tid >> 5, lane = tid & 31, n = jn.parts, ctas = 2 * n;
-    float* ref = (float*)sm; float* sum = ref + 128; float* f = sum + 128;      // of the share's rows; f [part][row]
-    const float4* stage = (const float4*)(sm + JN_STAGE);                       // [part][element]
-    auto slot = [&](int i) { return i ? (jn.slot0 & ~1) + 2 * i : jn.slot0; };
-    // this CTA's elements e: row group e / 1024, values 4 (e / 8 % 128), row e % 8
-    const int mine = cta - 2 * jn.q0, all = (jn.rows + 7) / 8 * 1024;
-    const int e0 = (int)((uint32_t)(all * mine) / (uint32_t)ctas), e1 = (int)((uint32_t)(all * (mine + 1)) / (uint32_t)ctas), ne = e1 - e0;
-    const int r0 = e0 >> 10 << 3, nr = ne ? min(jn.rows, ((e1 - 1) >> 10 << 3) + 8) - r0 : 0;
-    if (warp == 0) {
-        if (lane == 0) {
-            const unsigned long long t0 = globaltimer_ns();
-            int seen;
-            do {
-                asm volatile("ld.acquire.gpu.s32 %0, [%1];" : "=r"(seen) : "l"(wk.sync + jn.q0) : "memory");
-                if (seen < ctas && (*gave_up || globaltimer_ns() - t0 > WAIT_LIMIT_NS)) { att_error(p.err, DEV_ERR_TIMEOUT_FULL); *gave_up = 1; break; }
-            } while (seen < ctas);
-            asm volatile("fence.proxy.async;" ::: "memory");                    // the parts were written by ordinary stores
-            mbar_arrive_expect_tx(bar, (uint32_t)(n * ne) * 16);
-        }
-        __syncwarp();
-        if (ne) for (int i = lane; i < n; i += 32) bulk_g2s((void*)(stage + i * ne), wk.part + (int64_t)slot(i) * (128 * 128) + e0, ne * 16, bar);
-    }
-    named_bar_sync(1, 256);
-    for (int r = warp; r < nr; r += 8) {
-        float m = -INFINITY, l = 0.0f;
-        for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&wk.ml[slot(i) * 128 + r0 + r]).x);
-        #pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float rf = m == -INFINITY ? 0.0f : m;
-        for (int i = lane; i < n; i += 32) {
-            const float2 ml = __ldcg(&wk.ml[slot(i) * 128 + r0 + r]);
-            // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
-            const float v = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
-            f[i * nr + r] = v;
-            l += v == 0.0f ? 0.0f : v * ml.y;
-        }
-        #pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) { ref[r] = rf; sum[r] = l; }
-    }
-    named_bar_sync(1, 256);
-    wait_phase(bar, parity, gave_up, p.err);
-    for (int x = tid; x < ne; x += 256) {
-        const int e = e0 + x, r = (e >> 10 << 3) + (e & 7), c4 = (e >> 3) & 127;
-        if (r >= jn.rows) continue;
-        float4 s = make_float4(0, 0, 0, 0);
-        #pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const float4 v = stage[i * ne + x];
-            const float w = f[i * nr + r - r0];
-            s.x += w == 0.0f ? 0.0f : w * v.x;
-            s.y += w == 0.0f ? 0.0f : w * v.y;
-            s.z += w == 0.0f ? 0.0f : w * v.z;
-            s.w += w == 0.0f ? 0.0f : w * v.w;
-        }
-        const int gr = jn.row0 + r, tj = gr / p.H, h = gr - tj * p.H, t = jn.first + tj;
-        const float l = sum[r - r0], inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *(uint2*)((T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + 4 * c4) =
-            make_uint2(pack2<T>(s.x * inv, s.y * inv), pack2<T>(s.z * inv, s.w * inv));
-        if (c4 == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[r - r0] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
-    }
-    if (tid == 0 && atomicAdd(wk.sync + pairs + jn.q0, 1) == ctas - 1) { wk.sync[jn.q0] = 0; wk.sync[pairs + jn.q0] = 0; }
-    fence_async_smem();                                // the next join's copies come after these reads
-    named_bar_sync(1, 256);
-}
+static_assert(sizeof(TreeBars) <= 44 * 8, "barrier block");
 
 // the load role of one CTA, one thread: boxes of BOX rows x 64 values.  Its instructions are the loop's length (a loaded
 // stage feeds 512 cycles of MMAs), so the page lookups are made a tile ahead and nothing is computed per box.
@@ -134,7 +57,8 @@ template <int BOX>
 __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sched, int64_t u, int64_t u_end, const CUtensorMap* map,
                                           TreeBars& B, uint32_t smb, uint32_t rank) {
     constexpr int NB = 64 / BOX;                          // boxes of 64 rows
-    const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
+    constexpr uint32_t V = sizeof(B.k_full);              // from a stage's k_full to its v_full
+    const uint32_t full0 = peer_addr(smem_u32(&B.k_full[0]), 0);
     uint32_t st = 0, ph = 1, dst = smb + TR_RING, bar = full0;
     auto advance = [&]() {
         dst += TR_STAGE; bar += 8;
@@ -172,9 +96,9 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sche
                 #pragma unroll
                 for (int s = 0; s < 4; ++s) {             // column group s / 2, row half s % 2
                     if (!wait_phase(&B.empty[st], ph, &B.gave_up, p.err)) return false;
-                    uint32_t to = bar;
+                    uint32_t to = bar + V;
                     if (tail) { to = smem_u32(&B.land[st]); mbar_arrive_expect_tx(&B.land[st], TR_STAGE); }
-                    else arrive_expect_at(bar, TR_STAGE);
+                    else arrive_expect_at(to, TR_STAGE);
                     const int col = (s >> 1) * 256 + (int)rank * 128;
                     #pragma unroll
                     for (int c = 0; c < 2; ++c)
@@ -203,19 +127,22 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 
     if (warp == 2 && lane == 0) {
         B.gave_up = 0;
-        for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], 1); mbar_init(&B.land[s], 1); }
+        for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.k_full[s], 2); mbar_init(&B.v_full[s], 2); mbar_init(&B.land[s], 1); mbar_init(&B.empty[s], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 16); mbar_init(&B.drain[i], 1); }
-        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, 16); mbar_init(&B.joined, 1);
+        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, 16);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
     if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE>(p, sched, tid, TR_THREADS, pairs);
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = B.tmem;
+    pdl_trigger();
+    if (blockIdx.x == 0) for (int i = tid; i < (int)(sizeof(Sched) / 4); i += TR_THREADS) ((int*)wk.sched)[i] = ((const int*)&sched)[i];
     int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
     const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
     const uint32_t smb = smem_u32(sm);
@@ -232,10 +159,11 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both: S and O by a thread each
         if (rank == 0 && elect_one()) {
             constexpr uint32_t id_s = att_idesc(128, 128, BF, false), id_o = att_idesc(128, 256, BF, true);
-            uint32_t st = 0, ph = 0, n = 0, n_q = 0;      // ring place; tiles and segments so far
+            uint32_t st = 0, uses = 0, n = 0, n_q = 0;    // ring place; parity of this thread's uses of each stage; tiles, segments
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = wait_phase(bar, parity, gave_up, p.err); };
-            auto advance = [&](uint32_t k) { st += k; if (st >= TR_STAGES) { st -= TR_STAGES; ph ^= 1; } };
+            auto advance = [&](uint32_t k) { st = (st + k) % TR_STAGES; };
+            auto wait_stage = [&](uint64_t* full) { const bool got = wait(&full[st], (uses >> st) & 1); uses ^= 1u << st; return got; };
             if (warp == 1) {
                 for (Segment g; ok && sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
                     if (!wait(&B.q_full, n_q++ & 1)) break;
@@ -244,7 +172,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                         if (!wait(&B.s_free[buf], ((n >> 1) & 1) ^ 1)) break;
                         tc_fence_after();
                         for (int s = 0; s < 5; ++s) {
-                            if (!wait(&B.full[st], ph)) break;
+                            if (!wait_stage(B.k_full)) break;
                             const uint32_t kb = smb + TR_RING + st * TR_STAGE, qb = smb + TR_Q + 2 * s * TR_CHUNK;
                             umma2_x4<id_s, 32, 32>(d, sw128_lo(qb, 16), sw128_lo(kb, 16), s != 0);
                             if (s < 4) umma2_x4<id_s, 32, 32>(d, sw128_lo(qb + TR_CHUNK, 16), sw128_lo(kb + TR_CHUNK, 16), 1);
@@ -265,7 +193,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                         if (!wait(&B.p_full, n & 1)) break;
                         tc_fence_after();
                         for (int s = 0; s < 4; ++s) {
-                            if (!wait(&B.full[st], ph)) break;
+                            if (!wait_stage(B.v_full)) break;
                             const uint32_t vb = smb + TR_RING + st * TR_STAGE, pb = smb + TR_P + (s & 1) * TR_CHUNK;
                             umma2_x4<id_o, 32, 2048>(tmem + (s >> 1) * 128, sw128_lo(pb, 16), sw128_lo(vb, TR_CHUNK), j > g.t0 || (s & 1));
                             commit2(&B.empty[st]);
@@ -284,7 +212,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         }
     } else if (warp < 4) {
         // ---------------------------------------------------------------- repair of the O operand's tail tiles
-        const uint32_t full0 = peer_addr(smem_u32(&B.full[0]), 0);
+        const uint32_t full0 = peer_addr(smem_u32(&B.v_full[0]), 0);
         uint32_t st = 0, uses = 0;                        // bit s: parity of the uses of land[s]
         auto advance = [&](int n) { st = (st + n) % TR_STAGES; };
         for (Segment g; sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
@@ -293,7 +221,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 if (j == g.t0) continue;
                 if (j * ATT_TILE <= g.len) { advance(4); continue; }
                 for (int s = 0; s < 4; ++s, advance(1)) {
-                    wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err);
+                    warp_wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err);
                     uses ^= 1u << st;
                     // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each: eight lanes a row.  Each row's part is judged by
                     // itself: all that matters is that nothing non-finite is multiplied by 0
@@ -327,8 +255,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                        q_full0 = peer_addr(smem_u32(&B.q_full), 0);
         const float scale2 = p.scale * 1.4426950408889634f;
         uint32_t n = 0;                                   // tiles so far
-        int parts = 0;                                    // split items so far
-        auto wait = [&](uint64_t* bar, uint32_t parity) { wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); };
+        auto wait = [&](uint64_t* bar, uint32_t parity) { warp_wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); };
         // Q of a segment: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 8 rows a warp, whose places in q
         // the lanes that own the rows know
         auto start_q = [&](const Segment& g) {
@@ -384,9 +311,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 #pragma unroll
                 for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-                if (named_bar_or(1, 256, top > m + TR_JUMP)) {
+                if (group_or(top > m + TR_JUMP)) {
                     xch[part * 64 + row] = top;
-                    named_bar_sync(1, 256);
+                    group_sync();
                     const float m1 = fmaxf(fmaxf(m, fmaxf(xch[row], xch[64 + row])), fmaxf(xch[128 + row], xch[192 + row]));
                     const float f = m1 == m ? 1.0f : exp2_approx(m - m1);  // m = -inf: 0
                     l *= f;
@@ -404,7 +331,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                         tmem_wait_st();
                         tc_fence_before();
                     }
-                    named_bar_sync(1, 256);               // xch is free again
+                    group_sync();               // xch is free again
                 }
                 const float ref = (m == -INFINITY ? 0.0f : m) - TR_SHIFT;
                 uint32_t e2[16];
@@ -432,9 +359,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             wait(&B.o_done, (n - 1) & 1);
             if (more) finish_q();
             xch[part * 64 + row] = l;
-            named_bar_sync(1, 256);
+            group_sync();
             l = (xch[row] + xch[64 + row]) + (xch[128 + row] + xch[192 + row]);
-            named_bar_sync(1, 256);
+            group_sync();
             const float ref = (m == -INFINITY ? 0.0f : m) - TR_SHIFT;
             if (g.whole()) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -469,55 +396,111 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                             to[(c + i) * 2] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                 }
                 if (live && part == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
-                const int q0 = sched.owner(g.item);
-                if (tid == 128) {
-                    TreeJoin& jn = B.join[parts];
-                    jn.q0 = q0;
-                    jn.parts = sched.owner(g.item + g.tiles - 1) - q0 + 1;
-                    jn.slot0 = 2 * q0 + (g.item > sched.run_start(q0));
-                    jn.rows = min(ATT_ITEM, g.n * p.H - g.rt * ATT_ITEM);
-                    jn.row0 = g.rt * ATT_ITEM;
-                    jn.first = g.first;
-                }
-                ++parts;
-                __threadfence();
-                named_bar_sync(1, 256);
-                if (tid == 128) atomicAdd(wk.sync + q0, 1);
             }
             tc_fence_before();
             g = next;
         }
-        for (int i = 0; i < parts; ++i) tree_join<T>(p, wk, B.join[i], 2 * pair + (int)rank, pairs, sm, tid - 128, &B.joined, i, gave_up);
     }
+    __syncwarp();                                         // the single-thread roles' warps
     tc_fence_before();
     __syncthreads();
     cluster_sync();
     if (warp == 3) { tc_fence_after(); tmem_dealloc2(tmem, TR_TMEM); }
 }
 
-int tree_pairs(int nsm) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = nsm / 2 * 2; cfg.blockDim = TR_THREADS; cfg.dynamicSmemBytes = TR_SMEM; cfg.attrs = attr; cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaFuncSetAttribute(k_tree<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_tree<__half>, &cfg) != cudaSuccess) { cudaGetLastError(); return 0; }
-    n = n < nsm / 2 ? n : nsm / 2;
-    return n < JN_PARTS ? n : JN_PARTS;
+// ---------------------------------------------------------------- joining split items
+// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q, added in a fixed order.  A CTA takes
+// 8 rows of an item (a part's 128-byte lines) x 64 latent values; its 4 groups of 128 threads take every fourth part.  Items
+// that one run finished were written by k_tree.
+constexpr int MG_ROWS = 8, MG_C4 = 16, MG_GROUPS = 4, MG_ELEMS = MG_ROWS * MG_C4, MG_THREADS = MG_ELEMS * MG_GROUPS, MG_PARTS = 128;
+
+__device__ __forceinline__ float4 load_cg(const float4* p) {      // volatile: not moved behind a test of its weight
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
 }
+
+template <class T>
+__global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk) {
+    __shared__ float4 acc[MG_GROUPS][MG_ELEMS];
+    __shared__ float f[MG_PARTS][MG_ROWS];
+    __shared__ float ref[MG_ROWS], sum[MG_ROWS];
+    pdl_wait();
+    const Sched& s = *wk.sched;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // sequence b's groups of 8 rows are numbered from start[b] * H / 8 + b on: the last b whose first number is not above ours
+    int b = 0;
+    for (int lo = 1, hi = p.kv.n_seqs - 1; lo <= hi;) {
+        const int mid = (lo + hi) >> 1;
+        if ((int)((int64_t)s.start[mid] * p.H / MG_ROWS) + mid <= (int)blockIdx.x) { b = mid; lo = mid + 1; } else hi = mid - 1;
+    }
+    const int first = s.start[b], rows = (s.start[b + 1] - first) * p.H, row0 = (blockIdx.x - ((int)((int64_t)first * p.H / MG_ROWS) + b)) * MG_ROWS;
+    const int64_t units = s.prefix[b + 1] - s.prefix[b];
+    if (units == 0 || row0 < 0 || row0 >= rows) return;
+    const int64_t tiles = div_small(units, (rows + ATT_ITEM - 1) / ATT_ITEM), u0 = s.prefix[b] + row0 / ATT_ITEM * tiles;
+    const int q0 = s.owner(u0), n = s.owner(u0 + tiles - 1) - q0 + 1, pr0 = row0 % ATT_ITEM, nr = min(MG_ROWS, rows - row0);
+    if (n < 2) return;
+    const int slot0 = 2 * q0 + (u0 > s.run_start(q0));
+    auto slot = [&](int i) { return i ? (slot0 & ~1) + 2 * i : slot0; };
+    if (warp < nr) {                                    // the factors of one row
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]).x);
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float rf = m == -INFINITY ? 0.0f : m;
+        for (int i = lane; i < n; i += 32) {
+            const float2 ml = __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]);
+            // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
+            const float v = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
+            f[i][warp] = v;
+            l += v == 0.0f ? 0.0f : v * ml.y;
+        }
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) { ref[warp] = rf; sum[warp] = l; }
+    }
+    const int e = tid % MG_ELEMS, grp = tid / MG_ELEMS, r = e % MG_ROWS, c4 = blockIdx.y * MG_C4 + e / MG_ROWS;
+    const float4* src = wk.part + pr0 / 8 * 1024 + c4 * 8 + r;
+    float4 a = make_float4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i0 = grp; i0 < n; i0 += 8 * MG_GROUPS) {
+        float4 v[8];
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) if (i0 + k * MG_GROUPS < n) v[k] = load_cg(src + (int64_t)slot(i0 + k * MG_GROUPS) * (128 * 128));
+        #pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i0 + k * MG_GROUPS < n && r < nr) {
+                const float w = f[i0 + k * MG_GROUPS][r];
+                if (w != 0.0f) { a.x += w * v[k].x; a.y += w * v[k].y; a.z += w * v[k].z; a.w += w * v[k].w; }
+            }
+    }
+    acc[grp][e] = a;
+    __syncthreads();
+    if (grp || r >= nr) return;
+    a = make_float4(0, 0, 0, 0);
+    #pragma unroll
+    for (int q = 0; q < MG_GROUPS; ++q) {
+        const float4 v = acc[q][e];
+        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    const int tj = (row0 + r) / p.H, h = row0 + r - tj * p.H, t = first + tj;
+    const float l = sum[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *(uint2*)((T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + 4 * c4) =
+        make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+    if (c4 == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[r] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+}
+
+int tree_pairs(int nsm) { return nsm / 2 < MG_PARTS ? nsm / 2 : MG_PARTS; }
+size_t tree_sched_bytes() { return sizeof(Sched); }
 
 template <class T>
 static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeCooperative;      // pairs wait for one another's parts: all of them run at once
-    attr[0].val.cooperative = 1;
-    cfg.gridDim = 2 * pairs; cfg.blockDim = TR_THREADS; cfg.dynamicSmemBytes = TR_SMEM; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_tree<T>, p, map, wk);
+    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const unsigned groups = (unsigned)((int64_t)p.T * p.H / MG_ROWS) + p.kv.n_seqs;
+    return launch_pdl_n(k_merge<T>, dim3(groups, AT_LATENT / 4 / MG_C4), dim3(MG_THREADS), 0, st, p, wk);
 }
 
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {

@@ -489,3 +489,26 @@ def test_no_tokens(A, ctx):
     assert out.shape == (0, 4, 512) and lse.shape == (0, 4)
     x = ctx.rope(torch.empty(0, 2, 64, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), A.RopeTable(4, 64, device="cuda"))
     assert x.shape == (0, 2, 64)
+
+
+def test_repeated_calls_over_caches_beyond_l2(A):
+    """Back-to-back calls that alternate between contexts whose caches come from memory, not L2 (the key half of a tile
+    arrives long after the value half of the one before): every call gives the first one's bits."""
+    H, T = 128, 1
+    sets = []
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        n_pages = 480
+        rows = torch.randn(n_pages * 64, R.ROW, generator=g, device="cuda").to(torch.bfloat16)
+        table = torch.randperm(n_pages, generator=g, device="cuda").int()[None].contiguous()
+        cache = A.KvCache(rows, 64, table, torch.tensor([30011 + 100 * seed], dtype=torch.int32, device="cuda"))
+        q = torch.randn(T, H, R.ROW, generator=g, device="cuda").to(torch.bfloat16)
+        sets.append((A.AttnContext(0, 1, 1), cache, q, torch.tensor([0, T], dtype=torch.int32, device="cuda")))
+    first = [c.tree(q, k, s, None, SCALE) for c, k, q, s in sets]
+    torch.cuda.synchronize()
+    got = [sets[i % 3][0].tree(sets[i % 3][2], sets[i % 3][1], sets[i % 3][3], None, SCALE) for i in range(300)]
+    for i, (o, l) in enumerate(got):
+        assert torch.equal(o, first[i % 3][0]) and torch.equal(l, first[i % 3][1])
+    for c, *_ in sets:
+        c.device_error()
+        c.close()
