@@ -229,7 +229,9 @@ int lk_attn_mass(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     if (!lse) return set_err(c, LK_ERR_ARG, "null lse");
     OnDevice on(c->device);
     p.lse = const_cast<float*>(lse); p.weight = weight; p.decay = decay;
-    LK_CU(launch_mass(p, cache->dtype, c->nsm, (cudaStream_t)stream));
+    CUtensorMap map;
+    if (int rc = encode_map(c, cache, &map)) return rc;
+    LK_CU(launch_mass(p, cache->dtype, map, c->nsm / 2, (cudaStream_t)stream));
     return LK_OK;
 }
 

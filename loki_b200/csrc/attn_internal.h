@@ -62,7 +62,7 @@ struct TreeWork {
 int tree_pairs(int nsm);       // pairs of CTAs of a launch
 size_t tree_sched_bytes();
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st);
-cudaError_t launch_mass(const TreeParams& p, int dtype, int nsm, cudaStream_t st);
+cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, int pairs, cudaStream_t st);
 
 struct EvictParams {
     KvView kv;

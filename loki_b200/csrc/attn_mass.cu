@@ -1,75 +1,260 @@
 // attn_mass.cu -- the attention weight that every cached row received:
 //   mass[k] = decay * mass[k] + sum_t w_t sum_h exp(scale q_th . row_k - lse_th).
-// The sum runs over the rows of the score matrix, so the known lse lets each key add its terms alone: a CTA owns 32
-// keys (one per lane), its warps share out the (token, head) rows, and the partial sums are added in a fixed order.
-#include "attn_internal.h"
+//
+// The sum runs over the rows of the score matrix, so with the lse known each key adds its terms alone.  The products are
+// S^T = K Q^T: a pair of CTAs holds 256 keys (M = 256: 128 each, the tensor-memory lanes) and runs over the (token, head) rows
+// in blocks of up to 256 (N); a key's scores then lie in one lane, and its sum is a loop over columns without any exchange.
+// w exp(s - lse) = 2^(s' - c), c = lse / ln 2 - log2 w; tokens without a positive weight are left out of the rows.  One owner
+// adds a key's terms in a fixed order: nothing depends on timing.
+//
+// Bounds: 2 x 256 x 256 x 576 products of a block take 4608 cycles of both tensor pipes, its 65 536 exponentials 2048 cycles of
+// each SM's; Q is re-read per key tile (16 KB per 512 cycles and SM, from L2).  With one block (a decoded token) the cache's
+// 1152 bytes a key from HBM are the bound.
+//
+// The key tile stays in shared memory (9 chunks of 64 values, 144 KB); each chunk is replaced as soon as the last row block has
+// read it, so the next tile's loads run under the rest.  Q chunks go through a ring of 4 (16 KB: the CTA's half of the rows x 64
+// values).  Roles (512 threads): warp 0 loads K (TMA), warp 1 of CTA 0 issues the MMAs, warps 4-7 load Q, warps 8-15 add.
+#include <type_traits>
+#include "attn_tc.cuh"
+#include "attn_sched.cuh"
 
 namespace lk {
 
-constexpr int MS_K = 32, MS_WARPS = 8;
-constexpr int MS_LD = AT_ROW + 1;
+constexpr int MS_THREADS = 512, MS_TILE = 256, MS_ROWS = 256, MS_CHUNK = 16384, MS_RING = 4, MS_LAG = 2;
+constexpr int MS_Q = 9 * MS_CHUNK, MS_BARS = MS_Q + MS_RING * MS_CHUNK, MS_COL = MS_BARS + 48 * 8;
+constexpr int MS_TOK = MS_COL + 2 * MS_ROWS * 4, MS_PART = MS_TOK + 2 * MS_ROWS, MS_ACT = MS_PART + 128 * 4, MS_MASK = MS_ACT + 64 * 4;
+constexpr int MS_SCHED = MS_MASK + 64 * 8;
+constexpr int MS_SMEM = MS_SCHED + (int)sizeof(Sched);
+static_assert(MS_SMEM <= 232448 && MS_SCHED % 8 == 0, "227 KB a CTA");
+
+struct MassBars {
+    uint64_t k_full[9], k_empty[9], q_full[MS_RING], q_empty[MS_RING], d_full[2], d_free[2], drain;
+    uint32_t tmem;
+    int gave_up, n_act;
+};
+static_assert(sizeof(MassBars) <= 48 * 8, "barrier block");
+
+// columns of the MMA for `rows` rows of a block
+__device__ __forceinline__ int mass_cols(int rows) { return (min(rows, MS_ROWS) + 31) & ~31; }
 
 template <class T>
-__global__ void __launch_bounds__(MS_WARPS * 32) k_mass(TreeParams p) {
-    extern __shared__ float sm[];
-    float* K = sm;                                  // [32][577]: lanes read one column of 32 rows without conflicts
-    float* part = K + MS_K * MS_LD;                 // [8][32]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int item = blockIdx.x;                          // tiles of all sequences, numbered in order
-    for (int b = 0; b < p.kv.n_seqs; ++b) {
-        const int len = kv_len(p.kv, b, p.err);
-        const int2 sp = seq_tokens(p.starts, b, p.T, len, p.kv, p.err);
-        const int total = sp.y ? len + sp.y : 0, tiles = (total + MS_K - 1) / MS_K;
-        for (; item < tiles; item += gridDim.x) {
-            const int k0 = item * MS_K;
-            __syncthreads();
-            for (int r = warp; r < MS_K; r += MS_WARPS) {
-                const int slot = k0 + r < total ? kv_slot(p.kv, b, k0 + r, p.err) : -1;
-                for (int c = lane; c < AT_ROW; c += 32)
-                    K[r * MS_LD + c] = slot < 0 ? 0.0f : to_f<T>(((const T*)p.kv.rows)[(int64_t)slot * p.kv.row_stride + c]);
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MS_THREADS, 1)
+k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map) {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    MassBars& B = *(MassBars*)(sm + MS_BARS);
+    float* col = (float*)(sm + MS_COL);                       // [2][256] c of each row of a block
+    uint8_t* tok = sm + MS_TOK;                               // [2][256] its token's place in act
+    float* part = (float*)(sm + MS_PART);                     // [128]
+    int* act = (int*)(sm + MS_ACT);                           // the segment's tokens of positive weight (within the sequence)
+    uint64_t* see = (uint64_t*)(sm + MS_MASK);                // the drafted rows that each of them sees
+    Sched& sched = *(Sched*)(sm + MS_SCHED);
+    volatile int* gave_up = &B.gave_up;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+
+    if (warp == 2 && lane == 0) {
+        B.gave_up = 0;
+        for (int i = 0; i < 9; ++i) { mbar_init(&B.k_full[i], 2); mbar_init(&B.k_empty[i], 1); }
+        for (int i = 0; i < MS_RING; ++i) { mbar_init(&B.q_full[i], 8); mbar_init(&B.q_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&B.d_full[i], 1); mbar_init(&B.d_free[i], 16); }
+        mbar_init(&B.drain, 1);
+        fence_mbar_init();
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
+    }
+    if (warp == 3) tmem_alloc2(&B.tmem, 512);
+    if (warp == 0 || p.kv.n_seqs > 1) sched_load<MS_TILE, false>(p, sched, tid, MS_THREADS, pairs);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = B.tmem, smb = smem_u32(sm);
+    int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
+    const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
+    uint32_t n_tile = 0, n_q = 0, n_d = 0;                    // this role's key tiles, Q chunks and row blocks so far
+    bool ok = true;
+
+    for (Segment g; sched_next<MS_TILE>(p, sched, u, u_end, g);) {
+        __syncthreads();                                      // act of the last segment is free
+        if (warp == 2) {
+            int n = 0;
+            for (int j0 = 0; j0 < g.n; j0 += 32) {
+                const int j = j0 + lane;
+                const bool in = j < g.n && (!p.weight || p.weight[g.first + j] > 0.0f);
+                const uint32_t m = __ballot_sync(0xffffffffu, in);
+                const int at = n + __popc(m & ((1u << lane) - 1));
+                if (in) { act[at] = j; see[at] = node_mask(p.tree, g.first + j, j, g.n); }
+                n += __popc(m);
             }
-            __syncthreads();
-            const int i = k0 + lane;
-            float acc = 0.0f;
-            for (int j = 0; j < sp.y; ++j) {
-                const int t = sp.x + j;
-                const float w = p.weight ? p.weight[t] : 1.0f;
-                if (w == 0.0f) continue;
-                const uint64_t mask = node_mask(p.tree, t, j, sp.y);
-                const bool see = i < len || (i < total && ((mask >> (i - len)) & 1));
-                float sum = 0.0f;
-                for (int h = warp; h < p.H; h += MS_WARPS) {
-                    const T* q = (const T*)p.q + t * p.q_token + h * p.q_head;
-                    float s = 0.0f;
-                    for (int c = 0; c < AT_ROW; ++c) s += to_f<T>(q[c]) * K[lane * MS_LD + c];
-                    if (see) sum += expf(s * p.scale - p.lse[(int64_t)t * p.H + h]);
+            if (lane == 0) B.n_act = n;
+        }
+        __syncthreads();
+        const int rows = B.n_act * p.H, blocks = (rows + MS_ROWS - 1) / MS_ROWS;
+
+        if (warp == 0) {
+            // ---------------------------------------------------------------- K: 128 keys of this CTA, 9 chunks a tile
+            if (blocks && elect_one()) {
+                const uint32_t full0 = peer_addr(smem_u32(&B.k_full[0]), 0);
+                const int box = min(p.kv.page_size, 64);
+                for (int j = g.t0; ok && j < g.t1; ++j, ++n_tile) {
+                    int row[8];                               // pool rows of the boxes; those beyond the drafts read the last page again
+                    #pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        row[x] = (x * 16 & (box - 1)) == 0 ? max(0, kv_slot(p.kv, g.b, min(j * MS_TILE + (int)rank * 128 + x * 16, (g.total - 1) & ~15), p.err)) : 0;
+                    for (int c = 0; c < 9; ++c) {
+                        if (!(ok = wait_phase(&B.k_empty[c], (n_tile & 1) ^ 1, gave_up, p.err))) break;
+                        arrive_expect_at(full0 + 8 * c, MS_CHUNK);
+                        #pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            if ((x * 16 & (box - 1)) == 0) tma_2d_pair(smb + c * MS_CHUNK + x * 2048, &kv_map, c * 64, row[x], full0 + 8 * c);
+                    }
                 }
-                acc += w * sum;
+                if (!ok) __nanosleep(1000000);                // given up: the loads in flight land before the CTA ends
             }
-            part[warp * 32 + lane] = acc;
-            __syncthreads();
-            if (warp == 0 && i < total) {
-                float a = 0.0f;
-                for (int w = 0; w < MS_WARPS; ++w) a += part[w * 32 + lane];
-                const int slot = kv_slot(p.kv, b, i, p.err);
-                if (slot >= 0) p.kv.mass[slot] = p.decay * p.kv.mass[slot] + a;
+        } else if (warp == 1) {
+            // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both
+            if (rank == 0 && elect_one()) {
+                auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = wait_phase(bar, parity, gave_up, p.err); };
+                for (int j = g.t0; ok && j < g.t1; ++j, ++n_tile)
+                    for (int b = 0; ok && b < blocks; ++b, ++n_d) {
+                        const uint32_t buf = n_d & 1, d = tmem + buf * 256;
+                        const uint32_t idesc = att_idesc(256, 0, BF, false) | ((uint32_t)(mass_cols(rows - b * MS_ROWS) >> 3) << 17);
+                        if (!wait(&B.d_free[buf], ((n_d >> 1) & 1) ^ 1)) break;
+                        tc_fence_after();
+                        for (int c = 0; c < 9; ++c, ++n_q) {
+                            const uint32_t st = n_q % MS_RING;
+                            if (b == 0 && !wait(&B.k_full[c], n_tile & 1)) break;
+                            if (!wait(&B.q_full[st], (n_q / MS_RING) & 1)) break;
+                            umma2_x4_n(d, sw128_lo(smb + c * MS_CHUNK, 16), sw128_lo(smb + MS_Q + st * MS_CHUNK, 16), idesc, c != 0);
+                            commit2(&B.q_empty[st]);
+                            if (b == blocks - 1) commit2(&B.k_empty[c]);
+                        }
+                        if (!ok) break;
+                        commit2(&B.d_full[buf]);
+                    }
+                if (!ok) { commit2(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
+            }
+        } else if (warp >= 4 && warp < 8) {
+            // ---------------------------------------------------------------- Q: this CTA's half of a block's rows, 64 values a stage
+            // 8 lanes a row and 16 rows a pass of the four warps; a stage is passed on MS_LAG stages later, once its copies are in
+            const uint32_t full0 = peer_addr(smem_u32(&B.q_full[0]), 0);
+            auto pass_on = [&](uint32_t k) { fence_async_smem(); __syncwarp(); if (lane == 0) arrive_at(full0 + 8 * (k % MS_RING)); };
+            uint32_t passed = n_q;
+            for (int j = g.t0; j < g.t1; ++j)
+                for (int b = 0; b < blocks; ++b) {
+                    const int half = mass_cols(rows - b * MS_ROWS) / 2;
+                    int64_t at[8];
+                    #pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = k * 16 + (warp - 4) * 4 + (lane >> 3), gr = b * MS_ROWS + (int)rank * half + r, a = gr / p.H;
+                        at[k] = r < half && gr < rows ? (g.first + act[a]) * p.q_token + (gr - a * p.H) * p.q_head + (lane & 7) * 8 : -1;
+                    }
+                    for (int c = 0; c < 9; ++c, ++n_q) {
+                        warp_wait_phase(&B.q_empty[n_q % MS_RING], ((n_q / MS_RING) & 1) ^ 1, gave_up, p.err);
+                        const uint32_t to = smb + MS_Q + (n_q % MS_RING) * MS_CHUNK;
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int r = k * 16 + (warp - 4) * 4 + (lane >> 3);
+                            const T* src = (const T*)p.q + max(at[k], (int64_t)0) + (at[k] < 0 ? 0 : c * 64);
+                            if (k * 16 < half)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                             :: "r"(to + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), "l"(src), "r"(at[k] < 0 ? 0 : 16) : "memory");
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        if (n_q - passed >= MS_LAG) { asm volatile("cp.async.wait_group %0;" :: "n"(MS_LAG) : "memory"); pass_on(passed++); }
+                    }
+                }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            while (passed != n_q) pass_on(passed++);
+        } else if (warp >= 8) {
+            // ---------------------------------------------------------------- sums: lane = key; the two groups of four warps take
+            // every other 32 columns.  A wait that gives up is not acted on: the loops end.
+            const int t8 = tid - 256, L = t8 & 127, grp = t8 >> 7;
+            const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+            const uint32_t d_free0 = peer_addr(smem_u32(&B.d_free[0]), 0);
+            const float scale2 = p.scale * 1.4426950408889634f;
+            for (int j = g.t0; j < g.t1; ++j) {
+                const int key = j * MS_TILE + (int)rank * 128 + L, node = key - g.len;
+                const bool tail = j * MS_TILE + (int)rank * 128 + 127 >= g.len;
+                float acc[4] = { 0, 0, 0, 0 };
+                for (int b = 0; b < blocks; ++b, ++n_d) {
+                    const uint32_t buf = n_d & 1;
+                    {                                         // c of column t8
+                        const int gr = b * MS_ROWS + t8, a = gr / p.H;
+                        float c = INFINITY;                   // no row: 2^-inf
+                        if (gr < rows) {
+                            const int t = g.first + act[a];
+                            const float lse = p.lse[(int64_t)t * p.H + gr - a * p.H];
+                            if (lse != -INFINITY) c = lse * 1.4426950408889634f - (p.weight ? log2f(p.weight[t]) : 0.0f);
+                        }
+                        col[buf * MS_ROWS + t8] = c;
+                        tok[buf * MS_ROWS + t8] = (uint8_t)min(a, 63);
+                    }
+                    group_sync();
+                    warp_wait_phase(&B.d_full[buf], (n_d >> 1) & 1, gave_up, p.err);
+                    tc_fence_after();
+                    const int cols = mass_cols(rows - b * MS_ROWS);
+                    for (int c0 = grp * 32; c0 < cols; c0 += 64) {
+                        uint32_t s[32];
+                        tmem_ld32(tmem + lane_base + buf * 256 + c0, s);
+                        tmem_wait_ld();
+                        const float4* c4 = (const float4*)(col + buf * MS_ROWS + c0);
+                        if (!tail) {
+                            #pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 c = c4[i];
+                                acc[0] += exp2_approx(fmaf(__uint_as_float(s[4 * i]), scale2, -c.x));
+                                acc[1] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 1]), scale2, -c.y));
+                                acc[2] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 2]), scale2, -c.z));
+                                acc[3] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 3]), scale2, -c.w));
+                            }
+                        } else {
+                            const uint8_t* tk = tok + buf * MS_ROWS + c0;
+                            const int left = rows - b * MS_ROWS - c0;
+                            #pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const bool sees = i < left && (node < 0 || (node < 64 && ((see[tk[i]] >> node) & 1)));
+                                const float e = exp2_approx(fmaf(__uint_as_float(s[i]), scale2, -((const float*)c4)[i]));
+                                acc[i & 3] += sees ? e : 0.0f;
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(d_free0 + 8 * buf);
+                }
+                float a = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                if (grp) part[L] = a;
+                group_sync();
+                if (!grp && key < g.total) {
+                    a += part[L];
+                    const int slot = kv_slot(p.kv, g.b, key, p.err);
+                    if (slot >= 0) p.kv.mass[slot] = p.decay * p.kv.mass[slot] + a;
+                }
+                group_sync();                                 // part is free again
             }
         }
-        item -= tiles;
+        __syncwarp();                                         // the single-thread roles' warps
     }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 3) { tc_fence_after(); tmem_dealloc2(tmem, 512); }
 }
 
 template <class T>
-static cudaError_t mass_go(const TreeParams& p, int nsm, cudaStream_t st) {
-    constexpr int smem = (MS_K * MS_LD + MS_WARPS * 32) * 4;
-    cudaError_t e = cudaFuncSetAttribute(k_mass<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, int pairs, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(k_mass<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MS_SMEM);
     if (e != cudaSuccess) return e;
-    k_mass<T><<<2 * nsm, MS_WARPS * 32, smem, st>>>(p);
+    k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map);
     return cudaGetLastError();
 }
 
-cudaError_t launch_mass(const TreeParams& p, int dtype, int nsm, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? mass_go<__half>(p, nsm, st) : mass_go<__nv_bfloat16>(p, nsm, st);
+cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, int pairs, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? mass_go<__half>(p, map, pairs, st) : mass_go<__nv_bfloat16>(p, map, pairs, st);
 }
 
 }  // namespace lk

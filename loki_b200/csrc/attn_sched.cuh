@@ -37,9 +37,10 @@ struct Segment {
     __device__ __forceinline__ bool whole() const { return t1 - t0 == tiles; }
 };
 
+// ITEMS: a sequence's units are its items x tiles; otherwise its tiles.
 // the whole block calls it (one sequence: its first warp is enough), for at most `pairs` runs and no more than the longest
 // run's length needs; the caller synchronises before sched_next
-template <int TILE>
+template <int TILE, bool ITEMS>
 __device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int tid, int threads, int pairs) {
     for (int b = tid; b < p.kv.n_seqs; b += threads) {
         const int len0 = p.kv.lens[b], t0 = p.starts[b], t1 = p.starts[b + 1], cap = p.kv.table_stride << p.kv.page_shift;
@@ -48,7 +49,7 @@ __device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int ti
         if (len != len0) att_error(p.err, ATT_ERR_LEN);
         if (t0 < 0 || n < 0 || t1 > p.T || n > LK_ATTN_MAX_NODES) att_error(p.err, ATT_ERR_TREE);
         else if (n > cap - len) att_error(p.err, ATT_ERR_LEN);
-        else if (n) units = (int64_t)((n * p.H + ATT_ITEM - 1) / ATT_ITEM) * ((len + n + TILE - 1) / TILE);
+        else if (n) units = (int64_t)(ITEMS ? (n * p.H + ATT_ITEM - 1) / ATT_ITEM : 1) * ((len + n + TILE - 1) / TILE);
         s.len[b] = len;
         s.start[b] = t0;
         if (b == p.kv.n_seqs - 1) s.start[b + 1] = t1;

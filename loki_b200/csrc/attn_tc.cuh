@@ -91,6 +91,20 @@ __device__ __forceinline__ void umma2_x4(uint32_t d_tmem, uint32_t a_lo, uint32_
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t}"
                  :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(accumulate), "n"(SW128_HI), "n"(IDESC), "n"(A_STEP >> 4), "n"(B_STEP >> 4) : "memory");
 }
+// the same with the instruction descriptor in a register, both operands K-major
+__device__ __forceinline__ void umma2_x4_n(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\t"
+                 "setp.ne.b32 p, %3, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+                 "mov.b64 ad, {%1, %4};\n\tmov.b64 bd, {%2, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, p;\n\t"
+                 "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 ad, {al, %4};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t"
+                 "add.u32 al, al, 2;\n\tadd.u32 bl, bl, 2;\n\tmov.b64 ad, {al, %4};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t"
+                 "add.u32 al, al, 2;\n\tadd.u32 bl, bl, 2;\n\tmov.b64 ad, {al, %4};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, q;\n\t}"
+                 :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(accumulate), "n"(SW128_HI), "r"(idesc) : "memory");
+}
 // arrive on this barrier in both CTAs when every tcgen05.mma issued so far has completed
 __device__ __forceinline__ void commit2(uint64_t* bar) {
     asm volatile("{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
