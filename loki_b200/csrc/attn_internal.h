@@ -70,6 +70,7 @@ struct EvictParams {
     const int* next_pos; int* new_lens;
     int* src; int* dst; int* n_moves;              // [n_seqs][region] pool rows, [n_seqs]
     int64_t region;
+    int keys;                                      // keys that a CTA of the selection keeps
     int* err;
 };
 cudaError_t launch_evict(const EvictParams& p, int nsm, cudaStream_t st);
