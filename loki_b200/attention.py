@@ -41,7 +41,7 @@ def _rows(t, name, device, last):
 
 
 def _queue(stream, device):
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 class RopeTable:

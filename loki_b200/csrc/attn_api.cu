@@ -211,8 +211,8 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
         c->pairs = tree_pairs(c->nsm);
         const size_t part = (size_t)c->pairs * 2 * 128 * AT_LATENT * 4, ml = (size_t)c->pairs * 2 * 128 * 8;
         char* w = nullptr;
-        LK_CU(cudaMalloc((void**)&w, part + ml + tree_sched_bytes()));
-        c->work = TreeWork{ (float4*)w, (float2*)(w + part), (Sched*)(w + part + ml) };
+        LK_CU(cudaMalloc((void**)&w, part + ml + c->pairs * sizeof(TreeSplit)));
+        c->work = TreeWork{ (float4*)w, (float2*)(w + part), (TreeSplit*)(w + part + ml) };
     }
     LK_CU(launch_tree(p, cache->dtype, map, c->work, c->pairs, (cudaStream_t)stream));
     return LK_OK;

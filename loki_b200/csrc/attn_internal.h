@@ -52,15 +52,14 @@ struct TreeParams {
     const float* weight; float decay;              // mass
     int* err;
 };
-// parts of items that more than one pair of CTAs works on, and the call's cuts (attn_tree.cu)
-struct Sched;
+// parts of items that more than one pair of CTAs works on (attn_tree.cu)
+struct TreeSplit { int parts, slot0, rows, row0, first, pad[3]; };      // runs, the first part's slot, rows, first row, first token
 struct TreeWork {
     float4* part;              // [2 per pair][16 groups of 8 rows][512 / 4][8 rows]: O, not yet divided by the sum
     float2* ml;                // [2 per pair][128 rows]: reference and sum
-    Sched* sched;
+    TreeSplit* split;          // [pairs] the split item that starts in a run (parts 0: none)
 };
 int tree_pairs(int nsm);       // pairs of CTAs of a launch
-size_t tree_sched_bytes();
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st);
 cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, int pairs, cudaStream_t st);
 

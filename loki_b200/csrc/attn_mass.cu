@@ -64,7 +64,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, 512);
-    if (warp == 0 || p.kv.n_seqs > 1) sched_load<MS_TILE, false>(p, sched, tid, MS_THREADS, pairs);
+    if (warp == 0 || p.kv.n_seqs > 1) sched_load<MS_TILE, 0, false>(p, sched, tid, MS_THREADS, pairs);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -76,7 +76,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     uint32_t n_tile = 0, n_q = 0, n_d = 0;                    // this role's key tiles, Q chunks and row blocks so far
     bool ok = true;
 
-    for (Segment g; sched_next<MS_TILE>(p, sched, u, u_end, g);) {
+    for (Segment g; sched_next<MS_TILE, 0>(p, sched, u, u_end, g);) {
         __syncthreads();                                      // act of the last segment is free
         if (warp == 2) {
             int n = 0;

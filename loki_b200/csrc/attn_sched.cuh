@@ -1,7 +1,8 @@
 // attn_sched.cuh -- equal cuts of a ragged batch's work, made on the device from the lengths.
 //
 // Sequence b has ceil(n_b * H / 128) items of ceil((len_b + n_b) / TILE) tiles; (item, tile) units are numbered sequence by
-// sequence, item by item.  They are cut into `runs` of `base` or base + 1 units, the longer ones first.
+// sequence, item by item, each item's tiles after `lead` units that stand for what a further item costs a pair (Q, the output,
+// an empty pipeline).  They are cut into `runs` of `base` or base + 1 units, the longer ones first.
 #pragma once
 #include "attn_internal.h"
 
@@ -37,10 +38,10 @@ struct Segment {
     __device__ __forceinline__ bool whole() const { return t1 - t0 == tiles; }
 };
 
-// ITEMS: a sequence's units are its items x tiles; otherwise its tiles.
+// ITEMS: a sequence's units are its items x (LEAD + tiles); otherwise LEAD + its tiles.
 // the whole block calls it (one sequence: its first warp is enough), for at most `pairs` runs and no more than the longest
 // run's length needs; the caller synchronises before sched_next
-template <int TILE, bool ITEMS>
+template <int TILE, int LEAD, bool ITEMS>
 __device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int tid, int threads, int pairs) {
     for (int b = tid; b < p.kv.n_seqs; b += threads) {
         const int len0 = p.kv.lens[b], t0 = p.starts[b], t1 = p.starts[b + 1], cap = p.kv.table_stride << p.kv.page_shift;
@@ -49,7 +50,7 @@ __device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int ti
         if (len != len0) att_error(p.err, ATT_ERR_LEN);
         if (t0 < 0 || n < 0 || t1 > p.T || n > LK_ATTN_MAX_NODES) att_error(p.err, ATT_ERR_TREE);
         else if (n > cap - len) att_error(p.err, ATT_ERR_LEN);
-        else if (n) units = (int64_t)(ITEMS ? (n * p.H + ATT_ITEM - 1) / ATT_ITEM : 1) * ((len + n + TILE - 1) / TILE);
+        else if (n) units = (int64_t)(ITEMS ? (n * p.H + ATT_ITEM - 1) / ATT_ITEM : 1) * (LEAD + (len + n + TILE - 1) / TILE);
         s.len[b] = len;
         s.start[b] = t0;
         if (b == p.kv.n_seqs - 1) s.start[b + 1] = t1;
@@ -80,27 +81,30 @@ __device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int ti
 }
 
 // the next segment of [u, u_end): consecutive tiles of one item
-template <int TILE>
+template <int TILE, int LEAD>
 __device__ __forceinline__ bool sched_next(const TreeParams& p, const Sched& s, int64_t& u, int64_t u_end, Segment& g) {
-    if (u >= u_end) return false;
-    int lo = 0, hi = p.kv.n_seqs - 1;                    // the last sequence that starts at or before u: it has units
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s.prefix[mid] <= u) lo = mid; else hi = mid - 1;
+    for (;;) {
+        if (u >= u_end) return false;
+        int lo = 0, hi = p.kv.n_seqs - 1;                // the last sequence that starts at or before u: it has units
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s.prefix[mid] <= u) lo = mid; else hi = mid - 1;
+        }
+        g.b = lo;
+        g.len = s.len[lo];
+        g.first = s.start[lo];
+        g.n = s.start[lo + 1] - g.first;
+        g.total = g.len + g.n;
+        g.tiles = (g.total + TILE - 1) / TILE;
+        const int64_t rem = u - s.prefix[lo];
+        g.rt = rem < LEAD + g.tiles ? 0 : (int)div_small(rem, LEAD + g.tiles);
+        const int at = (int)(rem - (int64_t)g.rt * (LEAD + g.tiles)), end = (int)min((int64_t)(LEAD + g.tiles), at + (u_end - u));
+        g.item = u - at;
+        g.t0 = max(0, at - LEAD);
+        g.t1 = end - LEAD;
+        u += end - at;
+        if (g.t1 > g.t0) return true;
     }
-    g.b = lo;
-    g.len = s.len[lo];
-    g.first = s.start[lo];
-    g.n = s.start[lo + 1] - g.first;
-    g.total = g.len + g.n;
-    g.tiles = (g.total + TILE - 1) / TILE;
-    const int64_t rem = u - s.prefix[lo];
-    g.rt = rem < g.tiles ? 0 : (int)div_small(rem, g.tiles);
-    g.t0 = (int)(rem - (int64_t)g.rt * g.tiles);
-    g.t1 = (int)min((int64_t)g.tiles, g.t0 + (u_end - u));
-    g.item = u - g.t0;
-    u += g.t1 - g.t0;
-    return true;
 }
 
 template <class T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t v);

@@ -40,6 +40,7 @@ constexpr int TR_Q = 0, TR_P = 9 * TR_CHUNK, TR_RING = TR_P + TR_STAGE, TR_BARS 
 constexpr int TR_XCH = TR_BARS + 44 * 8, TR_SCHED = TR_XCH + 256 * 4;
 constexpr int TR_SMEM = TR_SCHED + (int)sizeof(Sched);
 static_assert(TR_SMEM <= 232448, "227 KB a CTA");
+constexpr int TR_LEAD = 3;                            // a further item of a run costs about as much as three tiles (4 us)
 constexpr uint32_t TR_S_COL = 256, TR_TMEM = 512;
 constexpr float TR_SHIFT = 7.0f, TR_JUMP = 8.0f;      // P <= 2^15 fits fp16; its smallest normal is 2^-21 of the reference
 
@@ -64,7 +65,7 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sche
         dst += TR_STAGE; bar += 8;
         if (++st == TR_STAGES) { st = 0; ph ^= 1; dst = smb + TR_RING; bar = full0; }
     };
-    for (Segment g; sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
+    for (Segment g; sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);) {
         int next[2 * NB], k[2 * NB], v[2 * NB];           // pool rows of the boxes of tiles j + 1, j and j - 1
         // boxes beyond the drafts read the last 16 rows' page again
         auto rows_of = [&](int j) {
@@ -134,7 +135,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
-    if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE, true>(p, sched, tid, TR_THREADS, pairs);
+    if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE, TR_LEAD, true>(p, sched, tid, TR_THREADS, pairs);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -142,7 +143,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     tc_fence_after();
     const uint32_t tmem = B.tmem;
     pdl_trigger();
-    if (blockIdx.x == 0) for (int i = tid; i < (int)(sizeof(Sched) / 4); i += TR_THREADS) ((int*)wk.sched)[i] = ((const int*)&sched)[i];
+    if (rank == 0 && tid == 128) wk.split[pair].parts = 0;
     int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
     const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
     const uint32_t smb = smem_u32(sm);
@@ -165,7 +166,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             auto advance = [&](uint32_t k) { st = (st + k) % TR_STAGES; };
             auto wait_stage = [&](uint64_t* full) { const bool got = wait(&full[st], (uses >> st) & 1); uses ^= 1u << st; return got; };
             if (warp == 1) {
-                for (Segment g; ok && sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
+                for (Segment g; ok && sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);) {
                     if (!wait(&B.q_full, n_q++ & 1)) break;
                     for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
                         const uint32_t buf = n & 1, d = tmem + TR_S_COL + buf * 64;
@@ -186,7 +187,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     advance(4);                           // V of the last tile
                 }
             } else {
-                for (Segment g; ok && sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
+                for (Segment g; ok && sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);) {
                     advance(5);                           // K of the first tile
                     for (int j = g.t0; ok && j < g.t1; ++j, ++n) {
                         if (j + 1 < g.t1) advance(5);     // K of tile j + 1
@@ -215,7 +216,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         const uint32_t full0 = peer_addr(smem_u32(&B.v_full[0]), 0);
         uint32_t st = 0, uses = 0;                        // bit s: parity of the uses of land[s]
         auto advance = [&](int n) { st = (st + n) % TR_STAGES; };
-        for (Segment g; sched_next<ATT_TILE>(p, sched, u, u_end, g);) {
+        for (Segment g; sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);) {
             for (int j = g.t0; j <= g.t1; ++j) {
                 if (j < g.t1) advance(5);
                 if (j == g.t0) continue;
@@ -280,7 +281,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             if (lane == 0) arrive_at(q_full0);
         };
         Segment g, next;
-        bool more = sched_next<ATT_TILE>(p, sched, u, u_end, g);
+        bool more = sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);
         if (more) { start_q(g); finish_q(); }
         while (more) {
             const int gr = g.rt * ATT_ITEM + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
@@ -354,7 +355,7 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 if (lane == 0) arrive_at(p_full0);
             }
             // ---- output: all of O, then the row's four sums; the next segment's Q and first S under them (this one's S are done)
-            more = sched_next<ATT_TILE>(p, sched, u, u_end, next);
+            more = sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, next);
             if (more) start_q(next);
             wait(&B.o_done, (n - 1) & 1);
             if (more) finish_q();
@@ -396,6 +397,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                             to[(c + i) * 2] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                 }
                 if (live && part == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
+                if (rank == 0 && tid == 128 && g.t0 == 0)        // the first part
+                    wk.split[pair] = TreeSplit{ sched.owner(g.item + TR_LEAD + g.tiles - 1) - pair + 1, slot, min(ATT_ITEM, g.n * p.H - g.rt * ATT_ITEM),
+                                                g.rt * ATT_ITEM, g.first };
             }
             tc_fence_before();
             g = next;
@@ -409,10 +413,11 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 }
 
 // ---------------------------------------------------------------- joining split items
-// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q, added in a fixed order.  A CTA takes
-// 8 rows of an item (a part's 128-byte lines) x 64 latent values; its 4 groups of 128 threads take every fourth part.  Items
-// that one run finished were written by k_tree.
-constexpr int MG_ROWS = 8, MG_C4 = 16, MG_GROUPS = 4, MG_ELEMS = MG_ROWS * MG_C4, MG_THREADS = MG_ELEMS * MG_GROUPS, MG_PARTS = 128;
+// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q, added in a fixed order.  A task is 8
+// rows of an item (a part's 128-byte lines) x 128 latent values, or x 32 for items of 8 parts and more (a decoded token's),
+// where 4 groups of 64 threads then take every fourth part.  The blocks share out the tasks of all split items; a task's first
+// parts are on their way before its factors are known, since its time is that of the loads one after another.
+constexpr int MG_ROWS = 8, MG_THREADS = 256, MG_PARTS = 128, MG_MANY = 8, MG_DEEP = 8;
 
 __device__ __forceinline__ float4 load_cg(const float4* p) {      // volatile: not moved behind a test of its weight
     float4 v;
@@ -421,77 +426,94 @@ __device__ __forceinline__ float4 load_cg(const float4* p) {      // volatile: n
 }
 
 template <class T>
-__global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk) {
-    __shared__ float4 acc[MG_GROUPS][MG_ELEMS];
+__global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk, int pairs) {
+    __shared__ TreeSplit split[MG_PARTS];
+    __shared__ int before[MG_PARTS + 1];                          // tasks of the items before
+    __shared__ float4 acc[MG_THREADS];
     __shared__ float f[MG_PARTS][MG_ROWS];
     __shared__ float ref[MG_ROWS], sum[MG_ROWS];
-    pdl_wait();
-    const Sched& s = *wk.sched;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // sequence b's groups of 8 rows are numbered from start[b] * H / 8 + b on: the last b whose first number is not above ours
-    int b = 0;
-    for (int lo = 1, hi = p.kv.n_seqs - 1; lo <= hi;) {
-        const int mid = (lo + hi) >> 1;
-        if ((int)((int64_t)s.start[mid] * p.H / MG_ROWS) + mid <= (int)blockIdx.x) { b = mid; lo = mid + 1; } else hi = mid - 1;
-    }
-    const int first = s.start[b], rows = (s.start[b + 1] - first) * p.H, row0 = (blockIdx.x - ((int)((int64_t)first * p.H / MG_ROWS) + b)) * MG_ROWS;
-    const int64_t units = s.prefix[b + 1] - s.prefix[b];
-    if (units == 0 || row0 < 0 || row0 >= rows) return;
-    const int64_t tiles = div_small(units, (rows + ATT_ITEM - 1) / ATT_ITEM), u0 = s.prefix[b] + row0 / ATT_ITEM * tiles;
-    const int q0 = s.owner(u0), n = s.owner(u0 + tiles - 1) - q0 + 1, pr0 = row0 % ATT_ITEM, nr = min(MG_ROWS, rows - row0);
-    if (n < 2) return;
-    const int slot0 = 2 * q0 + (u0 > s.run_start(q0));
-    auto slot = [&](int i) { return i ? (slot0 & ~1) + 2 * i : slot0; };
-    if (warp < nr) {                                    // the factors of one row
-        float m = -INFINITY, l = 0.0f;
-        for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]).x);
-        #pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float rf = m == -INFINITY ? 0.0f : m;
-        for (int i = lane; i < n; i += 32) {
-            const float2 ml = __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]);
-            // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
-            const float v = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
-            f[i][warp] = v;
-            l += v == 0.0f ? 0.0f : v * ml.y;
+    pdl_wait();
+    if (tid < pairs) split[tid] = wk.split[tid];
+    __syncthreads();
+    if (warp == 0) {
+        int b0 = 0;
+        for (int i0 = 0; i0 < pairs; i0 += 32) {
+            const int i = i0 + lane, n = i < pairs ? split[i].parts : 0;
+            int v = n ? (split[i].rows + MG_ROWS - 1) / MG_ROWS * (n < MG_MANY ? 4 : 16) : 0;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int w = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += w; }
+            if (i < pairs) before[i + 1] = b0 + v;
+            b0 += __shfl_sync(0xffffffffu, v, 31);
         }
-        #pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) { ref[warp] = rf; sum[warp] = l; }
+        if (lane == 0) before[0] = 0;
     }
-    const int e = tid % MG_ELEMS, grp = tid / MG_ELEMS, r = e % MG_ROWS, c4 = blockIdx.y * MG_C4 + e / MG_ROWS;
-    const float4* src = wk.part + pr0 / 8 * 1024 + c4 * 8 + r;
-    float4 a = make_float4(0, 0, 0, 0);
     __syncthreads();
-    for (int i0 = grp; i0 < n; i0 += 8 * MG_GROUPS) {
-        float4 v[8];
-        #pragma unroll
-        for (int k = 0; k < 8; ++k) if (i0 + k * MG_GROUPS < n) v[k] = load_cg(src + (int64_t)slot(i0 + k * MG_GROUPS) * (128 * 128));
-        #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (i0 + k * MG_GROUPS < n && r < nr) {
-                const float w = f[i0 + k * MG_GROUPS][r];
-                if (w != 0.0f) { a.x += w * v[k].x; a.y += w * v[k].y; a.z += w * v[k].z; a.w += w * v[k].w; }
+    const int tasks = before[pairs];
+    for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+        int lo = 0, hi = pairs - 1;
+        while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (before[mid] <= task) lo = mid; else hi = mid - 1; }
+        const TreeSplit& s = split[lo];
+        const int n = s.parts, chunks = n < MG_MANY ? 4 : 16, G = n < MG_MANY ? 1 : 4, elems = MG_THREADS / G, at = task - before[lo];
+        const int pr0 = at / chunks * MG_ROWS, nr = min(MG_ROWS, s.rows - pr0);
+        const int e = tid % elems, grp = tid / elems, r = e % MG_ROWS, c4 = at % chunks * (128 / chunks) + e / MG_ROWS;
+        const float4* src = wk.part + pr0 / MG_ROWS * 1024 + c4 * 8 + r;
+        auto slot = [&](int i) { return i ? (s.slot0 & ~1) + 2 * i : s.slot0; };
+        float4 v[MG_DEEP];
+        auto fetch = [&](int i0) {
+            #pragma unroll
+            for (int k = 0; k < MG_DEEP; ++k) if (i0 + k * G < n) v[k] = load_cg(src + (int64_t)slot(i0 + k * G) * (128 * 128));
+        };
+        fetch(grp);
+        if (warp < nr) {                                          // the factors of one row
+            float m = -INFINITY, l = 0.0f;
+            for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]).x);
+            #pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float rf = m == -INFINITY ? 0.0f : m;
+            for (int i = lane; i < n; i += 32) {
+                const float2 ml = __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]);
+                // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
+                const float w = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
+                f[i][warp] = w;
+                l += w == 0.0f ? 0.0f : w * ml.y;
             }
+            #pragma unroll
+            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (lane == 0) { ref[warp] = rf; sum[warp] = l; }
+        }
+        __syncthreads();
+        float4 a = make_float4(0, 0, 0, 0);
+        for (int i0 = grp; i0 < n; i0 += MG_DEEP * G) {
+            if (i0 != grp) fetch(i0);
+            #pragma unroll
+            for (int k = 0; k < MG_DEEP; ++k)
+                if (i0 + k * G < n && r < nr) {
+                    const float w = f[i0 + k * G][r];
+                    if (w != 0.0f) { a.x += w * v[k].x; a.y += w * v[k].y; a.z += w * v[k].z; a.w += w * v[k].w; }
+                }
+        }
+        if (G > 1) {
+            acc[tid] = a;
+            __syncthreads();
+            if (grp == 0)
+                for (int q = 1; q < G; ++q) {
+                    const float4 w = acc[q * elems + e];
+                    a.x += w.x; a.y += w.y; a.z += w.z; a.w += w.w;
+                }
+        }
+        if (grp == 0 && r < nr) {
+            const int gr = s.row0 + pr0 + r, tj = gr / p.H, h = gr - tj * p.H, t = s.first + tj;
+            const float l = sum[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
+            *(uint2*)((T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + 4 * c4) =
+                make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+            if (c4 == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[r] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
+        }
+        __syncthreads();
     }
-    acc[grp][e] = a;
-    __syncthreads();
-    if (grp || r >= nr) return;
-    a = make_float4(0, 0, 0, 0);
-    #pragma unroll
-    for (int q = 0; q < MG_GROUPS; ++q) {
-        const float4 v = acc[q][e];
-        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-    }
-    const int tj = (row0 + r) / p.H, h = row0 + r - tj * p.H, t = first + tj;
-    const float l = sum[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *(uint2*)((T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + 4 * c4) =
-        make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-    if (c4 == 0 && p.lse) p.lse[(int64_t)t * p.H + h] = l == 0.0f ? -INFINITY : (ref[r] - TR_SHIFT + log2f(l)) * 0.6931471805599453f;
 }
 
 int tree_pairs(int nsm) { return nsm / 2 < MG_PARTS ? nsm / 2 : MG_PARTS; }
-size_t tree_sched_bytes() { return sizeof(Sched); }
 
 template <class T>
 static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
@@ -499,8 +521,7 @@ static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const Tr
     if (e != cudaSuccess) return e;
     k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const unsigned groups = (unsigned)((int64_t)p.T * p.H / MG_ROWS) + p.kv.n_seqs;
-    return launch_pdl_n(k_merge<T>, dim3(groups, AT_LATENT / 4 / MG_C4), dim3(MG_THREADS), 0, st, p, wk);
+    return launch_pdl_n(k_merge<T>, dim3(16 * pairs), dim3(MG_THREADS), 0, st, p, wk, pairs);      // 8 blocks an SM
 }
 
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
