@@ -15,6 +15,8 @@ __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // the shared::cluster address of the same shared variable in CTA `rank` of the cluster
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     uint32_t r;

@@ -139,15 +139,16 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();
-    tc_fence_after();
-    const uint32_t tmem = B.tmem;
+    cluster_arrive();                                     // the wait comes with each role's first use of the other CTA
     pdl_trigger();
     if (rank == 0 && tid == 128) wk.split[pair].parts = 0;
     int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
     const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
     const uint32_t smb = smem_u32(sm);
 
+    if (warp < 4) cluster_wait();                         // the softmax warps start Q first
+    tc_fence_after();
+    const uint32_t tmem = B.tmem;
     if (warp == 0) {
         // ---------------------------------------------------------------- loads
         if (elect_one()) {
@@ -282,7 +283,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         };
         Segment g, next;
         bool more = sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);
-        if (more) { start_q(g); finish_q(); }
+        if (more) start_q(g);
+        cluster_wait();
+        if (more) finish_q();
         while (more) {
             const int gr = g.rt * ATT_ITEM + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
             const bool live = gr < g.n * p.H;
@@ -414,10 +417,10 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 
 // ---------------------------------------------------------------- joining split items
 // out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q, added in a fixed order.  A task is 8
-// rows of an item (a part's 128-byte lines) x 128 latent values, or x 32 for items of 8 parts and more (a decoded token's),
+// rows of an item (a part's 128-byte lines) x 128 latent values, or x 32 for items of 24 parts and more (a decoded token's),
 // where 4 groups of 64 threads then take every fourth part.  The blocks share out the tasks of all split items; a task's first
 // parts are on their way before its factors are known, since its time is that of the loads one after another.
-constexpr int MG_ROWS = 8, MG_THREADS = 256, MG_PARTS = 128, MG_MANY = 8, MG_DEEP = 8;
+constexpr int MG_ROWS = 8, MG_THREADS = 256, MG_PARTS = 128, MG_MANY = 24, MG_DEEP = 8;
 
 __device__ __forceinline__ float4 load_cg(const float4* p) {      // volatile: not moved behind a test of its weight
     float4 v;
@@ -466,18 +469,27 @@ __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ Tr
         };
         fetch(grp);
         if (warp < nr) {                                          // the factors of one row
+            float2 ml[MG_PARTS / 32];
             float m = -INFINITY, l = 0.0f;
-            for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]).x);
+            #pragma unroll
+            for (int k = 0; k < MG_PARTS / 32; ++k)
+                if (32 * k < n) {
+                    const int i = 32 * k + lane;
+                    ml[k] = i < n ? __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]) : make_float2(-INFINITY, 0.0f);
+                }
+            #pragma unroll
+            for (int k = 0; k < MG_PARTS / 32; ++k) if (32 * k < n) m = fmaxf(m, ml[k].x);
             #pragma unroll
             for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             const float rf = m == -INFINITY ? 0.0f : m;
-            for (int i = lane; i < n; i += 32) {
-                const float2 ml = __ldcg(&wk.ml[slot(i) * 128 + pr0 + warp]);
-                // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
-                const float w = ml.y == 0.0f ? 0.0f : exp2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - rf);
-                f[i][warp] = w;
-                l += w == 0.0f ? 0.0f : w * ml.y;
-            }
+            #pragma unroll
+            for (int k = 0; k < MG_PARTS / 32; ++k)
+                if (32 * k < n) {
+                    // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
+                    const float w = ml[k].y == 0.0f ? 0.0f : exp2_approx((ml[k].x == -INFINITY ? 0.0f : ml[k].x) - rf);
+                    if (32 * k + lane < n) f[32 * k + lane][warp] = w;
+                    l += w == 0.0f ? 0.0f : w * ml[k].y;
+                }
             #pragma unroll
             for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             if (lane == 0) { ref[warp] = rf; sum[warp] = l; }
