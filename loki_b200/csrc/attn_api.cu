@@ -33,8 +33,9 @@ struct OnDevice {
 
 static bool is16(const void* p) { return p && !((uintptr_t)p & 15); }
 
-// the cache's rows as a tensor map: boxes of 64 values x up to 64 rows of one page, 128-byte swizzle
-static int encode_map(LkAttnCtx* c, const LkKvCache* k, CUtensorMap* map) {
+// rows of 64-value columns as a tensor map: dims[0] values of a row, the outer strides in elements, boxes of 64 values x `rows` of
+// the next dimension, 128-byte swizzle, zeros outside
+static int encode_map(LkAttnCtx* c, CUtensorMap* map, int dtype, const void* base, int rank, const int64_t* dims, const int64_t* strides, int rows) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static const Encode encode = [] {
@@ -44,12 +45,19 @@ static int encode_map(LkAttnCtx* c, const LkKvCache* k, CUtensorMap* map) {
         return ok ? (Encode)f : nullptr;
     }();
     if (!encode) return set_err(c, LK_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-    const cuuint64_t dims[2] = { AT_ROW, (cuuint64_t)k->n_pages * k->page_size }, strides[1] = { (cuuint64_t)k->row_stride * 2 };
-    const cuuint32_t box[2] = { 64, (cuuint32_t)(k->page_size < 64 ? k->page_size : 64) }, step[2] = { 1, 1 };
-    const CUresult r = encode(map, k->dtype == LK_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, k->rows, dims, strides,
+    cuuint64_t d[3], s[2];
+    for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i];
+    for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)strides[i] * 2;
+    const cuuint32_t box[3] = { 64, (cuuint32_t)rows, 1 }, step[3] = { 1, 1, 1 };
+    const CUresult r = encode(map, dtype == LK_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s,
                               box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? LK_OK : set_err(c, LK_ERR_CUDA, "cuTensorMapEncodeTiled: %d", (int)r);
+}
+// the cache: boxes of up to 64 rows of one page
+static int kv_map(LkAttnCtx* c, const LkKvCache* k, CUtensorMap* map) {
+    const int64_t dims[2] = { AT_ROW, (int64_t)k->n_pages * k->page_size }, strides[1] = { k->row_stride };
+    return encode_map(c, map, k->dtype, k->rows, 2, dims, strides, k->page_size < 64 ? k->page_size : 64);
 }
 
 // a workspace that is made on the first call that needs it; not inside a stream capture
@@ -205,7 +213,7 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     OnDevice on(c->device);
     p.out = out; p.out_token = out_token; p.out_head = out_head; p.lse = lse;
     CUtensorMap map;
-    if (int rc = encode_map(c, cache, &map)) return rc;
+    if (int rc = kv_map(c, cache, &map)) return rc;
     if (!c->work.part) {                              // parts of at most two items per pair of SMs: 0.5 MB a pair
         if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
         c->pairs = tree_pairs(c->nsm);
@@ -229,9 +237,13 @@ int lk_attn_mass(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     if (!lse) return set_err(c, LK_ERR_ARG, "null lse");
     OnDevice on(c->device);
     p.lse = const_cast<float*>(lse); p.weight = weight; p.decay = decay;
-    CUtensorMap map;
-    if (int rc = encode_map(c, cache, &map)) return rc;
-    LK_CU(launch_mass(p, cache->dtype, map, c->nsm / 2, (cudaStream_t)stream));
+    CUtensorMap map, q_map;
+    if (int rc = kv_map(c, cache, &map)) return rc;
+    // a dimension of one has no stride of its own
+    const int64_t dims[3] = { AT_ROW, H, T }, strides[2] = { H > 1 ? q_head : AT_ROW, T > 1 ? q_token : AT_ROW };
+    if (strides[0] <= 0 || strides[1] <= 0) return set_err(c, LK_ERR_UNSUPPORTED, "q strides must be positive");
+    if (int rc = encode_map(c, &q_map, cache->dtype, q, 3, dims, strides, mass_q_box(H))) return rc;
+    LK_CU(launch_mass(p, cache->dtype, map, q_map, c->nsm / 2, (cudaStream_t)stream));
     return LK_OK;
 }
 

@@ -61,7 +61,8 @@ struct TreeWork {
 };
 int tree_pairs(int nsm);       // pairs of CTAs of a launch
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st);
-cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, int pairs, cudaStream_t st);
+int mass_q_box(int H);         // heads of a box of q's tensor map
+cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st);
 
 struct EvictParams {
     KvView kv;

@@ -13,14 +13,16 @@
 //
 // The key tile stays in shared memory (9 chunks of 64 values, 144 KB); each chunk is replaced as soon as the last row block has
 // read it, so the next tile's loads run under the rest.  Q chunks go through a ring of 4 (16 KB: the CTA's half of the rows x 64
-// values).  Roles (512 threads): warp 0 loads K (TMA), warp 1 of CTA 0 issues the MMAs, warps 4-7 load Q, warps 8-15 add.
+// values), as boxes of `hb` heads of a token: heads are padded to a multiple of 8, which the tensor map fills with zeros, and hb
+// is the largest power of two up to 64 that divides that.  (Q by cp.async took 1150 cycles a chunk, of 512 of MMAs.)
+// Roles (384 threads): warp 0 loads K, warp 1 of CTA 0 issues the MMAs, warp 2 loads Q, warps 4-11 add.
 #include <type_traits>
 #include "attn_tc.cuh"
 #include "attn_sched.cuh"
 
 namespace lk {
 
-constexpr int MS_THREADS = 512, MS_TILE = 256, MS_ROWS = 256, MS_CHUNK = 16384, MS_RING = 4, MS_LAG = 2;
+constexpr int MS_THREADS = 384, MS_TILE = 256, MS_ROWS = 256, MS_CHUNK = 16384, MS_RING = 4;
 constexpr int MS_Q = 9 * MS_CHUNK, MS_BARS = MS_Q + MS_RING * MS_CHUNK, MS_COL = MS_BARS + 48 * 8;
 constexpr int MS_TOK = MS_COL + 2 * MS_ROWS * 4, MS_PART = MS_TOK + 2 * MS_ROWS, MS_ACT = MS_PART + 128 * 4, MS_MASK = MS_ACT + 64 * 4;
 constexpr int MS_SCHED = MS_MASK + 64 * 8;
@@ -34,12 +36,14 @@ struct MassBars {
 };
 static_assert(sizeof(MassBars) <= 48 * 8, "barrier block");
 
-// columns of the MMA for `rows` rows of a block
-__device__ __forceinline__ int mass_cols(int rows) { return (min(rows, MS_ROWS) + 31) & ~31; }
+__host__ __device__ inline int mass_heads(int H) { return (H + 7) & ~7; }            // padded heads
+__host__ __device__ inline int mass_box(int H) { const int p = mass_heads(H), b = p & -p; return b < 64 ? b : 64; }
+// columns of the MMA for `rows` rows of a block: whole boxes in each CTA's half
+__device__ __forceinline__ int mass_cols(int rows, int hb) { const int u = max(32, 2 * hb); return (min(rows, MS_ROWS) + u - 1) / u * u; }
 
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MS_THREADS, 1)
-k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map) {
+k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map) {
     extern __shared__ __align__(1024) uint8_t sm[];
     MassBars& B = *(MassBars*)(sm + MS_BARS);
     float* col = (float*)(sm + MS_COL);                       // [2][256] c of each row of a block
@@ -57,11 +61,12 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     if (warp == 2 && lane == 0) {
         B.gave_up = 0;
         for (int i = 0; i < 9; ++i) { mbar_init(&B.k_full[i], 2); mbar_init(&B.k_empty[i], 1); }
-        for (int i = 0; i < MS_RING; ++i) { mbar_init(&B.q_full[i], 8); mbar_init(&B.q_empty[i], 1); }
+        for (int i = 0; i < MS_RING; ++i) { mbar_init(&B.q_full[i], 2); mbar_init(&B.q_empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&B.d_full[i], 1); mbar_init(&B.d_free[i], 16); }
         mbar_init(&B.drain, 1);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&q_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, 512);
     if (warp == 0 || p.kv.n_seqs > 1) sched_load<MS_TILE, 0, false>(p, sched, tid, MS_THREADS, pairs);
@@ -75,6 +80,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
     uint32_t n_tile = 0, n_q = 0, n_d = 0;                    // this role's key tiles, Q chunks and row blocks so far
     bool ok = true;
+    const int Hp = mass_heads(p.H), hb = mass_box(p.H);
 
     for (Segment g; sched_next<MS_TILE, 0>(p, sched, u, u_end, g);) {
         __syncthreads();                                      // act of the last segment is free
@@ -91,7 +97,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             if (lane == 0) B.n_act = n;
         }
         __syncthreads();
-        const int rows = B.n_act * p.H, blocks = (rows + MS_ROWS - 1) / MS_ROWS;
+        const int rows = B.n_act * Hp, blocks = (rows + MS_ROWS - 1) / MS_ROWS;
 
         if (warp == 0) {
             // ---------------------------------------------------------------- K: 128 keys of this CTA, 9 chunks a tile
@@ -120,7 +126,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 for (int j = g.t0; ok && j < g.t1; ++j, ++n_tile)
                     for (int b = 0; ok && b < blocks; ++b, ++n_d) {
                         const uint32_t buf = n_d & 1, d = tmem + buf * 256;
-                        const uint32_t idesc = att_idesc(256, 0, BF, false) | ((uint32_t)(mass_cols(rows - b * MS_ROWS) >> 3) << 17);
+                        const uint32_t idesc = att_idesc(256, 0, BF, false) | ((uint32_t)(mass_cols(rows - b * MS_ROWS, hb) >> 3) << 17);
                         if (!wait(&B.d_free[buf], ((n_d >> 1) & 1) ^ 1)) break;
                         tc_fence_after();
                         for (int c = 0; c < 9; ++c, ++n_q) {
@@ -136,42 +142,32 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     }
                 if (!ok) { commit2(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
             }
-        } else if (warp >= 4 && warp < 8) {
+        } else if (warp == 2) {
             // ---------------------------------------------------------------- Q: this CTA's half of a block's rows, 64 values a stage
-            // 8 lanes a row and 16 rows a pass of the four warps; a stage is passed on MS_LAG stages later, once its copies are in
-            const uint32_t full0 = peer_addr(smem_u32(&B.q_full[0]), 0);
-            auto pass_on = [&](uint32_t k) { fence_async_smem(); __syncwarp(); if (lane == 0) arrive_at(full0 + 8 * (k % MS_RING)); };
-            uint32_t passed = n_q;
-            for (int j = g.t0; j < g.t1; ++j)
-                for (int b = 0; b < blocks; ++b) {
-                    const int half = mass_cols(rows - b * MS_ROWS) / 2;
-                    int64_t at[8];
-                    #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int r = k * 16 + (warp - 4) * 4 + (lane >> 3), gr = b * MS_ROWS + (int)rank * half + r, a = gr / p.H;
-                        at[k] = r < half && gr < rows ? (g.first + act[a]) * p.q_token + (gr - a * p.H) * p.q_head + (lane & 7) * 8 : -1;
-                    }
-                    for (int c = 0; c < 9; ++c, ++n_q) {
-                        warp_wait_phase(&B.q_empty[n_q % MS_RING], ((n_q / MS_RING) & 1) ^ 1, gave_up, p.err);
-                        const uint32_t to = smb + MS_Q + (n_q % MS_RING) * MS_CHUNK;
-                        #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int r = k * 16 + (warp - 4) * 4 + (lane >> 3);
-                            const T* src = (const T*)p.q + max(at[k], (int64_t)0) + (at[k] < 0 ? 0 : c * 64);
-                            if (k * 16 < half)
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                                             :: "r"(to + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), "l"(src), "r"(at[k] < 0 ? 0 : 16) : "memory");
+            if (blocks && elect_one()) {
+                const uint32_t full0 = peer_addr(smem_u32(&B.q_full[0]), 0);
+                for (int j = g.t0; ok && j < g.t1; ++j)
+                    for (int b = 0; ok && b < blocks; ++b) {
+                        const int half = mass_cols(rows - b * MS_ROWS, hb) / 2, r0 = b * MS_ROWS + (int)rank * half;
+                        const int a0 = r0 / Hp, h0 = r0 - a0 * Hp;
+                        for (int c = 0; c < 9; ++c, ++n_q) {
+                            const uint32_t st = n_q % MS_RING, bar = full0 + 8 * st;
+                            if (!(ok = wait_phase(&B.q_empty[st], ((n_q / MS_RING) & 1) ^ 1, gave_up, p.err))) break;
+                            arrive_expect_at(bar, half * 128);
+                            uint32_t to = smb + MS_Q + st * MS_CHUNK;
+                            for (int r = 0, a = a0, h = h0; r < half; r += hb, to += hb * 128) {
+                                // rows beyond the last token's: that token's again (their c is infinite)
+                                tma_3d_pair(to, &q_map, c * 64, h, g.first + act[min(a, rows / Hp - 1)], bar);
+                                if ((h += hb) == Hp) { h = 0; ++a; }
+                            }
                         }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        if (n_q - passed >= MS_LAG) { asm volatile("cp.async.wait_group %0;" :: "n"(MS_LAG) : "memory"); pass_on(passed++); }
                     }
-                }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            while (passed != n_q) pass_on(passed++);
-        } else if (warp >= 8) {
+                if (!ok) __nanosleep(1000000);
+            }
+        } else if (warp >= 4) {
             // ---------------------------------------------------------------- sums: lane = key; the two groups of four warps take
             // every other 32 columns.  A wait that gives up is not acted on: the loops end.
-            const int t8 = tid - 256, L = t8 & 127, grp = t8 >> 7;
+            const int t8 = tid - 128, L = t8 & 127, grp = t8 >> 7;
             const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
             const uint32_t d_free0 = peer_addr(smem_u32(&B.d_free[0]), 0);
             const float scale2 = p.scale * 1.4426950408889634f;
@@ -182,11 +178,11 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 for (int b = 0; b < blocks; ++b, ++n_d) {
                     const uint32_t buf = n_d & 1;
                     {                                         // c of column t8
-                        const int gr = b * MS_ROWS + t8, a = gr / p.H;
+                        const int gr = b * MS_ROWS + t8, a = gr / Hp, h = gr - a * Hp;
                         float c = INFINITY;                   // no row: 2^-inf
-                        if (gr < rows) {
+                        if (gr < rows && h < p.H) {
                             const int t = g.first + act[a];
-                            const float lse = p.lse[(int64_t)t * p.H + gr - a * p.H];
+                            const float lse = p.lse[(int64_t)t * p.H + h];
                             if (lse != -INFINITY) c = lse * 1.4426950408889634f - (p.weight ? log2f(p.weight[t]) : 0.0f);
                         }
                         col[buf * MS_ROWS + t8] = c;
@@ -195,7 +191,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     group_sync();
                     warp_wait_phase(&B.d_full[buf], (n_d >> 1) & 1, gave_up, p.err);
                     tc_fence_after();
-                    const int cols = mass_cols(rows - b * MS_ROWS);
+                    const int cols = mass_cols(rows - b * MS_ROWS, hb);
                     for (int c0 = grp * 32; c0 < cols; c0 += 64) {
                         uint32_t s[32];
                         tmem_ld32(tmem + lane_base + buf * 256 + c0, s);
@@ -246,15 +242,17 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 }
 
 template <class T>
-static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, int pairs, cudaStream_t st) {
+static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_mass<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MS_SMEM);
     if (e != cudaSuccess) return e;
-    k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map);
+    k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map, q_map);
     return cudaGetLastError();
 }
 
-cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, int pairs, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? mass_go<__half>(p, map, pairs, st) : mass_go<__nv_bfloat16>(p, map, pairs, st);
+int mass_q_box(int H) { return mass_box(H); }
+
+cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? mass_go<__half>(p, map, q_map, pairs, st) : mass_go<__nv_bfloat16>(p, map, q_map, pairs, st);
 }
 
 }  // namespace lk
