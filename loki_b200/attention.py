@@ -128,7 +128,7 @@ class AttnContext:
         _need(layout in _LAYOUT, "layout: interleaved or half")
         T, H, D = x.shape
         if out is None:
-            out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+            out = x.new_empty((T, H, D))
         to, so = _rows(out, "out", dev, D)
         _need(out.shape == x.shape and out.dtype is x.dtype, "out: x's shape and dtype")
         rc = self._lib.lk_attn_rope(self.ctx, _DTYPE[x.dtype], at, st[0], st[1], to, so[0], so[1], T, H, D, rot_offset, table.rot_dim,
@@ -167,9 +167,9 @@ class AttnContext:
         at, st, starts_at, tree_at = self._query(q, cache, starts, tree)
         T, H, _ = q.shape
         if out is None:
-            out = torch.empty((T, H, ATTN_LATENT), dtype=q.dtype, device=q.device)
+            out = q.new_empty((T, H, ATTN_LATENT))
         if lse is None:
-            lse = torch.empty((T, H), dtype=_F32, device=q.device)
+            lse = q.new_empty((T, H), dtype=_F32)
         to, so = _rows(out, "out", self.device, ATTN_LATENT)
         _need(out.dim() == 3 and out.shape[:2] == q.shape[:2] and out.dtype is q.dtype, "out: [T][H][512] of q's dtype")
         rc = self._lib.lk_attn_tree(self.ctx, cache._ref, at, st[0], st[1], T, H, starts_at, tree_at, scale, to, so[0], so[1],
@@ -193,7 +193,7 @@ class AttnContext:
         mass, then row order); kept rows beyond the budget fill the holes before it.  Returns new_lens [n_seqs], which may
         be cache.lens itself."""
         if new_lens is None:
-            new_lens = torch.empty((cache.n_seqs,), dtype=_I32, device=next_pos.device)
+            new_lens = next_pos.new_empty((cache.n_seqs,))
         self._check(self._lib.lk_attn_evict(self.ctx, cache._ref, budget, sinks, recent,
                                             _dense(next_pos, "next_pos", _I32, self.device, cache.n_seqs),
                                             _dense(new_lens, "new_lens", _I32, self.device, cache.n_seqs), _queue(stream, self.device)))

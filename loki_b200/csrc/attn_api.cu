@@ -54,10 +54,10 @@ static int encode_map(LkAttnCtx* c, CUtensorMap* map, int dtype, const void* bas
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? LK_OK : set_err(c, LK_ERR_CUDA, "cuTensorMapEncodeTiled: %d", (int)r);
 }
-// the cache: boxes of up to 64 rows of one page
-static int kv_map(LkAttnCtx* c, const LkKvCache* k, CUtensorMap* map) {
+// the cache: boxes of up to `most` rows of one page
+static int kv_map(LkAttnCtx* c, const LkKvCache* k, CUtensorMap* map, int most = 64) {
     const int64_t dims[2] = { AT_ROW, (int64_t)k->n_pages * k->page_size }, strides[1] = { k->row_stride };
-    return encode_map(c, map, k->dtype, k->rows, 2, dims, strides, k->page_size < 64 ? k->page_size : 64);
+    return encode_map(c, map, k->dtype, k->rows, 2, dims, strides, k->page_size < most ? k->page_size : most);
 }
 
 // a workspace that is made on the first call that needs it; not inside a stream capture
@@ -108,6 +108,9 @@ int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
     if (e == cudaSuccess) e = cudaMalloc((void**)&c->err, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(c->err, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaMalloc((void**)&c->n_moves, (size_t)cfg->max_seqs * sizeof(int));
+    if (e == cudaSuccess) e = tree_setup();
+    if (e == cudaSuccess) e = mass_setup();
+    if (e == cudaSuccess) e = evict_setup();
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     cudaSetDevice(prev);
     if (e != cudaSuccess) { lk_attn_destroy(c); return LK_ERR_CUDA; }
@@ -212,8 +215,9 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     if (int rc = check_rows(c, "out", out, out_token, out_head)) return rc;
     OnDevice on(c->device);
     p.out = out; p.out_token = out_token; p.out_head = out_head; p.lse = lse;
-    CUtensorMap map;
+    CUtensorMap map, map16;
     if (int rc = kv_map(c, cache, &map)) return rc;
+    if (int rc = kv_map(c, cache, &map16, 16)) return rc;
     if (!c->work.part) {                              // parts of at most two items per pair of SMs: 0.5 MB a pair
         if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
         c->pairs = tree_pairs(c->nsm);
@@ -222,7 +226,7 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
         LK_CU(cudaMalloc((void**)&w, part + ml + c->pairs * sizeof(TreeSplit)));
         c->work = TreeWork{ (float4*)w, (float2*)(w + part), (TreeSplit*)(w + part + ml) };
     }
-    LK_CU(launch_tree(p, cache->dtype, map, c->work, c->pairs, (cudaStream_t)stream));
+    LK_CU(launch_tree(p, cache->dtype, map, map16, c->work, c->pairs, (cudaStream_t)stream));
     return LK_OK;
 }
 

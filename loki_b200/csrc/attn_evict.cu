@@ -174,15 +174,16 @@ __global__ void __launch_bounds__(EM_LANES * EM_ROWS) k_evict_move(EvictParams p
     }
 }
 
+cudaError_t evict_setup() { return cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4); }
+
 cudaError_t launch_evict(const EvictParams& p0, int nsm, cudaStream_t st) {
     EvictParams p = p0;
     const int64_t cap = (int64_t)p.kv.table_stride * p.kv.page_size;         // most rows of a sequence
     const int64_t share = (cap + EV_CTAS - 1) / EV_CTAS;
     p.keys = share <= EV_KEYS ? (int)share : EV_KEYS;
-    cudaError_t e = cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4);
-    if (e != cudaSuccess) return e;
     k_evict_select<<<p.kv.n_seqs * EV_CTAS, EV_THREADS, p.keys * 4, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess || p.region == 0) return e;
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || p.region == 0) return e;
     // enough blocks for every SM's 7 at a time, and no more than the most rows that can move
     int64_t per = (7 * nsm + p.kv.n_seqs - 1) / p.kv.n_seqs, most = (p.region + EM_ROWS - 1) / EM_ROWS;
     if (per > most) per = most;

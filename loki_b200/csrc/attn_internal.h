@@ -60,7 +60,12 @@ struct TreeWork {
     TreeSplit* split;          // [pairs] the split item that starts in a run (parts 0: none)
 };
 int tree_pairs(int nsm);       // pairs of CTAs of a launch
-cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st);
+// what a device needs once before the launches below (shared-memory sizes)
+cudaError_t tree_setup();
+cudaError_t mass_setup();
+cudaError_t evict_setup();
+// map, map16: the cache in boxes of up to 64 rows of a page, and of 16
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st);
 int mass_q_box(int H);         // heads of a box of q's tensor map
 cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st);
 

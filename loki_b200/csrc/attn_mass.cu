@@ -243,12 +243,14 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 
 template <class T>
 static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(k_mass<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MS_SMEM);
-    if (e != cudaSuccess) return e;
     k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map, q_map);
     return cudaGetLastError();
 }
 
+cudaError_t mass_setup() {
+    const cudaError_t e = cudaFuncSetAttribute(k_mass<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, MS_SMEM);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(k_mass<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, MS_SMEM);
+}
 int mass_q_box(int H) { return mass_box(H); }
 
 cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st) {

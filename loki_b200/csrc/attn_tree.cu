@@ -26,8 +26,8 @@
 // of O, which can reach a stage while the K before it is still on its way (V is in L2 by then), would take that phase for its own.
 //
 // Rows that must not matter: a tile's rows beyond the drafts, and drafted rows that a token does not see, get P = 0; but
-// 0 * NaN is NaN, so warp 3 zeroes the former in the O operand, and every drafted row there that holds a non-finite
-// value (a token that does see it gets its NaN through S and P).
+// 0 * NaN is NaN, so the former are loaded as zeros from outside the pool (the last 16 rows' rest is zeroed by warp 3), and warp 3
+// zeroes every drafted row of the O operand that holds a non-finite value (a token that does see it gets its NaN through S and P).
 #include <type_traits>
 #include "attn_tc.cuh"
 #include "attn_sched.cuh"
@@ -52,11 +52,14 @@ struct TreeBars {
 };
 static_assert(sizeof(TreeBars) <= 44 * 8, "barrier block");
 
+// whether rows i0 .. i0 + 63 hold drafted ones: warp 3 looks them over before the MMAs do
+__device__ __forceinline__ bool tail_rows(const Segment& g, int i0) { return i0 + 64 > g.len && i0 < g.total; }
+
 // the load role of one CTA, one thread: boxes of BOX rows x 64 values.  Its instructions are the loop's length (a loaded
 // stage feeds 512 cycles of MMAs), so the page lookups are made a tile ahead and nothing is computed per box.
 template <int BOX>
 __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sched, int64_t u, int64_t u_end, const CUtensorMap* map,
-                                          TreeBars& B, uint32_t smb, uint32_t rank) {
+                                          const CUtensorMap* map16, TreeBars& B, uint32_t smb, uint32_t rank) {
     constexpr int NB = 64 / BOX;                          // boxes of 64 rows
     constexpr uint32_t V = sizeof(B.k_full);              // from a stage's k_full to its v_full
     const uint32_t full0 = peer_addr(smem_u32(&B.k_full[0]), 0);
@@ -93,18 +96,25 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sche
                 }
             }
             if (j > g.t0) {
-                const bool tail = j * ATT_TILE > g.len;   // tile j - 1 reaches beyond the context: warp 3 passes it on
                 #pragma unroll
                 for (int s = 0; s < 4; ++s) {             // column group s / 2, row half s % 2
                     if (!wait_phase(&B.empty[st], ph, &B.gave_up, p.err)) return false;
+                    const int i0 = (j - 1) * ATT_TILE + (s & 1) * 64, col = (s >> 1) * 256 + (int)rank * 128;
                     uint32_t to = bar + V;
-                    if (tail) { to = smem_u32(&B.land[st]); mbar_arrive_expect_tx(&B.land[st], TR_STAGE); }
+                    if (tail_rows(g, i0)) { to = smem_u32(&B.land[st]); mbar_arrive_expect_tx(&B.land[st], TR_STAGE); }
                     else arrive_expect_at(to, TR_STAGE);
-                    const int col = (s >> 1) * 256 + (int)rank * 128;
-                    #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    if (i0 + 64 <= g.len) {
                         #pragma unroll
-                        for (int x = 0; x < NB; ++x) tma_2d_pair(dst + c * TR_CHUNK + x * BOX * 128, map, col + c * 64, v[(s & 1) * NB + x], to);
+                        for (int c = 0; c < 2; ++c)
+                            #pragma unroll
+                            for (int x = 0; x < NB; ++x) tma_2d_pair(dst + c * TR_CHUNK + x * BOX * 128, map, col + c * 64, v[(s & 1) * NB + x], to);
+                    } else                                // 16 rows at a time; beyond the drafts from outside the pool: zeros
+                        for (int x = 0; x < 4; ++x) {
+                            int row = p.kv.n_pages << p.kv.page_shift;
+                            #pragma unroll
+                            for (int y = 0; y < NB; ++y) if (x * 16 / BOX == y && i0 + x * 16 < g.total) row = v[(s & 1) * NB + y] + x * 16 % BOX;
+                            for (int c = 0; c < 2; ++c) tma_2d_pair(dst + c * TR_CHUNK + x * 2048, map16, col + c * 64, row, to);
+                        }
                     advance();
                 }
             }
@@ -115,7 +125,7 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sche
 
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TR_THREADS, 1)
-k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, TreeWork wk) {
+k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap kv_map16, TreeWork wk) {
     extern __shared__ __align__(1024) uint8_t sm[];
     TreeBars& B = *(TreeBars*)(sm + TR_BARS);
     float* xch = (float*)(sm + TR_XCH);
@@ -152,9 +162,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     if (warp == 0) {
         // ---------------------------------------------------------------- loads
         if (elect_one()) {
-            const bool ok = p.kv.page_size >= 64 ? tree_load<64>(p, sched, u, u_end, &kv_map, B, smb, rank)
-                          : p.kv.page_size == 32 ? tree_load<32>(p, sched, u, u_end, &kv_map, B, smb, rank)
-                                                 : tree_load<16>(p, sched, u, u_end, &kv_map, B, smb, rank);
+            const bool ok = p.kv.page_size >= 64 ? tree_load<64>(p, sched, u, u_end, &kv_map, &kv_map16, B, smb, rank)
+                          : p.kv.page_size == 32 ? tree_load<32>(p, sched, u, u_end, &kv_map, &kv_map16, B, smb, rank)
+                                                 : tree_load<16>(p, sched, u, u_end, &kv_map, &kv_map16, B, smb, rank);
             if (!ok) __nanosleep(1000000);                // given up: the loads in flight land before the CTA ends
         }
     } else if (warp < 3) {
@@ -221,14 +231,14 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             for (int j = g.t0; j <= g.t1; ++j) {
                 if (j < g.t1) advance(5);
                 if (j == g.t0) continue;
-                if (j * ATT_TILE <= g.len) { advance(4); continue; }
                 for (int s = 0; s < 4; ++s, advance(1)) {
+                    const int i0 = (j - 1) * ATT_TILE + (s & 1) * 64;
+                    if (!tail_rows(g, i0)) continue;
                     warp_wait_phase(&B.land[st], (uses >> st) & 1, gave_up, p.err);
                     uses ^= 1u << st;
                     // rows (s % 2) * 64 .. + 63 of the tile, 2 x 128 bytes each: eight lanes a row.  Each row's part is judged by
                     // itself: all that matters is that nothing non-finite is multiplied by 0
-                    const int i0 = (j - 1) * ATT_TILE + (s & 1) * 64;
-                    for (int r = max(0, g.len - i0) & ~3; r < 64; r += 4) {
+                    for (int r = max(0, g.len - i0) & ~3; r < min(64, (g.total - i0 + 15) & ~15); r += 4) {
                         const int i = i0 + r + (lane >> 3);
                         uint4* v = (uint4*)(sm + TR_RING + st * TR_STAGE + (r + (lane >> 3)) * 128) + (lane & 7);
                         bool bad = i >= g.total;
@@ -527,17 +537,21 @@ __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ Tr
 
 int tree_pairs(int nsm) { return nsm / 2 < MG_PARTS ? nsm / 2 : MG_PARTS; }
 
+cudaError_t tree_setup() {
+    const cudaError_t e = cudaFuncSetAttribute(k_tree<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(k_tree<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+}
+
 template <class T>
-static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(k_tree<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TR_SMEM);
+static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st) {
+    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, map16, wk);
+    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, wk);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
     return launch_pdl_n(k_merge<T>, dim3(16 * pairs), dim3(MG_THREADS), 0, st, p, wk, pairs);      // 8 blocks an SM
 }
 
-cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const TreeWork& wk, int pairs, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, wk, pairs, st) : tree_go<__nv_bfloat16>(p, map, wk, pairs, st);
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, map16, wk, pairs, st) : tree_go<__nv_bfloat16>(p, map, map16, wk, pairs, st);
 }
 
 }  // namespace lk
