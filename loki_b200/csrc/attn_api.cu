@@ -12,6 +12,7 @@ struct LkAttnCtx {
     int* err = nullptr;
     int* n_moves = nullptr; int* moves = nullptr; int64_t moves_cap = 0;      // eviction: [2][n_seqs][region]
     TreeWork work{}; int pairs = 0;                                           // lk_attn_tree: parts of split items
+    MassWork mass{};
     char msg[256] = {0};
 };
 
@@ -108,6 +109,10 @@ int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
     if (e == cudaSuccess) e = cudaMalloc((void**)&c->err, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(c->err, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaMalloc((void**)&c->n_moves, (size_t)cfg->max_seqs * sizeof(int));
+    const size_t sums = (size_t)(c->nsm / 2) * 2 * 256 * sizeof(float), counts = (size_t)(c->nsm / 2) * 2 * sizeof(unsigned);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&c->mass.part, sums + counts);
+    if (e == cudaSuccess) e = cudaMemset(c->mass.part, 0, sums + counts);
+    c->mass.arrived = (unsigned*)((char*)c->mass.part + sums);
     if (e == cudaSuccess) e = tree_setup();
     if (e == cudaSuccess) e = mass_setup();
     if (e == cudaSuccess) e = evict_setup();
@@ -121,7 +126,7 @@ int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
 void lk_attn_destroy(LkAttnCtx* c) {
     if (!c) return;
     OnDevice on(c->device);
-    void* ptrs[] = { c->err, c->n_moves, c->moves, c->work.part };
+    void* ptrs[] = { c->err, c->n_moves, c->moves, c->work.part, c->mass.part };
     for (void* p : ptrs) if (p) cudaFree(p);
     delete c;
 }
@@ -247,7 +252,7 @@ int lk_attn_mass(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     const int64_t dims[3] = { AT_ROW, H, T }, strides[2] = { H > 1 ? q_head : AT_ROW, T > 1 ? q_token : AT_ROW };
     if (strides[0] <= 0 || strides[1] <= 0) return set_err(c, LK_ERR_UNSUPPORTED, "q strides must be positive");
     if (int rc = encode_map(c, &q_map, cache->dtype, q, 3, dims, strides, mass_q_box(H))) return rc;
-    LK_CU(launch_mass(p, cache->dtype, map, q_map, c->nsm / 2, (cudaStream_t)stream));
+    LK_CU(launch_mass(p, cache->dtype, map, q_map, c->mass, c->nsm / 2, (cudaStream_t)stream));
     return LK_OK;
 }
 

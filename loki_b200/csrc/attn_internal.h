@@ -67,7 +67,10 @@ cudaError_t evict_setup();
 // map, map16: the cache in boxes of up to 64 rows of a page, and of 16
 cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st);
 int mass_q_box(int H);         // heads of a box of q's tensor map
-cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st);
+// sums of key tiles that more than one pair of CTAs works on (attn_mass.cu): [2 per pair][256 keys], and for the tile that
+// starts in a run the parts that have arrived, one counter a CTA, 0 between calls
+struct MassWork { float* part; unsigned* arrived; };
+cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, const MassWork& wk, int pairs, cudaStream_t st);
 
 struct EvictParams {
     KvView kv;

@@ -25,14 +25,14 @@ namespace lk {
 constexpr int MS_THREADS = 384, MS_TILE = 256, MS_ROWS = 256, MS_CHUNK = 16384, MS_RING = 4;
 constexpr int MS_Q = 9 * MS_CHUNK, MS_BARS = MS_Q + MS_RING * MS_CHUNK, MS_COL = MS_BARS + 48 * 8;
 constexpr int MS_TOK = MS_COL + 2 * MS_ROWS * 4, MS_PART = MS_TOK + 2 * MS_ROWS, MS_ACT = MS_PART + 128 * 4, MS_MASK = MS_ACT + 64 * 4;
-constexpr int MS_SCHED = MS_MASK + 64 * 8;
+constexpr int MS_HALVES = MS_MASK + 64 * 8, MS_SCHED = MS_HALVES + 2 * LK_ATTN_MAX_SEQS;
 constexpr int MS_SMEM = MS_SCHED + (int)sizeof(Sched);
 static_assert(MS_SMEM <= 232448 && MS_SCHED % 8 == 0, "227 KB a CTA");
 
 struct MassBars {
     uint64_t k_full[9], k_empty[9], q_full[MS_RING], q_empty[MS_RING], d_full[2], d_free[2], drain;
     uint32_t tmem;
-    int gave_up, n_act;
+    int gave_up, n_act, last;
 };
 static_assert(sizeof(MassBars) <= 48 * 8, "barrier block");
 
@@ -41,9 +41,50 @@ __host__ __device__ inline int mass_box(int H) { const int p = mass_heads(H), b 
 // columns of the MMA for `rows` rows of a block: whole boxes in each CTA's half
 __device__ __forceinline__ int mass_cols(int rows, int hb) { const int u = max(32, 2 * hb); return (min(rows, MS_ROWS) + u - 1) / u * u; }
 
+// Units: half a block of rows (128 columns of the MMA) over one key tile, 2304 cycles of products.  A tile has as many as its
+// rows need, but at least MS_MIN, the time its 288 KB take from HBM when all pairs load; the work is the last ones, so a
+// tile of one half block is never split.  A tile that several runs share is read by each; they leave their sums in `part`
+// (run q: slot 2 q for its first tile, 2 q + 1 for its last) and the last to arrive adds them, in the runs' order.
+constexpr int MS_HALF = 128, MS_MIN = 3;
+
+struct MassSegment {
+    int b, first, n, len, total;              // sequence, its first drafted token, drafted tokens, context, all rows
+    int j, off, per, work;                    // next tile, the next unit of its `per`, of which the last `work` are rows
+    int64_t unit, left;                       // unit 0 of that tile, units that remain
+    // the next piece of work: half blocks [h0, h1) of a tile
+    __device__ __forceinline__ bool next(int& tile, int& h0, int& h1) {
+        while (left > 0) {
+            const int end = (int)min((int64_t)per, off + left), skip = per - work;
+            tile = j; h0 = max(off, skip) - skip; h1 = end - skip;
+            left -= end - off; unit += per; ++j; off = 0;
+            if (h1 > h0) return true;
+        }
+        return false;
+    }
+};
+
+__device__ __forceinline__ bool mass_next(const TreeParams& p, const Sched& s, const uint16_t* halves, int64_t& u, int64_t u_end, MassSegment& g) {
+    if (u >= u_end) return false;
+    g.b = s.sequence(u, p.kv.n_seqs);
+    g.len = s.len[g.b];
+    g.first = s.start[g.b];
+    g.n = s.start[g.b + 1] - g.first;
+    g.total = g.len + g.n;
+    g.work = max((int)halves[g.b], 1);
+    g.per = max(g.work, MS_MIN);
+    const int64_t rem = u - s.prefix[g.b];
+    g.j = (int)div_small(rem, g.per);
+    g.off = (int)(rem - (int64_t)g.j * g.per);
+    g.unit = u - g.off;
+    g.left = min(u_end, s.prefix[g.b + 1]) - u;
+    u += g.left;
+    return true;
+}
+
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MS_THREADS, 1)
-k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map) {
+k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
+       const MassWork wk) {
     extern __shared__ __align__(1024) uint8_t sm[];
     MassBars& B = *(MassBars*)(sm + MS_BARS);
     float* col = (float*)(sm + MS_COL);                       // [2][256] c of each row of a block
@@ -51,6 +92,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     float* part = (float*)(sm + MS_PART);                     // [128]
     int* act = (int*)(sm + MS_ACT);                           // the segment's tokens of positive weight (within the sequence)
     uint64_t* see = (uint64_t*)(sm + MS_MASK);                // the drafted rows that each of them sees
+    uint16_t* halves = (uint16_t*)(sm + MS_HALVES);           // half blocks of rows of each sequence
     Sched& sched = *(Sched*)(sm + MS_SCHED);
     volatile int* gave_up = &B.gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -69,7 +111,30 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         asm volatile("prefetch.tensormap [%0];" :: "l"(&q_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, 512);
-    if (warp == 0 || p.kv.n_seqs > 1) sched_load<MS_TILE, 0, false>(p, sched, tid, MS_THREADS, pairs);
+    if (warp == 0 || p.kv.n_seqs > 1)
+        sched_load<MS_TILE>(p, sched, tid, MS_THREADS, pairs, [](int, int tiles) { return (int64_t)tiles; }, [&]() {
+            const int warps = p.kv.n_seqs > 1 ? MS_THREADS / 32 : 1;
+            for (int b0 = warp; b0 < p.kv.n_seqs; b0 += 4 * warps) {          // four sequences' weights in flight
+                int got[4];
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int b = b0 + i * warps, t0 = b < p.kv.n_seqs ? sched.start[b] : 0;
+                    const int n = b < p.kv.n_seqs && sched.prefix[b + 1] ? sched.start[b + 1] - t0 : 0;
+                    got[i] = 0;
+                    if (lane < n) got[i] = !p.weight || p.weight[t0 + lane] > 0.0f;
+                    if (lane + 32 < n) got[i] += !p.weight || p.weight[t0 + lane + 32] > 0.0f;
+                }
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int b = b0 + i * warps, act_b = __reduce_add_sync(0xffffffffu, got[i]);
+                    if (lane == 0 && b < p.kv.n_seqs) {
+                        halves[b] = (uint16_t)((act_b * mass_heads(p.H) + MS_HALF - 1) / MS_HALF);
+                        sched.prefix[b + 1] *= max((int)halves[b], MS_MIN);
+                    }
+                }
+            }
+            if (p.kv.n_seqs > 1) __syncthreads(); else __syncwarp();
+        });
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -82,7 +147,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     bool ok = true;
     const int Hp = mass_heads(p.H), hb = mass_box(p.H);
 
-    for (Segment g; sched_next<MS_TILE, 0>(p, sched, u, u_end, g);) {
+    for (MassSegment g; mass_next(p, sched, halves, u, u_end, g);) {
         __syncthreads();                                      // act of the last segment is free
         if (warp == 2) {
             int n = 0;
@@ -97,14 +162,15 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             if (lane == 0) B.n_act = n;
         }
         __syncthreads();
-        const int rows = B.n_act * Hp, blocks = (rows + MS_ROWS - 1) / MS_ROWS;
+        const int rows = B.n_act * Hp;
+        int j, h0, h1;
 
         if (warp == 0) {
             // ---------------------------------------------------------------- K: 128 keys of this CTA, 9 chunks a tile
-            if (blocks && elect_one()) {
+            if (rows && elect_one()) {
                 const uint32_t full0 = peer_addr(smem_u32(&B.k_full[0]), 0);
                 const int box = min(p.kv.page_size, 64);
-                for (int j = g.t0; ok && j < g.t1; ++j, ++n_tile) {
+                for (; ok && g.next(j, h0, h1); ++n_tile) {
                     int row[8];                               // pool rows of the boxes; those beyond the drafts read the last page again
                     #pragma unroll
                     for (int x = 0; x < 8; ++x)
@@ -121,47 +187,52 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             }
         } else if (warp == 1) {
             // ---------------------------------------------------------------- MMAs, issued by CTA 0 for both
-            if (rank == 0 && elect_one()) {
+            if (rows && rank == 0 && elect_one()) {
                 auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = wait_phase(bar, parity, gave_up, p.err); };
-                for (int j = g.t0; ok && j < g.t1; ++j, ++n_tile)
-                    for (int b = 0; ok && b < blocks; ++b, ++n_d) {
+                for (; ok && g.next(j, h0, h1); ++n_tile) {
+                    const int end = min(h1 * MS_HALF, rows);
+                    for (int r = h0 * MS_HALF; ok && r < end; r += MS_ROWS, ++n_d) {
+                        const bool first = r == h0 * MS_HALF, last = r + MS_ROWS >= end;
                         const uint32_t buf = n_d & 1, d = tmem + buf * 256;
-                        const uint32_t idesc = att_idesc(256, 0, BF, false) | ((uint32_t)(mass_cols(rows - b * MS_ROWS, hb) >> 3) << 17);
+                        const uint32_t idesc = att_idesc(256, 0, BF, false) | ((uint32_t)(mass_cols(end - r, hb) >> 3) << 17);
                         if (!wait(&B.d_free[buf], ((n_d >> 1) & 1) ^ 1)) break;
                         tc_fence_after();
                         for (int c = 0; c < 9; ++c, ++n_q) {
                             const uint32_t st = n_q % MS_RING;
-                            if (b == 0 && !wait(&B.k_full[c], n_tile & 1)) break;
+                            if (first && !wait(&B.k_full[c], n_tile & 1)) break;
                             if (!wait(&B.q_full[st], (n_q / MS_RING) & 1)) break;
                             umma2_x4_n(d, sw128_lo(smb + c * MS_CHUNK, 16), sw128_lo(smb + MS_Q + st * MS_CHUNK, 16), idesc, c != 0);
                             commit2(&B.q_empty[st]);
-                            if (b == blocks - 1) commit2(&B.k_empty[c]);
+                            if (last) commit2(&B.k_empty[c]);
                         }
                         if (!ok) break;
                         commit2(&B.d_full[buf]);
                     }
+                }
                 if (!ok) { commit2(&B.drain); mbar_wait(&B.drain, 0, nullptr, 0); }
             }
         } else if (warp == 2) {
             // ---------------------------------------------------------------- Q: this CTA's half of a block's rows, 64 values a stage
-            if (blocks && elect_one()) {
+            if (rows && elect_one()) {
                 const uint32_t full0 = peer_addr(smem_u32(&B.q_full[0]), 0);
-                for (int j = g.t0; ok && j < g.t1; ++j)
-                    for (int b = 0; ok && b < blocks; ++b) {
-                        const int half = mass_cols(rows - b * MS_ROWS, hb) / 2, r0 = b * MS_ROWS + (int)rank * half;
-                        const int a0 = r0 / Hp, h0 = r0 - a0 * Hp;
+                while (ok && g.next(j, h0, h1)) {
+                    const int end = min(h1 * MS_HALF, rows);
+                    for (int r1 = h0 * MS_HALF; ok && r1 < end; r1 += MS_ROWS) {
+                        const int half = mass_cols(end - r1, hb) / 2, r0 = r1 + (int)rank * half;
+                        const int a0 = r0 / Hp, hd0 = r0 - a0 * Hp;
                         for (int c = 0; c < 9; ++c, ++n_q) {
                             const uint32_t st = n_q % MS_RING, bar = full0 + 8 * st;
                             if (!(ok = wait_phase(&B.q_empty[st], ((n_q / MS_RING) & 1) ^ 1, gave_up, p.err))) break;
                             arrive_expect_at(bar, half * 128);
                             uint32_t to = smb + MS_Q + st * MS_CHUNK;
-                            for (int r = 0, a = a0, h = h0; r < half; r += hb, to += hb * 128) {
+                            for (int r = 0, a = a0, h = hd0; r < half; r += hb, to += hb * 128) {
                                 // rows beyond the last token's: that token's again (their c is infinite)
                                 tma_3d_pair(to, &q_map, c * 64, h, g.first + act[min(a, rows / Hp - 1)], bar);
                                 if ((h += hb) == Hp) { h = 0; ++a; }
                             }
                         }
                     }
+                }
                 if (!ok) __nanosleep(1000000);
             }
         } else if (warp >= 4) {
@@ -171,14 +242,18 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
             const uint32_t d_free0 = peer_addr(smem_u32(&B.d_free[0]), 0);
             const float scale2 = p.scale * 1.4426950408889634f;
-            for (int j = g.t0; j < g.t1; ++j) {
+            while (g.next(j, h0, h1)) {
+                const int end = min(h1 * MS_HALF, rows);
                 const int key = j * MS_TILE + (int)rank * 128 + L, node = key - g.len;
                 const bool tail = j * MS_TILE + (int)rank * 128 + 127 >= g.len;
+                uint64_t seen = node < 0 ? ~0ull : 0;         // the tokens that see this key (read where `tail`)
+                if (node >= 0 && node < 64)
+                    for (int a = 0; a < B.n_act; ++a) seen |= ((see[a] >> node) & 1) << a;
                 float acc[4] = { 0, 0, 0, 0 };
-                for (int b = 0; b < blocks; ++b, ++n_d) {
+                for (int r = h0 * MS_HALF; r < end; r += MS_ROWS, ++n_d) {
                     const uint32_t buf = n_d & 1;
                     {                                         // c of column t8
-                        const int gr = b * MS_ROWS + t8, a = gr / Hp, h = gr - a * Hp;
+                        const int gr = r + t8, a = gr / Hp, h = gr - a * Hp;
                         float c = INFINITY;                   // no row: 2^-inf
                         if (gr < rows && h < p.H) {
                             const int t = g.first + act[a];
@@ -191,30 +266,28 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     group_sync();
                     warp_wait_phase(&B.d_full[buf], (n_d >> 1) & 1, gave_up, p.err);
                     tc_fence_after();
-                    const int cols = mass_cols(rows - b * MS_ROWS, hb);
+                    const int cols = mass_cols(end - r, hb);
                     for (int c0 = grp * 32; c0 < cols; c0 += 64) {
                         uint32_t s[32];
                         tmem_ld32(tmem + lane_base + buf * 256 + c0, s);
                         tmem_wait_ld();
                         const float4* c4 = (const float4*)(col + buf * MS_ROWS + c0);
-                        if (!tail) {
-                            #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float4 c = c4[i];
-                                acc[0] += exp2_approx(fmaf(__uint_as_float(s[4 * i]), scale2, -c.x));
-                                acc[1] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 1]), scale2, -c.y));
-                                acc[2] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 2]), scale2, -c.z));
-                                acc[3] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 3]), scale2, -c.w));
-                            }
-                        } else {
+                        if (tail) {                               // eight columns are heads of one token
                             const uint8_t* tk = tok + buf * MS_ROWS + c0;
-                            const int left = rows - b * MS_ROWS - c0;
                             #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const bool sees = i < left && (node < 0 || (node < 64 && ((see[tk[i]] >> node) & 1)));
-                                const float e = exp2_approx(fmaf(__uint_as_float(s[i]), scale2, -((const float*)c4)[i]));
-                                acc[i & 3] += sees ? e : 0.0f;
+                            for (int i = 0; i < 32; i += 8) {
+                                const bool sees = (seen >> tk[i]) & 1;
+                                #pragma unroll
+                                for (int x = i; x < i + 8; ++x) s[x] = sees ? s[x] : 0xff800000u;
                             }
+                        }
+                        #pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 c = c4[i];
+                            acc[0] += exp2_approx(fmaf(__uint_as_float(s[4 * i]), scale2, -c.x));
+                            acc[1] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 1]), scale2, -c.y));
+                            acc[2] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 2]), scale2, -c.z));
+                            acc[3] += exp2_approx(fmaf(__uint_as_float(s[4 * i + 3]), scale2, -c.w));
                         }
                     }
                     tc_fence_before();
@@ -224,8 +297,23 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                 float a = (acc[0] + acc[1]) + (acc[2] + acc[3]);
                 if (grp) part[L] = a;
                 group_sync();
-                if (!grp && key < g.total) {
-                    a += part[L];
+                a += part[L];
+                if (h1 - h0 < g.work) {                       // others have rows of this tile too
+                    const int64_t lo = g.unit - g.work, hi = g.unit - 1;      // its first and last unit of work
+                    const int q0 = sched.owner(lo), q1 = sched.owner(hi);
+                    float* mine = wk.part + (int)rank * 128 + L;
+                    if (!grp) __stcg(mine + (int64_t)(pair == q0 ? 2 * pair + 1 : 2 * pair) * MS_TILE, a);
+                    __threadfence();
+                    group_sync();
+                    if (t8 == 0) B.last = atomicInc(wk.arrived + 2 * q0 + rank, q1 - q0) == (unsigned)(q1 - q0);
+                    group_sync();
+                    if (B.last && !grp) {
+                        __threadfence();
+                        a = 0;
+                        for (int q = q0; q <= q1; ++q) a += __ldcg(mine + (int64_t)(q == q0 ? 2 * q + 1 : 2 * q) * MS_TILE);
+                    }
+                }
+                if (!grp && key < g.total && (h1 - h0 == g.work || B.last)) {
                     const int slot = kv_slot(p.kv, g.b, key, p.err);
                     if (slot >= 0) p.kv.mass[slot] = p.decay * p.kv.mass[slot] + a;
                 }
@@ -242,8 +330,8 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 }
 
 template <class T>
-static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st) {
-    k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map, q_map);
+static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& q_map, const MassWork& wk, int pairs, cudaStream_t st) {
+    k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map, q_map, wk);
     return cudaGetLastError();
 }
 
@@ -253,8 +341,8 @@ cudaError_t mass_setup() {
 }
 int mass_q_box(int H) { return mass_box(H); }
 
-cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, int pairs, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? mass_go<__half>(p, map, q_map, pairs, st) : mass_go<__nv_bfloat16>(p, map, q_map, pairs, st);
+cudaError_t launch_mass(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& q_map, const MassWork& wk, int pairs, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? mass_go<__half>(p, map, q_map, wk, pairs, st) : mass_go<__nv_bfloat16>(p, map, q_map, wk, pairs, st);
 }
 
 }  // namespace lk

@@ -1,8 +1,8 @@
 // attn_sched.cuh -- equal cuts of a ragged batch's work, made on the device from the lengths.
 //
-// Sequence b has ceil(n_b * H / 128) items of ceil((len_b + n_b) / TILE) tiles; (item, tile) units are numbered sequence by
-// sequence, item by item, each item's tiles after `lead` units that stand for what a further item costs a pair (Q, the output,
-// an empty pipeline).  They are cut into `runs` of `base` or base + 1 units, the longer ones first.
+// Every sequence has units of about equal cost, numbered sequence by sequence and cut into `runs` of `base` or base + 1 units,
+// the longer ones first.  Attention: sequence b has ceil(n_b * H / 128) items of ceil((len_b + n_b) / TILE) tiles, each item's
+// after LEAD units that stand for what a further item costs a pair (Q, the output, an empty pipeline).
 #pragma once
 #include "attn_internal.h"
 
@@ -20,6 +20,15 @@ struct Sched {
     // the run that has unit u.  A run leaves a part of its first item in slot 2 q and of its last in 2 q + 1, so an item that
     // starts inside run q has its first part in 2 q + 1 and the others in even slots
     __device__ __forceinline__ int owner(int64_t u) const;
+    // the sequence that has unit u: the last that starts at or before it
+    __device__ __forceinline__ int sequence(int64_t u, int n_seqs) const {
+        int lo = 0, hi = n_seqs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+        }
+        return lo;
+    }
 };
 
 // 64-bit values that nearly always fit 32 bits, where a division takes a fifth of the instructions
@@ -38,11 +47,12 @@ struct Segment {
     __device__ __forceinline__ bool whole() const { return t1 - t0 == tiles; }
 };
 
-// ITEMS: a sequence's units are its items x (LEAD + tiles); otherwise LEAD + its tiles.
+// units(n, tiles): the units of a sequence with n drafted tokens; then(): the whole block again, after the sequences' fields are
+// there and before the units are summed (it may change s.prefix[b + 1], still the sequence's own units).
 // the whole block calls it (one sequence: its first warp is enough), for at most `pairs` runs and no more than the longest
-// run's length needs; the caller synchronises before sched_next
-template <int TILE, int LEAD, bool ITEMS>
-__device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int tid, int threads, int pairs) {
+// run's length needs; the caller synchronises before it reads the runs
+template <int TILE, class Units, class Then>
+__device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int tid, int threads, int pairs, Units units_of, Then then) {
     for (int b = tid; b < p.kv.n_seqs; b += threads) {
         const int len0 = p.kv.lens[b], t0 = p.starts[b], t1 = p.starts[b + 1], cap = p.kv.table_stride << p.kv.page_shift;
         const int len = min(max(len0, 0), cap), n = t1 - t0;
@@ -50,14 +60,15 @@ __device__ __forceinline__ void sched_load(const TreeParams& p, Sched& s, int ti
         if (len != len0) att_error(p.err, ATT_ERR_LEN);
         if (t0 < 0 || n < 0 || t1 > p.T || n > LK_ATTN_MAX_NODES) att_error(p.err, ATT_ERR_TREE);
         else if (n > cap - len) att_error(p.err, ATT_ERR_LEN);
-        else if (n) units = (int64_t)(ITEMS ? (n * p.H + ATT_ITEM - 1) / ATT_ITEM : 1) * (LEAD + (len + n + TILE - 1) / TILE);
+        else if (n) units = units_of(n, (len + n + TILE - 1) / TILE);
         s.len[b] = len;
         s.start[b] = t0;
         if (b == p.kv.n_seqs - 1) s.start[b + 1] = t1;
         s.prefix[b + 1] = units;
     }
     if (tid == 0) s.prefix[0] = 0;
-    if (p.kv.n_seqs > 1) __syncthreads();
+    if (p.kv.n_seqs > 1) __syncthreads(); else __syncwarp();
+    then();
     if (tid < 32) {
         __syncwarp();
         int64_t before = 0;
@@ -85,11 +96,7 @@ template <int TILE, int LEAD>
 __device__ __forceinline__ bool sched_next(const TreeParams& p, const Sched& s, int64_t& u, int64_t u_end, Segment& g) {
     for (;;) {
         if (u >= u_end) return false;
-        int lo = 0, hi = p.kv.n_seqs - 1;                // the last sequence that starts at or before u: it has units
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s.prefix[mid] <= u) lo = mid; else hi = mid - 1;
-        }
+        const int lo = s.sequence(u, p.kv.n_seqs);
         g.b = lo;
         g.len = s.len[lo];
         g.first = s.start[lo];

@@ -145,7 +145,8 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
     }
     if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
-    if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE, TR_LEAD, true>(p, sched, tid, TR_THREADS, pairs);
+    if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE>(p, sched, tid, TR_THREADS, pairs,
+        [&](int n, int tiles) { return (int64_t)((n * p.H + ATT_ITEM - 1) / ATT_ITEM) * (TR_LEAD + tiles); }, []() {});
     __syncwarp();
     tc_fence_before();
     __syncthreads();
