@@ -110,6 +110,8 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" :: "l"(&q_map) : "memory");
     }
+    __syncwarp();
+    cluster_arrive();                                         // the barriers are there; the wait is below, after the schedule
     if (warp == 3) tmem_alloc2(&B.tmem, 512);
     if (warp == 0 || p.kv.n_seqs > 1)
         sched_load<MS_TILE>(p, sched, tid, MS_THREADS, pairs, [](int, int tiles) { return (int64_t)tiles; }, [&]() {
@@ -138,7 +140,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();
+    cluster_wait();
     tc_fence_after();
     const uint32_t tmem = B.tmem, smb = smem_u32(sm);
     int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
@@ -148,7 +150,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     const int Hp = mass_heads(p.H), hb = mass_box(p.H);
 
     for (MassSegment g; mass_next(p, sched, halves, u, u_end, g);) {
-        __syncthreads();                                      // act of the last segment is free
+        if (warp != 0) asm volatile("bar.sync 2, %0;" :: "n"(MS_THREADS - 32) : "memory");      // act of the last segment is free
         if (warp == 2) {
             int n = 0;
             for (int j0 = 0; j0 < g.n; j0 += 32) {
@@ -161,13 +163,13 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             }
             if (lane == 0) B.n_act = n;
         }
-        __syncthreads();
-        const int rows = B.n_act * Hp;
+        if (warp != 0) asm volatile("bar.sync 2, %0;" :: "n"(MS_THREADS - 32) : "memory");
+        const int rows = B.n_act * Hp;                        // not for warp 0, which loads K meanwhile
         int j, h0, h1;
 
         if (warp == 0) {
             // ---------------------------------------------------------------- K: 128 keys of this CTA, 9 chunks a tile
-            if (rows && elect_one()) {
+            if (halves[g.b] && elect_one()) {
                 const uint32_t full0 = peer_addr(smem_u32(&B.k_full[0]), 0);
                 const int box = min(p.kv.page_size, 64);
                 for (; ok && g.next(j, h0, h1); ++n_tile) {
@@ -303,12 +305,15 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                     const int q0 = sched.owner(lo), q1 = sched.owner(hi);
                     float* mine = wk.part + (int)rank * 128 + L;
                     if (!grp) __stcg(mine + (int64_t)(pair == q0 ? 2 * pair + 1 : 2 * pair) * MS_TILE, a);
-                    __threadfence();
                     group_sync();
-                    if (t8 == 0) B.last = atomicInc(wk.arrived + 2 * q0 + rank, q1 - q0) == (unsigned)(q1 - q0);
+                    if (t8 == 0) {                            // back to 0 with the last
+                        uint32_t before;
+                        asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                                     : "=r"(before) : "l"(wk.arrived + 2 * q0 + rank), "r"(q1 - q0) : "memory");
+                        B.last = before == (uint32_t)(q1 - q0);
+                    }
                     group_sync();
                     if (B.last && !grp) {
-                        __threadfence();
                         a = 0;
                         for (int q = q0; q <= q1; ++q) a += __ldcg(mine + (int64_t)(q == q0 ? 2 * q + 1 : 2 * q) * MS_TILE);
                     }
