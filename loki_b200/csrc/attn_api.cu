@@ -220,18 +220,24 @@ int lk_attn_tree(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     if (int rc = check_rows(c, "out", out, out_token, out_head)) return rc;
     OnDevice on(c->device);
     p.out = out; p.out_token = out_token; p.out_head = out_head; p.lse = lse;
-    CUtensorMap map, map16;
+    CUtensorMap map, map16, q_map{};
     if (int rc = kv_map(c, cache, &map)) return rc;
     if (int rc = kv_map(c, cache, &map16, 16)) return rc;
+    const int64_t step = H > 1 ? q_head : q_token;       // from one (token, head) row to the next
+    p.q_flat = (H == 1 || T == 1 || q_token == H * q_head) && step >= AT_ROW;
+    if (p.q_flat) {
+        const int64_t dims[2] = { AT_ROW, (int64_t)T * H };
+        if (int rc = encode_map(c, &q_map, cache->dtype, q, 2, dims, &step, 64)) return rc;
+    }
     if (!c->work.part) {                              // parts of at most two items per pair of SMs: 0.5 MB a pair
         if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
         c->pairs = tree_pairs(c->nsm);
         const size_t part = (size_t)c->pairs * 2 * 128 * AT_LATENT * 4, ml = (size_t)c->pairs * 2 * 128 * 8;
         char* w = nullptr;
-        LK_CU(cudaMalloc((void**)&w, part + ml + c->pairs * sizeof(TreeSplit)));
+        LK_CU(cudaMalloc((void**)&w, part + ml + 2 * c->pairs * sizeof(TreeSplit)));
         c->work = TreeWork{ (float4*)w, (float2*)(w + part), (TreeSplit*)(w + part + ml) };
     }
-    LK_CU(launch_tree(p, cache->dtype, map, map16, c->work, c->pairs, (cudaStream_t)stream));
+    LK_CU(launch_tree(p, cache->dtype, map, map16, q_map, c->work, c->pairs, (cudaStream_t)stream));
     return LK_OK;
 }
 

@@ -50,22 +50,23 @@ struct TreeParams {
     void* out; int64_t out_token, out_head;
     float* lse;                                    // tree: out; mass: in
     const float* weight; float decay;              // mass
+    int q_flat;                                    // tree: q's rows (t, h) lie at equal distances
     int* err;
 };
 // parts of items that more than one pair of CTAs works on (attn_tree.cu)
-struct TreeSplit { int parts, slot0, rows, row0, first, pad[3]; };      // runs, the first part's slot, rows, first row, first token
+struct alignas(16) TreeSplit { int info, slot0, row0, first; };      // parts + 256 x this one's place among them + 65536 x rows; slot of the first part; first row, first token
 struct TreeWork {
     float4* part;              // [2 per pair][16 groups of 8 rows][512 / 4][8 rows]: O, not yet divided by the sum
     float2* ml;                // [2 per pair][128 rows]: reference and sum
-    TreeSplit* split;          // [pairs] the split item that starts in a run (parts 0: none)
+    TreeSplit* split;          // [2 per pair] the item that a part belongs to (info 0: no part)
 };
 int tree_pairs(int nsm);       // pairs of CTAs of a launch
 // what a device needs once before the launches below (shared-memory sizes)
 cudaError_t tree_setup();
 cudaError_t mass_setup();
 cudaError_t evict_setup();
-// map, map16: the cache in boxes of up to 64 rows of a page, and of 16
-cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st);
+// map, map16: the cache in boxes of up to 64 rows of a page, and of 16; q_map: q's T * H rows in boxes of 64, where p.q_flat
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const CUtensorMap& q_map, const TreeWork& wk, int pairs, cudaStream_t st);
 int mass_q_box(int H);         // heads of a box of q's tensor map
 // sums of key tiles that more than one pair of CTAs works on (attn_mass.cu): [2 per pair][256 keys], and for the tile that
 // starts in a run the parts that have arrived, one counter a CTA, 0 between calls

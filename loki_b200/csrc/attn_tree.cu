@@ -125,7 +125,8 @@ __device__ __forceinline__ bool tree_load(const TreeParams& p, const Sched& sche
 
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TR_THREADS, 1)
-k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap kv_map16, TreeWork wk) {
+k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap kv_map16,
+       const __grid_constant__ CUtensorMap q_map, TreeWork wk) {
     extern __shared__ __align__(1024) uint8_t sm[];
     TreeBars& B = *(TreeBars*)(sm + TR_BARS);
     float* xch = (float*)(sm + TR_XCH);
@@ -140,24 +141,25 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         B.gave_up = 0;
         for (int s = 0; s < TR_STAGES; ++s) { mbar_init(&B.k_full[s], 2); mbar_init(&B.v_full[s], 2); mbar_init(&B.land[s], 1); mbar_init(&B.empty[s], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&B.s_full[i], 1); mbar_init(&B.s_free[i], 16); mbar_init(&B.drain[i], 1); }
-        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, 16);
+        mbar_init(&B.p_full, 16); mbar_init(&B.o_done, 1); mbar_init(&B.q_full, p.q_flat ? 2 : 16);
         fence_mbar_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kv_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&q_map) : "memory");
     }
+    cluster_arrive();                                     // the barriers are there; the wait comes with a role's first use of the other CTA
     if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
     if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE>(p, sched, tid, TR_THREADS, pairs,
         [&](int n, int tiles) { return (int64_t)((n * p.H + ATT_ITEM - 1) / ATT_ITEM) * (TR_LEAD + tiles); }, []() {});
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_arrive();                                     // the wait comes with each role's first use of the other CTA
     pdl_trigger();
-    if (rank == 0 && tid == 128) wk.split[pair].parts = 0;
+    if (rank == 0 && tid == 128) wk.split[2 * pair].info = wk.split[2 * pair + 1].info = 0;
     int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
     const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
     const uint32_t smb = smem_u32(sm);
 
-    if (warp < 4) cluster_wait();                         // the softmax warps start Q first
+    if (warp < 4) cluster_wait();                         // the softmax warps may start Q first
     tc_fence_after();
     const uint32_t tmem = B.tmem;
     if (warp == 0) {
@@ -269,8 +271,17 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         const float scale2 = p.scale * 1.4426950408889634f;
         uint32_t n = 0;                                   // tiles so far
         auto wait = [&](uint64_t* bar, uint32_t parity) { warp_wait_phase(bar, parity, gave_up, p.err); tc_fence_after(); };
-        // Q of a segment: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values; 8 rows a warp, whose places in q
-        // the lanes that own the rows know
+        // Q of a segment: this CTA's 64 rows of the item, 9 swizzled chunks of 64 values.  Rows in equal steps through q, whatever
+        // the heads, are nine boxes (rows beyond the sequence's are another's or zeros, and are not used); where a token's step is
+        // not its heads', 8 rows a warp by 16-byte copies, their places in q from the lanes that own the rows (4000 cycles).
+        auto box_q = [&](const Segment& g) {
+            if (warp == 4 && elect_one()) {
+                arrive_expect_at(q_full0, 9 * TR_CHUNK);
+                #pragma unroll
+                for (int c = 0; c < 9; ++c) tma_2d_pair(smb + TR_Q + c * TR_CHUNK, &q_map, c * 64, g.first * p.H + g.rt * ATT_ITEM + (int)rank * 64, q_full0);
+            }
+            __syncwarp();
+        };
         auto start_q = [&](const Segment& g) {
             const int gr = g.rt * ATT_ITEM + (int)rank * 64 + row, tj = gr / p.H;
             const int64_t q_at = gr < g.n * p.H ? (g.first + tj) * p.q_token + (gr - tj * p.H) * p.q_head : -1;
@@ -294,9 +305,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
         };
         Segment g, next;
         bool more = sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, g);
-        if (more) start_q(g);
+        if (more && !p.q_flat) start_q(g);
         cluster_wait();
-        if (more) finish_q();
+        if (more) { if (p.q_flat) box_q(g); else finish_q(); }
         while (more) {
             const int gr = g.rt * ATT_ITEM + (int)rank * 64 + row, tj = gr / p.H, h = gr - tj * p.H, t = g.first + tj;
             const bool live = gr < g.n * p.H;
@@ -370,9 +381,9 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             }
             // ---- output: all of O, then the row's four sums; the next segment's Q and first S under them (this one's S are done)
             more = sched_next<ATT_TILE, TR_LEAD>(p, sched, u, u_end, next);
-            if (more) start_q(next);
+            if (more) { if (p.q_flat) box_q(next); else start_q(next); }
             wait(&B.o_done, (n - 1) & 1);
-            if (more) finish_q();
+            if (more && !p.q_flat) finish_q();
             xch[part * 64 + row] = l;
             group_sync();
             l = (xch[row] + xch[64 + row]) + (xch[128 + row] + xch[192 + row]);
@@ -411,9 +422,12 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                             to[(c + i) * 2] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                 }
                 if (live && part == 0) wk.ml[slot * 128 + pr] = make_float2(m, l);
-                if (rank == 0 && tid == 128 && g.t0 == 0)        // the first part
-                    wk.split[pair] = TreeSplit{ sched.owner(g.item + TR_LEAD + g.tiles - 1) - pair + 1, slot, min(ATT_ITEM, g.n * p.H - g.rt * ATT_ITEM),
-                                                g.rt * ATT_ITEM, g.first };
+                if (rank == 0 && tid == 128) {
+                    const int64_t first = g.item + TR_LEAD;       // the units of the item's tiles; those of its start leave no part
+                    const int q0 = sched.owner(first), n_parts = sched.owner(first + g.tiles - 1) - q0 + 1;
+                    wk.split[slot] = TreeSplit{ n_parts | (pair - q0) << 8 | min(ATT_ITEM, g.n * p.H - g.rt * ATT_ITEM) << 16,
+                                                2 * q0 + (g.item > sched.run_start(q0)), g.rt * ATT_ITEM, g.first };
+                }
             }
             tc_fence_before();
             g = next;
@@ -427,11 +441,13 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 }
 
 // ---------------------------------------------------------------- joining split items
-// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q, added in a fixed order.  A task is 8
-// rows of an item (a part's 128-byte lines) x 128 latent values, or x 32 for items of 24 parts and more (a decoded token's),
-// where 4 groups of 64 threads then take every fourth part.  The blocks share out the tasks of all split items; a task's first
-// parts are on their way before its factors are known, since its time is that of the loads one after another.
-constexpr int MG_ROWS = 8, MG_THREADS = 256, MG_PARTS = 128, MG_MANY = 24, MG_DEEP = 8;
+// out = sum_q f_q O_q / sum_q f_q l_q with f_q = 2^(m_q - max m) over an item's parts q, added in a fixed order.  The runs that
+// worked on an item share its rows out: MG_BLOCKS blocks for each of them, which read that run's record alone (one list that all
+// blocks searched took 3 us more, most of it waiting for the same few lines).  A task is 8 rows (a part's 128-byte lines) x 128
+// latent values, or x 32 for items of 24 parts and more (a decoded token's), where 4 groups of 64 threads then take every fourth
+// part.  A task's first 8 parts a thread are on their way before its factors are known, since its time is that of the loads one
+// after another.  Items of 60 parts: 29.4 us a call so, 32.7 with 8 groups and all parts at once; 4 blocks a run 1 us more.
+constexpr int MG_ROWS = 8, MG_THREADS = 256, MG_PARTS = 128, MG_DEEP = 8, MG_BLOCKS = 8, MG_MANY = 24;
 
 __device__ __forceinline__ float4 load_cg(const float4* p) {      // volatile: not moved behind a test of its weight
     float4 v;
@@ -441,38 +457,22 @@ __device__ __forceinline__ float4 load_cg(const float4* p) {      // volatile: n
 
 template <class T>
 __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ TreeParams p, TreeWork wk, int pairs) {
-    __shared__ TreeSplit split[MG_PARTS];
-    __shared__ int before[MG_PARTS + 1];                          // tasks of the items before
     __shared__ float4 acc[MG_THREADS];
     __shared__ float f[MG_PARTS][MG_ROWS];
     __shared__ float ref[MG_ROWS], sum[MG_ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int own = blockIdx.x / MG_BLOCKS, sub = blockIdx.x % MG_BLOCKS;
     pdl_wait();
-    if (tid < pairs) split[tid] = wk.split[tid];
-    __syncthreads();
-    if (warp == 0) {
-        int b0 = 0;
-        for (int i0 = 0; i0 < pairs; i0 += 32) {
-            const int i = i0 + lane, n = i < pairs ? split[i].parts : 0;
-            int v = n ? (split[i].rows + MG_ROWS - 1) / MG_ROWS * (n < MG_MANY ? 4 : 16) : 0;
-            #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) { const int w = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += w; }
-            if (i < pairs) before[i + 1] = b0 + v;
-            b0 += __shfl_sync(0xffffffffu, v, 31);
-        }
-        if (lane == 0) before[0] = 0;
-    }
-    __syncthreads();
-    const int tasks = before[pairs];
-    for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-        int lo = 0, hi = pairs - 1;
-        while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (before[mid] <= task) lo = mid; else hi = mid - 1; }
-        const TreeSplit& s = split[lo];
-        const int n = s.parts, chunks = n < MG_MANY ? 4 : 16, G = n < MG_MANY ? 1 : 4, elems = MG_THREADS / G, at = task - before[lo];
-        const int pr0 = at / chunks * MG_ROWS, nr = min(MG_ROWS, s.rows - pr0);
-        const int e = tid % elems, grp = tid / elems, r = e % MG_ROWS, c4 = at % chunks * (128 / chunks) + e / MG_ROWS;
+    const int4 s = __ldcg((const int4*)wk.split + own);
+    const int n = s.x & 0xff, rank = s.x >> 8 & 0xff, rows = s.x >> 16;
+    if (!n) return;
+    const int lg = n < MG_MANY ? 0 : 2, G = 1 << lg;
+    const int e = tid & (MG_THREADS / G - 1), grp = tid >> (8 - lg), r = e % MG_ROWS;
+    auto slot = [&](int i) { return i ? (s.y & ~1) + 2 * i : s.y; };
+    for (int at = rank * MG_BLOCKS + sub; at < (rows + MG_ROWS - 1) / MG_ROWS << (2 + lg); at += n * MG_BLOCKS) {
+        const int pr0 = (at >> (2 + lg)) * MG_ROWS, nr = min(MG_ROWS, rows - pr0);
+        const int c4 = ((at & ((4 << lg) - 1)) << (5 - lg)) + e / MG_ROWS;
         const float4* src = wk.part + pr0 / MG_ROWS * 1024 + c4 * 8 + r;
-        auto slot = [&](int i) { return i ? (s.slot0 & ~1) + 2 * i : s.slot0; };
         float4 v[MG_DEEP];
         auto fetch = [&](int i0) {
             #pragma unroll
@@ -520,13 +520,13 @@ __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ Tr
             acc[tid] = a;
             __syncthreads();
             if (grp == 0)
-                for (int q = 1; q < G; ++q) {
-                    const float4 w = acc[q * elems + e];
+                for (int k = 1; k < G; ++k) {
+                    const float4 w = acc[k * (MG_THREADS / G) + e];
                     a.x += w.x; a.y += w.y; a.z += w.z; a.w += w.w;
                 }
         }
         if (grp == 0 && r < nr) {
-            const int gr = s.row0 + pr0 + r, tj = gr / p.H, h = gr - tj * p.H, t = s.first + tj;
+            const int gr = s.z + pr0 + r, tj = gr / p.H, h = gr - tj * p.H, t = s.w + tj;
             const float l = sum[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
             *(uint2*)((T*)p.out + (int64_t)t * p.out_token + (int64_t)h * p.out_head + 4 * c4) =
                 make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
@@ -544,15 +544,15 @@ cudaError_t tree_setup() {
 }
 
 template <class T>
-static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st) {
-    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, map16, wk);
+static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& map16, const CUtensorMap& q_map, const TreeWork& wk, int pairs, cudaStream_t st) {
+    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, map16, q_map, wk);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_pdl_n(k_merge<T>, dim3(16 * pairs), dim3(MG_THREADS), 0, st, p, wk, pairs);      // 8 blocks an SM
+    return launch_pdl_n(k_merge<T>, dim3(2 * pairs * MG_BLOCKS), dim3(MG_THREADS), 0, st, p, wk, pairs);
 }
 
-cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const TreeWork& wk, int pairs, cudaStream_t st) {
-    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, map16, wk, pairs, st) : tree_go<__nv_bfloat16>(p, map, map16, wk, pairs, st);
+cudaError_t launch_tree(const TreeParams& p, int dtype, const CUtensorMap& map, const CUtensorMap& map16, const CUtensorMap& q_map, const TreeWork& wk, int pairs, cudaStream_t st) {
+    return dtype == LK_DT_F16 ? tree_go<__half>(p, map, map16, q_map, wk, pairs, st) : tree_go<__nv_bfloat16>(p, map, map16, q_map, wk, pairs, st);
 }
 
 }  // namespace lk
