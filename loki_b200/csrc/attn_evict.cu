@@ -66,8 +66,9 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS) k_
     __shared__ int s_digit, s_need;
     const int b = blockIdx.x / EV_CTAS, tid = threadIdx.x, lane = tid & 31;
     const uint32_t rank = cluster_rank();
-    const int len = kv_len(p.kv, b, p.err);
+    pdl_wait();
     pdl_trigger();
+    const int len = kv_len(p.kv, b, p.err);
     if (len <= p.budget) {                                       // the whole cluster alike
         cluster_sync();                                          // every CTA has read lens before new_lens, which may be the same array, is written
         if (rank == 0 && tid == 0) { p.n_moves[b] = 0; p.new_lens[b] = len; }
@@ -154,6 +155,7 @@ constexpr int EM_LANES = AT_ROW / 8, EM_ROWS = 4;
 
 __global__ void __launch_bounds__(EM_LANES * EM_ROWS) k_evict_move(EvictParams p) {
     pdl_wait();
+    pdl_trigger();
     const int b = blockIdx.y, n = p.n_moves[b], c = threadIdx.x % EM_LANES, r = threadIdx.x / EM_LANES;
     const int* src = p.src + b * p.region;
     const int* dst = p.dst + b * p.region;
@@ -181,8 +183,7 @@ cudaError_t launch_evict(const EvictParams& p0, int nsm, cudaStream_t st) {
     const int64_t cap = (int64_t)p.kv.table_stride * p.kv.page_size;         // most rows of a sequence
     const int64_t share = (cap + EV_CTAS - 1) / EV_CTAS;
     p.keys = share <= EV_KEYS ? (int)share : EV_KEYS;
-    k_evict_select<<<p.kv.n_seqs * EV_CTAS, EV_THREADS, p.keys * 4, st>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_pdl_n(k_evict_select, dim3(p.kv.n_seqs * EV_CTAS), dim3(EV_THREADS), p.keys * 4, st, p);
     if (e != cudaSuccess || p.region == 0) return e;
     // enough blocks for every SM's 7 at a time, and no more than the most rows that can move
     int64_t per = (7 * nsm + p.kv.n_seqs - 1) / p.kv.n_seqs, most = (p.region + EM_ROWS - 1) / EM_ROWS;

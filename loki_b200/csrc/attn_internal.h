@@ -22,6 +22,9 @@ struct KvView {
     float* mass; int* pos;
 };
 
+// Launches.  Every kernel here is set up while the one before it in the stream ends (launch_pdl_n): it waits for that one before
+// its first access to memory (pdl_wait), and only then lets the next be set up (pdl_trigger), so that a kernel never runs beside
+// one two places before it.  2 us less a call of 10 to 100 us in a stream (append of 8 x 1024 rows 10.2 -> 8.3 us).
 struct RopeParams {
     const void* x; int64_t x_token, x_head;
     void* y; int64_t y_token, y_head;

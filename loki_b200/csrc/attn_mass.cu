@@ -19,6 +19,7 @@
 #include <type_traits>
 #include "attn_tc.cuh"
 #include "attn_sched.cuh"
+#include "moe_internal.h"
 
 namespace lk {
 
@@ -113,6 +114,8 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     __syncwarp();
     cluster_arrive();                                         // the barriers are there; the wait is below, after the schedule
     if (warp == 3) tmem_alloc2(&B.tmem, 512);
+    pdl_wait();
+    pdl_trigger();
     if (warp == 0 || p.kv.n_seqs > 1)
         sched_load<MS_TILE>(p, sched, tid, MS_THREADS, pairs, [](int, int tiles) { return (int64_t)tiles; }, [&]() {
             const int warps = p.kv.n_seqs > 1 ? MS_THREADS / 32 : 1;
@@ -336,8 +339,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
 
 template <class T>
 static cudaError_t mass_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& q_map, const MassWork& wk, int pairs, cudaStream_t st) {
-    k_mass<T><<<2 * pairs, MS_THREADS, MS_SMEM, st>>>(p, map, q_map, wk);
-    return cudaGetLastError();
+    return launch_pdl_n(k_mass<T>, dim3(2 * pairs), dim3(MS_THREADS), MS_SMEM, st, p, map, q_map, wk);
 }
 
 cudaError_t mass_setup() {

@@ -7,6 +7,8 @@
 // 4e-3 at position 1e5, and sin/cos in the kernel would cost more than the rotation.
 #include <math.h>
 #include "attn_internal.h"
+#include "attn_tc.cuh"
+#include "moe_internal.h"
 
 namespace lk {
 
@@ -82,6 +84,8 @@ __global__ void __launch_bounds__(256) k_rope(RopeParams p, int units, int block
     T* y = (T*)p.y + t * p.y_token;
     Vt va[N], vb[N];
     int h[N], ea[N], u[N];
+    pdl_wait();
+    pdl_trigger();
     #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int idx = idx0 + k * blockDim.x;
@@ -121,9 +125,8 @@ static cudaError_t rope_n(const RopeParams& p, int layout, cudaStream_t st) {
     const int units = p.rot / 2 / V + (p.copy ? (p.head_dim - p.rot) / V : 0), all = p.H * units;
     const int threads = all >= 256 * N ? 256 : ((all + N - 1) / N + 31) / 32 * 32;
     const int bpt = (all + threads * N - 1) / (threads * N);
-    if (layout == LK_ROPE_HALF) k_rope<T, V, LK_ROPE_HALF, N><<<(unsigned)(p.T * bpt), threads, 0, st>>>(p, units, bpt);
-    else k_rope<T, V, LK_ROPE_INTERLEAVED, N><<<(unsigned)(p.T * bpt), threads, 0, st>>>(p, units, bpt);
-    return cudaGetLastError();
+    if (layout == LK_ROPE_HALF) return launch_pdl_n(k_rope<T, V, LK_ROPE_HALF, N>, dim3(p.T * bpt), dim3(threads), 0, st, p, units, bpt);
+    return launch_pdl_n(k_rope<T, V, LK_ROPE_INTERLEAVED, N>, dim3(p.T * bpt), dim3(threads), 0, st, p, units, bpt);
 }
 
 // few tokens: a unit a thread fills more SMs; many: four in flight
@@ -173,6 +176,8 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p) {
     const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int t = (int)(idx / AP_UNITS), u = (int)(idx % AP_UNITS);
     if (t >= p.T) return;
+    pdl_wait();
+    pdl_trigger();
     int b = 0;                                   // the sequence: last b with starts[b] <= t
     for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
         const int mid = (lo + hi) >> 1;
@@ -207,9 +212,8 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p) {
 template <class TI, class TO>
 static cudaError_t append_go(const AppendParams& p, int layout, cudaStream_t st) {
     const unsigned grid = (unsigned)(((int64_t)p.T * AP_UNITS + 255) / 256);
-    if (layout == LK_ROPE_HALF) k_append<TI, TO, LK_ROPE_HALF><<<grid, 256, 0, st>>>(p);
-    else k_append<TI, TO, LK_ROPE_INTERLEAVED><<<grid, 256, 0, st>>>(p);
-    return cudaGetLastError();
+    if (layout == LK_ROPE_HALF) return launch_pdl_n(k_append<TI, TO, LK_ROPE_HALF>, dim3(grid), dim3(256), 0, st, p);
+    return launch_pdl_n(k_append<TI, TO, LK_ROPE_INTERLEAVED>, dim3(grid), dim3(256), 0, st, p);
 }
 
 cudaError_t launch_append(const AppendParams& p, int in_dtype, int kv_dtype, int layout, cudaStream_t st) {

@@ -148,12 +148,13 @@ k_tree(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
     }
     cluster_arrive();                                     // the barriers are there; the wait comes with a role's first use of the other CTA
     if (warp == 3) tmem_alloc2(&B.tmem, TR_TMEM);
+    pdl_wait();
+    pdl_trigger();
     if (warp == 0 || p.kv.n_seqs > 1) sched_load<ATT_TILE>(p, sched, tid, TR_THREADS, pairs,
         [&](int n, int tiles) { return (int64_t)((n * p.H + ATT_ITEM - 1) / ATT_ITEM) * (TR_LEAD + tiles); }, []() {});
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    pdl_trigger();
     if (rank == 0 && tid == 128) wk.split[2 * pair].info = wk.split[2 * pair + 1].info = 0;
     int64_t u = pair < sched.runs ? sched.run_start(pair) : 0;
     const int64_t u_end = pair < sched.runs ? sched.run_start(pair + 1) : 0;
@@ -463,6 +464,7 @@ __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ Tr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int own = blockIdx.x / MG_BLOCKS, sub = blockIdx.x % MG_BLOCKS;
     pdl_wait();
+    pdl_trigger();
     const int4 s = __ldcg((const int4*)wk.split + own);
     const int n = s.x & 0xff, rank = s.x >> 8 & 0xff, rows = s.x >> 16;
     if (!n) return;
@@ -545,8 +547,7 @@ cudaError_t tree_setup() {
 
 template <class T>
 static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& map16, const CUtensorMap& q_map, const TreeWork& wk, int pairs, cudaStream_t st) {
-    k_tree<T><<<2 * pairs, TR_THREADS, TR_SMEM, st>>>(p, map, map16, q_map, wk);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_pdl_n(k_tree<T>, dim3(2 * pairs), dim3(TR_THREADS), TR_SMEM, st, p, map, map16, q_map, wk);
     if (e != cudaSuccess) return e;
     return launch_pdl_n(k_merge<T>, dim3(2 * pairs * MG_BLOCKS), dim3(MG_THREADS), 0, st, p, wk, pairs);
 }
