@@ -50,7 +50,8 @@ typedef struct LkRopeConfig {
 } LkRopeConfig;
 
 /* The paged cache of n_seqs sequences.  Row i of sequence b is pool row
- * block_table[b * table_stride + i / page_size] * page_size + i % page_size. */
+ * block_table[b * table_stride + i / page_size] * page_size + i % page_size.  Sequences may share pages where a call only
+ * reads rows (lk_attn_tree); lk_attn_append, lk_attn_mass and lk_attn_evict write what their sequences' pages hold. */
 typedef struct LkKvCache {
     void* rows;                        /* [n_pages * page_size] rows, 16-byte aligned */
     int64_t row_stride;                /* elements from one row to the next: >= 576 and a multiple of 8 */
@@ -104,8 +105,9 @@ LK_API int lk_attn_tree(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, i
                         float* lse, lk_stream_t stream);
 
 /* cache->mass[row k] = decay * mass + sum_t weight[t] * sum_h exp(scale * q . row_k - lse[t][h]) for every row of every
- * sequence (context and drafted), over the tokens that see it: the attention weight that lk_attn_tree gave it (sequences without tokens keep theirs).  weight
- * [T] (null: all 1; 0 for rejected drafts: only tokens of positive weight count).  One owner adds each row's terms in a fixed order, so results repeat. */
+ * sequence (context and drafted), over the tokens that see it: the attention weight that lk_attn_tree gave it (sequences
+ * without tokens keep theirs).  weight [T] (null: all 1; 0 for rejected drafts: only tokens of positive weight count).
+ * Each row's terms are added in a fixed order, so results repeat. */
 LK_API int lk_attn_mass(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H,
                         const int* starts, const uint64_t* tree, float scale, const float* lse, const float* weight,
                         float decay, lk_stream_t stream);
