@@ -327,6 +327,32 @@ def test_mass_of_tree_sums_to_the_rows(A, ctx):
     assert torch.equal(m, again)
 
 
+def test_mass_weights_and_shared_key_tiles(A, ctx):
+    """Few key tiles and many rows, so that several CTA pairs share a tile; weights that are zero, negative or NaN take their
+    token out; a sequence whose tokens are all out only decays; calls of other shapes between leave the repeats' bits alone."""
+    pg = R.Paged([700, 300, 500, 90], [40, 3, 0, 5], 64, torch.bfloat16, "cuda", seed=31)
+    H, new = 40, [40, 3, 0, 5]
+    q, masks = _q(pg, H), R.tree_masks(new, 9)
+    _, lse, _, _ = R.tree(pg, q, masks, SCALE)
+    lse = lse.float()
+    w = torch.rand(48, generator=torch.Generator().manual_seed(8)) * 2
+    w[torch.arange(1, 40, 4)] = torch.tensor([0.0, -1.0, float("nan"), 0.0, -0.0, float("-inf"), 0.0, 0.0, -3.0, 0.0])
+    w[40:43] = 0.0
+    m0 = torch.rand(pg.n_slots, generator=torch.Generator().manual_seed(6))
+    words, other = R.to_words(masks, "cuda"), R.Paged([1000], [2], 16, torch.bfloat16, "cuda", seed=2)
+    qo, mo = _q(other, 16).cuda(), torch.zeros(other.n_slots, device="cuda")
+    runs = []
+    for _ in range(20):
+        m = m0.cuda()
+        ctx.mass(q.cuda(), lse.cuda(), pg.cache(A, mass=m), pg.starts, words, SCALE, weight=w.cuda(), decay=0.5)
+        ctx.mass(qo, torch.zeros(2, 16, device="cuda"), other.cache(A, mass=mo), other.starts, None, 1e-3)
+        runs.append(m)
+    ctx.device_error()
+    want, tol = R.mass(pg, q, lse, masks, SCALE, torch.where(w > 0, w, torch.zeros(())), 0.5, m0)
+    assert ((runs[0].cpu().double() - want).abs() <= tol + 1e-30).all()
+    assert all(torch.equal(m, runs[0]) for m in runs)
+
+
 # ---------------------------------------------------------------- eviction
 def _evict_case(lens, page, seed, ties=False):
     pg = R.Paged(lens, [0] * len(lens), page, torch.bfloat16, "cuda", seed=seed)
