@@ -353,6 +353,30 @@ def test_mass_weights_and_shared_key_tiles(A, ctx):
     assert all(torch.equal(m, runs[0]) for m in runs)
 
 
+def test_many_sequences(A):
+    """More sequences than a warp has lanes and than a launch has CTA pairs: attention and mass."""
+    g = torch.Generator().manual_seed(3)
+    n = 230
+    lens, new = torch.randint(0, 300, (n,), generator=g).tolist(), torch.randint(0, 4, (n,), generator=g).tolist()
+    H, T = 8, sum(new)
+    many = A.AttnContext(0, n, T)
+    pg = R.Paged(lens, new, 16, torch.bfloat16, "cuda", seed=41)
+    q, masks = _q(pg, H), R.tree_masks(new, 5)
+    words = R.to_words(masks, "cuda")
+    m0 = torch.rand(pg.n_slots, generator=g)
+    m = m0.cuda()
+    cache = pg.cache(A, mass=m)
+    out, lse = many.tree(q.cuda(), cache, pg.starts, words, SCALE)
+    w = torch.rand(T, generator=g) * (torch.rand(T, generator=g) < 0.7)
+    many.mass(q.cuda(), lse, cache, pg.starts, words, SCALE, weight=w.cuda(), decay=0.25)
+    many.device_error()
+    want, wl, tol, ltol = R.tree(pg, q, masks, SCALE)
+    assert ((out.cpu().double() - want).abs() <= tol).all() and ((lse.cpu().double() - wl).abs() <= ltol).all()
+    wm, mt = R.mass(pg, q, lse.cpu(), masks, SCALE, w, 0.25, m0)
+    assert ((m.cpu().double() - wm).abs() <= mt + 1e-30).all()
+    many.close()
+
+
 # ---------------------------------------------------------------- eviction
 def _evict_case(lens, page, seed, ties=False):
     pg = R.Paged(lens, [0] * len(lens), page, torch.bfloat16, "cuda", seed=seed)
