@@ -128,9 +128,11 @@ class AttnContext:
         _need(layout in _LAYOUT, "layout: interleaved or half")
         T, H, D = x.shape
         if out is None:
-            out = x.new_empty((T, H, D))
-        to, so = _rows(out, "out", dev, D)
-        _need(out.shape == x.shape and out.dtype is x.dtype, "out: x's shape and dtype")
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            to, so = out.data_ptr(), (H * D, D)
+        else:
+            to, so = _rows(out, "out", dev, D)
+            _need(out.shape == x.shape and out.dtype is x.dtype, "out: x's shape and dtype")
         rc = self._lib.lk_attn_rope(self.ctx, _DTYPE[x.dtype], at, st[0], st[1], to, so[0], so[1], T, H, D, rot_offset, table.rot_dim,
                                     _LAYOUT[layout], grad, _dense(pos, "pos", _I32, dev, T), table.address, table.max_pos,
                                     _queue(stream, dev))
@@ -168,12 +170,17 @@ class AttnContext:
         T, H, _ = q.shape
         if out is None:
             out = q.new_empty((T, H, ATTN_LATENT))
+            to, so = out.data_ptr(), (H * ATTN_LATENT, ATTN_LATENT)
+        else:
+            to, so = _rows(out, "out", self.device, ATTN_LATENT)
+            _need(out.dim() == 3 and out.shape[:2] == q.shape[:2] and out.dtype is q.dtype, "out: [T][H][512] of q's dtype")
         if lse is None:
             lse = q.new_empty((T, H), dtype=_F32)
-        to, so = _rows(out, "out", self.device, ATTN_LATENT)
-        _need(out.dim() == 3 and out.shape[:2] == q.shape[:2] and out.dtype is q.dtype, "out: [T][H][512] of q's dtype")
+            lse_at = lse.data_ptr()
+        else:
+            lse_at = _dense(lse, "lse", _F32, self.device, T, H)
         rc = self._lib.lk_attn_tree(self.ctx, cache._ref, at, st[0], st[1], T, H, starts_at, tree_at, scale, to, so[0], so[1],
-                                    _dense(lse, "lse", _F32, self.device, T, H), _queue(stream, self.device))
+                                    lse_at, _queue(stream, self.device))
         if rc:
             self._check(rc)
         return out, lse

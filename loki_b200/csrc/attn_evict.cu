@@ -10,7 +10,7 @@
 // memory (sequences of up to 8 x EV_KEYS rows; beyond, it computes them again in each pass).  Per digit the CTAs' histograms
 // are added over distributed shared memory by each CTA alike, so one cluster barrier a digit is all they exchange; ranks come
 // from ordered block scans and the CTAs' totals.  It reads 8 bytes a row once and is bound by its ~10 barriers and scans
-// (one CTA per sequence took 170 us of a 16-sequence call).  1200 rows cut to 1024: 13.6 us a call, nearly all of it this.
+// (one CTA per sequence took 170 us of a 16-sequence call).  1200 rows cut to 1024: 12.9 us a call, nearly all of it this.
 // k_evict_move: 72 threads copy a row's 1152 bytes; memory-bound.  16 sequences of 6000 to 40 000 rows cut to 8192: both 22.5 us,
 // 168 MB at 7.5 TB/s, which L2 gives in part (the plain forms 377 and 470).
 #include "attn_tc.cuh"

@@ -17,7 +17,8 @@
 // waits at five stages of K a tile.  L2 is not what bounds it (136 KB a CTA; leaving V's loads out gains under 5 %).
 // Times a call: 64 nodes over 65 000 rows 1055 us (1.10 PFLOP/s at the 1.2 to 1.4 GHz that the power allows), 8 nodes over 16 384
 // rows 49.7, one token over 30 011 rows 27.6 (of them 8 the tiles and 10 the parts and their merge), 16 sequences of 3 to 17
-// nodes on 32 heads 95, one tile 15.6 (two launches, 3 us of set-up each way; the plain forms: 24 960, 1472, 836, 6247, 694).
+// nodes on 32 heads 95, one tile 11.6 (14 where the pages could hold more and the merge is launched); the plain forms: 24 960, 1472,
+// 836, 6247, 694.
 //
 // Roles (384 threads a CTA): warp 0 loads (TMA, ring of 8 x 16 KB), warps 1 and 2 of CTA 0 issue the MMAs of S and of O,
 // warp 3 repairs tail tiles, warps 4-11 do softmax, O's scaling and the output (two threads per tensor-memory lane, four per
@@ -550,7 +551,8 @@ cudaError_t tree_setup() {
 template <class T>
 static cudaError_t tree_go(const TreeParams& p, const CUtensorMap& map, const CUtensorMap& map16, const CUtensorMap& q_map, const TreeWork& wk, int pairs, cudaStream_t st) {
     const cudaError_t e = launch_pdl_n(k_tree<T>, dim3(2 * pairs), dim3(TR_THREADS), TR_SMEM, st, p, map, map16, q_map, wk);
-    if (e != cudaSuccess) return e;
+    // no item is split where a sequence's pages hold one tile at most: a launch less (one tile 2 us less a call)
+    if (e != cudaSuccess || p.kv.table_stride << p.kv.page_shift <= ATT_TILE) return e;
     return launch_pdl_n(k_merge<T>, dim3(2 * pairs * MG_BLOCKS), dim3(MG_THREADS), 0, st, p, wk, pairs);
 }
 
