@@ -152,19 +152,10 @@ cudaError_t launch_rope(const RopeParams& p, int dtype, int layout, cudaStream_t
 }
 
 // ---------------------------------------------------------------- append
-// One thread per 8 latent values (64 of them) or 8 rotated pairs (4): 68 units a token.  8 x 1024 fp32 rows take 8.3 us a call,
-// 3.2 of them the bytes: the launch and the chain of loads from starts to page to row are the rest.
+// One thread per 8 latent values (64 of them) or 8 rotated pairs (4): 68 units a token.  8 x 1024 fp32 rows take 7.1 us a call,
+// 3.2 of them the bytes: the launch and the chain of loads from starts to page are the rest (8.3 with the values loaded after it).
 constexpr int AP_UNITS = AT_LATENT / 8 + AT_ROPE / 16;
 
-template <class T> __device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
-    constexpr int N = 16 / sizeof(T);
-    #pragma unroll
-    for (int k = 0; k < 8 / N; ++k) {
-        const Vec<T, N> w = *(const Vec<T, N>*)(src + k * N);
-        #pragma unroll
-        for (int i = 0; i < N; ++i) v[k * N + i] = to_f<T>(w.v[i]);
-    }
-}
 template <class T> __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
     Vec<T, 8> w;
     #pragma unroll
@@ -179,6 +170,18 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p) {
     if (t >= p.T) return;
     pdl_wait();
     pdl_trigger();
+    // the values first: their loads run under the search for their place.  u < 64: 8 of the latent in x; else 8 pairs in x and y
+    const int r = u - AT_LATENT / 8;
+    const int ea = LAYOUT == LK_ROPE_HALF ? 8 * r : 16 * r, eb = ea + (LAYOUT == LK_ROPE_HALF ? AT_ROPE / 2 : 8);
+    const TI* src = r < 0 ? (const TI*)p.latent + t * p.latent_ld + u * 8 : (const TI*)p.k_rope + t * p.rope_ld + ea;
+    constexpr int N = 16 / sizeof(TI);
+    Vec<TI, N> x[8 / N], y[8 / N];
+    #pragma unroll
+    for (int k = 0; k < 8 / N; ++k) x[k] = ((const Vec<TI, N>*)src)[k];
+    if (r >= 0)
+        #pragma unroll
+        for (int k = 0; k < 8 / N; ++k) y[k] = ((const Vec<TI, N>*)(src + (eb - ea)))[k];
+    const int pos = p.pos[t];
     int b = 0;                                   // the sequence: last b with starts[b] <= t
     for (int lo = 0, hi = p.kv.n_seqs - 1; lo <= hi;) {
         const int mid = (lo + hi) >> 1;
@@ -189,24 +192,22 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p) {
     const int slot = kv_slot(p.kv, b, kv_len(p.kv, b, p.err) + i, p.err);
     if (slot < 0) return;
     TO* row = (TO*)p.kv.rows + (int64_t)slot * p.kv.row_stride;
-    if (u < AT_LATENT / 8) {
-        float v[8];
-        load8<TI>((const TI*)p.latent + t * p.latent_ld + u * 8, v);
+    float v[8];
+    #pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = to_f<TI>(x[k / N].v[k % N]);
+    if (r < 0) {
         store8<TO>(row + u * 8, v);
         if (u == 0) {
-            if (p.kv.pos) p.kv.pos[slot] = p.pos[t];
+            if (p.kv.pos) p.kv.pos[slot] = pos;
             if (p.kv.mass) p.kv.mass[slot] = 0.0f;
         }
         return;
     }
-    const int r = u - AT_LATENT / 8;
-    const int ea = LAYOUT == LK_ROPE_HALF ? 8 * r : 16 * r, eb = ea + (LAYOUT == LK_ROPE_HALF ? AT_ROPE / 2 : 8);
-    const TI* k = (const TI*)p.k_rope + t * p.rope_ld;
-    float a[8], c[8];
-    load8<TI>(k + ea, a);
-    load8<TI>(k + eb, c);
-    rotate<8, LAYOUT>(a, c, p.table + (int64_t)checked_pos(p.pos[t], p.max_pos, p.err) * (AT_ROPE / 2) + 8 * r, 1.0f);
-    store8<TO>(row + AT_LATENT + ea, a);
+    float c[8];
+    #pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = to_f<TI>(y[k / N].v[k % N]);
+    rotate<8, LAYOUT>(v, c, p.table + (int64_t)checked_pos(pos, p.max_pos, p.err) * (AT_ROPE / 2) + 8 * r, 1.0f);
+    store8<TO>(row + AT_LATENT + ea, v);
     store8<TO>(row + AT_LATENT + eb, c);
 }
 
