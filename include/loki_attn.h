@@ -116,7 +116,8 @@ LK_API int lk_attn_mass(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, i
  * position >= next_pos[b] - recent), then those of the largest mass; equal ones in row order, a NaN mass last.  The kept
  * rows at or beyond `budget` move, in order, into the holes before it (row, mass and pos); nothing else is written.
  * new_lens [n_seqs] receives min(lens, budget) and may be the cache's lens array itself.  Needs cache->mass and pos.
- * Rows need no order: each key carries its position in its rotated part, and pos tells it. */
+ * Rows need no order: each key carries its position in its rotated part, and pos tells it.
+ * The move lists are made on the first call that needs ones of their size, so not under capture; a captured call keeps its own. */
 LK_API int lk_attn_evict(LkAttnCtx* ctx, const LkKvCache* cache, int budget, int sinks, int recent, const int* next_pos,
                          int* new_lens, lk_stream_t stream);
 

@@ -10,7 +10,10 @@ struct LkAttnCtx {
     LkAttnConfig cfg;
     int device = 0, nsm = 0;
     int* err = nullptr;
-    int* n_moves = nullptr; int* moves = nullptr; int64_t moves_cap = 0;      // eviction: [2][n_seqs][region]
+    int* n_moves = nullptr;
+    // eviction: [2][n_seqs][region] of the last of `moves`.  A captured graph keeps the address that its call had, so a list that
+    // became too small stays until the context ends; sizes are powers of two, so the ones before take no more than the last.
+    int* moves[64] = {}; int n_lists = 0; int64_t moves_cap = 0;
     TreeWork work{}; int pairs = 0;                                           // lk_attn_tree: parts of split items
     MassWork mass{};
     char msg[256] = {0};
@@ -126,8 +129,9 @@ int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
 void lk_attn_destroy(LkAttnCtx* c) {
     if (!c) return;
     OnDevice on(c->device);
-    void* ptrs[] = { c->err, c->n_moves, c->moves, c->work.part, c->mass.part };
+    void* ptrs[] = { c->err, c->n_moves, c->work.part, c->mass.part };
     for (void* p : ptrs) if (p) cudaFree(p);
+    for (int i = 0; i < c->n_lists; ++i) cudaFree(c->moves[i]);
     delete c;
 }
 
@@ -276,13 +280,14 @@ int lk_attn_evict(LkAttnCtx* c, const LkKvCache* cache, int budget, int sinks, i
     const int64_t need = 2 * p.region * p.kv.n_seqs;
     if (need > c->moves_cap) {
         if (int rc = may_allocate(c, (cudaStream_t)stream)) return rc;
-        LK_CU(cudaFree(c->moves));
-        c->moves = nullptr; c->moves_cap = 0;
-        LK_CU(cudaMalloc((void**)&c->moves, need * sizeof(int)));
-        c->moves_cap = need;
+        int64_t cap2 = 1024;
+        while (cap2 < need) cap2 *= 2;
+        LK_CU(cudaMalloc((void**)&c->moves[c->n_lists], cap2 * sizeof(int)));
+        ++c->n_lists;
+        c->moves_cap = cap2;
     }
     p.budget = budget; p.sinks = sinks; p.recent = recent; p.next_pos = next_pos; p.new_lens = new_lens;
-    p.src = c->moves; p.dst = c->moves + p.region * p.kv.n_seqs; p.n_moves = c->n_moves; p.err = c->err;
+    p.src = c->n_lists ? c->moves[c->n_lists - 1] : nullptr; p.dst = p.src + p.region * p.kv.n_seqs; p.n_moves = c->n_moves; p.err = c->err;
     LK_CU(launch_evict(p, c->nsm, (cudaStream_t)stream));
     return LK_OK;
 }

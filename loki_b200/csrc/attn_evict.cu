@@ -157,14 +157,16 @@ constexpr int EM_LANES = AT_ROW / 8, EM_ROWS = 4;
 __global__ void __launch_bounds__(EM_LANES * EM_ROWS) k_evict_move(EvictParams p) {
     pdl_wait();
     pdl_trigger();
-    const int b = blockIdx.y, n = p.n_moves[b], c = threadIdx.x % EM_LANES, r = threadIdx.x / EM_LANES;
+    const int b = blockIdx.y, n = (int)min((int64_t)p.n_moves[b], p.region), c = threadIdx.x % EM_LANES, r = threadIdx.x / EM_LANES;
+    const unsigned pool = (unsigned)p.kv.n_pages << p.kv.page_shift;
     const int* src = p.src + b * p.region;
     const int* dst = p.dst + b * p.region;
     const int step = gridDim.x * EM_ROWS;
     for (int m = blockIdx.x * EM_ROWS + r; m < n; m += 2 * step) {
         const int m2 = m + step;
         const int s0 = src[m], d0 = dst[m], s1 = m2 < n ? src[m2] : -1, d1 = m2 < n ? dst[m2] : -1;
-        const bool go0 = s0 >= 0 && d0 >= 0, go1 = s1 >= 0 && d1 >= 0;       // a bad page's rows stay
+        // a bad page's rows (-1) stay
+        const bool go0 = (unsigned)s0 < pool && (unsigned)d0 < pool, go1 = (unsigned)s1 < pool && (unsigned)d1 < pool;
         const uint16_t* rows = (const uint16_t*)p.kv.rows + c * 8;
         uint4 v0, v1;
         if (go0) v0 = __ldcs((const uint4*)(rows + (int64_t)s0 * p.kv.row_stride));

@@ -1,0 +1,78 @@
+"""What the latent-cache attention operators promise around their numbers: captured graphs, streams, workspaces, error
+words, refused arguments, and non-finite values where they must and must not show."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import attn_ref as R
+
+pytestmark = pytest.mark.gpu
+
+SCALE = 192 ** -0.5
+
+
+@pytest.fixture(scope="module")
+def A(native):
+    from loki_b200 import attention
+    return attention
+
+
+@pytest.fixture()
+def ctx(A):
+    c = A.AttnContext(0, max_seqs=16, max_tokens=512)
+    yield c
+    c.close()
+
+
+def _eviction(lens, page, seed):
+    """A filled pool whose rows have random masses and their index as position, and what `expect` needs of it."""
+    pg = R.Paged(lens, [0] * len(lens), page, torch.bfloat16, "cuda", seed=seed)
+    mass = torch.rand(pg.n_slots, generator=torch.Generator().manual_seed(seed))
+    pos = torch.zeros(pg.n_slots, dtype=torch.int32)
+    for s in pg.slots:
+        pos[s] = torch.arange(len(s), dtype=torch.int32)
+    return pg, mass, pos
+
+
+def _evicted(pg, rows0, mass, pos, budget, nxt):
+    """rows, mass and pos after the rule's moves; the new lengths."""
+    new, moves = R.evict(pg.lens, pg.slots, mass.numpy(), pos.numpy(), budget, 2, 8, nxt)
+    rows, m, p = rows0.clone(), mass.clone(), pos.clone()
+    for s, d in moves:
+        rows[d], m[d], p[d] = rows0[s], mass[s], pos[s]
+    return rows, m, p, new, len(moves)
+
+
+def test_captured_eviction_after_a_larger_call(A, ctx):
+    """A graph that holds an eviction replays rightly after later calls of the context needed larger move lists."""
+    pg, mass, pos = _eviction([400], 16, 1)
+    md, pd, nxt = mass.cuda(), pos.cuda(), torch.tensor([400], dtype=torch.int32, device="cuda")
+    cache, new = pg.cache(A, mass=md, pos=pd), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows0 = pg.rows.clone()
+    ctx.evict(cache, 64, nxt, sinks=2, recent=8, new_lens=new)           # makes the lists
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ctx.evict(cache, 64, nxt, sinks=2, recent=8, new_lens=new)
+    want_rows, want_m, want_p, want_new, n_moves = _evicted(pg, rows0, mass, pos, 64, [400])
+    assert n_moves > 20
+    held = []
+    for n in (2000, 9000, 30000):                                        # lists of 8, 16 and 32 times the size and more
+        big, bm, bp = _eviction([n, n - 7, 5], 64, n)
+        bmd, bpd = bm.cuda(), bp.cuda()
+        big_nxt = [n, n - 7, 5]
+        b0 = big.rows.clone()
+        got = ctx.evict(big.cache(A, mass=bmd, pos=bpd), n // 2, torch.tensor(big_nxt, dtype=torch.int32, device="cuda"), sinks=2, recent=8)
+        held.append(torch.full((1 << 18,), 0x7fffffff, dtype=torch.int32, device="cuda"))      # memory that was let go is used again
+        for t, v in ((pg.rows, rows0), (md, mass), (pd, pos)):
+            t.copy_(v)
+        g.replay()
+        torch.cuda.synchronize()
+        ctx.device_error()
+        assert new.tolist() == want_new
+        assert torch.equal(pg.rows.view(torch.int16), want_rows.view(torch.int16)) and torch.equal(md.cpu(), want_m) and torch.equal(pd.cpu(), want_p)
+        w_rows, w_m, w_p, w_new, _ = _evicted(big, b0, bm, bp, n // 2, big_nxt)
+        assert got.tolist() == w_new and torch.equal(big.rows.view(torch.int16), w_rows.view(torch.int16))
+        assert torch.equal(bmd.cpu(), w_m) and torch.equal(bpd.cpu(), w_p)
