@@ -79,7 +79,7 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS) k_
     // this CTA's rows [lo, hi); thread t ranks rows [lo + t * per, ..) of them
     const int share = (len + EV_CTAS - 1) / EV_CTAS, lo = min(len, (int)rank * share), hi = min(len, lo + share), n = hi - lo;
     const bool kept_keys = share <= p.keys;
-    auto key_at = [&](int i) { return kept_keys ? keys[i - lo] : evict_key(p, kv_slot(p.kv, b, i, nullptr), next); };
+    auto key_at = [&](int i, int* err = nullptr) { return kept_keys ? keys[i - lo] : evict_key(p, kv_slot(p.kv, b, i, err), next); };
     if (kept_keys) for (int i = tid; i < n; i += EV_THREADS) keys[i] = evict_key(p, kv_slot(p.kv, b, lo + i, p.err), next);
     uint32_t prefix = 0;
     int need = p.budget;                                         // rank of the threshold among keys with this prefix
@@ -90,7 +90,7 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS) k_
         __syncthreads();
         for (int i0 = 0; i0 < n; i0 += EV_THREADS) {
             const int i = i0 + tid;
-            const uint32_t k = i < n ? key_at(lo + i) : 0;
+            const uint32_t k = i < n ? key_at(lo + i, d ? nullptr : p.err) : 0;      // bad pages are reported once
             const bool in = i < n && (d == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
             // one addition per distinct digit of a warp: masses share their leading digits
             const uint32_t digit = in ? (k >> shift) & 255 : 256, same = __match_any_sync(0xffffffffu, digit);

@@ -76,3 +76,45 @@ def test_captured_eviction_after_a_larger_call(A, ctx):
         w_rows, w_m, w_p, w_new, _ = _evicted(big, b0, bm, bp, n // 2, big_nxt)
         assert got.tolist() == w_new and torch.equal(big.rows.view(torch.int16), w_rows.view(torch.int16))
         assert torch.equal(bmd.cpu(), w_m) and torch.equal(bpd.cpu(), w_p)
+
+
+def _long_eviction(n, budget, bad_page=None):
+    """One sequence whose keys do not fit the selection's shared memory, rows coded by their place: what is left of it."""
+    page, n_pages = 256, (n + 255) // 256
+    g = torch.Generator(device="cuda").manual_seed(n)
+    ids = torch.randperm(n_pages, generator=g, device="cuda").int()
+    at = ids.long()[torch.arange(n, device="cuda") // page] * page + torch.arange(n, device="cuda") % page
+    i = torch.arange(n, device="cuda")
+    rows = torch.zeros(n_pages * page, R.ROW, dtype=torch.float16, device="cuda")
+    rows[at, 0], rows[at, 575] = (i // 1024).half(), (i % 1024).half()
+    mass, pos = torch.zeros(n_pages * page, device="cuda"), torch.zeros(n_pages * page, dtype=torch.int32, device="cuda")
+    mass[at], pos[at] = (torch.rand(n, generator=g, device="cuda") * 4096).floor(), i.int()          # ties among them
+    if bad_page is not None:
+        ids[bad_page] = n_pages
+    return rows, page, ids[None].contiguous(), mass, pos, at
+
+
+@pytest.mark.parametrize("bad", [False, True])
+def test_eviction_beyond_the_keys_that_fit(A, native, bad):
+    """Sequences of more than 8 x 49 152 rows: the same rule, and a bad page id is reported and its rows rank last."""
+    n, budget = 400_016, 150_001
+    rows, page, table, mass, pos, at = _long_eviction(n, budget, 1500 if bad else None)
+    ctx, m0, p0, r0 = A.AttnContext(0, 1, 1), mass.clone(), pos.clone(), rows[:, [0, 575]].clone()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    new = ctx.evict(A.KvCache(rows, page, table, lens, mass=mass, pos=pos), budget, lens.clone(), sinks=4, recent=100)
+    torch.cuda.synchronize()
+    i = torch.arange(n, device="cuda")
+    key = m0[at].double()
+    key[(i < 4) | (i >= n - 100)] = math.inf
+    key[(i // page == 1500) & bad] = -1.0
+    keep = torch.zeros(n, dtype=torch.bool, device="cuda")
+    keep[torch.sort(key, descending=True, stable=True).indices[:budget]] = True
+    dst, src = at[(i < budget) & ~keep], at[(i >= budget) & keep]
+    assert len(dst) == len(src) > 50_000 and new.tolist() == [budget]
+    r0[dst], m0[dst], p0[dst] = r0[src], m0[src], p0[src]
+    assert torch.equal(rows[:, [0, 575]], r0) and torch.equal(mass, m0) and torch.equal(pos, p0)
+    if bad:
+        with pytest.raises(native.NativeError, match="page"):
+            ctx.device_error()
+    ctx.device_error()
+    ctx.close()
