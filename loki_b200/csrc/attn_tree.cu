@@ -501,8 +501,9 @@ __global__ void __launch_bounds__(MG_THREADS) k_merge(const __grid_constant__ Tr
             #pragma unroll
             for (int k = 0; k < MG_PARTS / 32; ++k)
                 if (32 * k < n) {
-                    // a part that saw nothing has sum 0; one of NaN scores alone has no maximum, and a NaN sum
-                    const float w = ml[k].y == 0.0f ? 0.0f : exp2_approx((ml[k].x == -INFINITY ? 0.0f : ml[k].x) - rf);
+                    // a part that saw nothing has sum 0; one that saw a NaN score has a NaN sum, which must reach the row however
+                    // small the part's maximum is against the others' (or with none, where all its scores are NaN)
+                    const float w = ml[k].y == 0.0f ? 0.0f : ml[k].y != ml[k].y ? ml[k].y : exp2_approx(ml[k].x - rf);
                     if (32 * k + lane < n) f[32 * k + lane][warp] = w;
                     l += w == 0.0f ? 0.0f : w * ml[k].y;
                 }

@@ -118,3 +118,16 @@ def test_eviction_beyond_the_keys_that_fit(A, native, bad):
             ctx.device_error()
     ctx.device_error()
     ctx.close()
+
+
+@pytest.mark.parametrize("n", [100, 9000])
+def test_a_seen_nan_reaches_every_output(A, ctx, n):
+    """A NaN context row is seen by every token, so every row of out and lse is NaN: also where the cache is shared out in parts
+    and another part's scores are so large that the NaN's part has no weight against them."""
+    pg = R.Paged([n], [2], 64, torch.bfloat16, "cuda", seed=3)
+    q = torch.randn(2, 4, R.ROW, generator=torch.Generator().manual_seed(1)).bfloat16()
+    pg.set_row(0, 5, float("nan"))
+    pg.set_row(0, n - 10, (6 * q[0, 0].float()).bfloat16())              # a score of about 250 for one (token, head)
+    out, lse = ctx.tree(q.cuda(), pg.cache(A), pg.starts, R.to_words([1, 3], "cuda"), SCALE)
+    ctx.device_error()
+    assert lse.isnan().all() and out.isnan().all()
