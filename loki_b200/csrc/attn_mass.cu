@@ -254,7 +254,7 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             while (g.next(j, h0, h1)) {
                 const int end = min(h1 * MS_HALF, rows);
                 const int key = j * MS_TILE + (int)rank * 128 + L, node = key - g.len;
-                const bool tail = j * MS_TILE + (int)rank * 128 + 127 >= g.len;
+                const bool tail = j * MS_TILE + (int)rank * 128 + 127 >= g.len, careful = tail || Hp != p.H;
                 uint64_t seen = node < 0 ? ~0ull : 0;         // the tokens that see this key (read where `tail`)
                 if (node >= 0 && node < 64)
                     for (int a = 0; a < B.n_act; ++a) seen |= ((see[a] >> node) & 1) << a;
@@ -281,14 +281,22 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
                         tmem_ld32(tmem + lane_base + buf * 256 + c0, s);
                         tmem_wait_ld();
                         const float4* c4 = (const float4*)(col + buf * MS_ROWS + c0);
-                        if (tail) {                               // eight columns are heads of one token
+                        if (careful) {
+                            // a term that does not count is taken out by its exponent and not by its score or its c: a token's lse may
+                            // be NaN, and the zeros of padded heads times an infinite key are
                             const uint8_t* tk = tok + buf * MS_ROWS + c0;
                             #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                const bool sees = (seen >> tk[i]) & 1;
+                            for (int i = 0; i < 8; ++i) {
+                                const bool sees = !tail | ((seen >> tk[i / 2 * 8]) & 1);       // eight columns are heads of one token
+                                const float4 v = c4[i];
+                                const float c[4] = { v.x, v.y, v.z, v.w };
                                 #pragma unroll
-                                for (int x = i; x < i + 8; ++x) s[x] = sees ? s[x] : 0xff800000u;
+                                for (int x = 0; x < 4; ++x) {
+                                    const float e = fmaf(__uint_as_float(s[4 * i + x]), scale2, -c[x]);
+                                    acc[x] += exp2_approx(sees & (c[x] != INFINITY) ? e : -INFINITY);
+                                }
                             }
+                            continue;
                         }
                         #pragma unroll
                         for (int i = 0; i < 8; ++i) {

@@ -131,3 +131,45 @@ def test_a_seen_nan_reaches_every_output(A, ctx, n):
     out, lse = ctx.tree(q.cuda(), pg.cache(A), pg.starts, R.to_words([1, 3], "cuda"), SCALE)
     ctx.device_error()
     assert lse.isnan().all() and out.isnan().all()
+
+
+@pytest.mark.parametrize("H", [1, 20, 24, 128])
+def test_mass_of_rows_that_a_nan_token_does_not_see(A, ctx, H):
+    """A token that sees a NaN row has lse NaN, and so the rows that it sees have a NaN mass; drafted rows that it does not see
+    keep the sum over the tokens that do."""
+    pg = R.Paged([130], [3], 64, torch.bfloat16, "cuda", seed=4)
+    pg.set_row(0, 131, float("nan"))
+    q, masks = torch.randn(3, H, R.ROW, generator=torch.Generator().manual_seed(2)).bfloat16(), [0b001, 0b011, 0b101]
+    words = R.to_words(masks, "cuda")
+    m0 = torch.rand(pg.n_slots, generator=torch.Generator().manual_seed(3))
+    m = m0.cuda()
+    cache = pg.cache(A, mass=m)
+    _, lse = ctx.tree(q.cuda(), cache, pg.starts, words, SCALE)
+    assert lse[1].isnan().all() and not lse[0].isnan().any() and not lse[2].isnan().any()
+    ctx.mass(q.cuda(), lse, cache, pg.starts, words, SCALE, decay=0.5)
+    at = pg.slots[0]
+    want, tol = R.mass(pg, q, lse.cpu(), masks, SCALE, torch.ones(3), 0.5, m0)
+    got = m.cpu().double()
+    assert got[at[:132]].isnan().all()                                   # the context, and drafted rows 0 and 1, which token 1 sees
+    assert abs(got[at[132]] - want[at[132]]) <= tol[at[132]]
+
+
+@pytest.mark.parametrize("H", [1, 20, 24, 128])
+def test_mass_of_an_infinite_row(A, ctx, H):
+    """A row whose scores are all -infinity gets no weight, whatever the number of heads."""
+    pg = R.Paged([300], [2], 64, torch.bfloat16, "cuda", seed=5)
+    q = torch.randn(2, H, R.ROW, generator=torch.Generator().manual_seed(2)).bfloat16()
+    q[:, :, 7] = q[:, :, 7].abs() + 0.5
+    row = pg.seq[0][40].clone()
+    row[7] = -math.inf
+    pg.set_row(0, 40, row)
+    words = R.to_words([1, 3], "cuda")
+    m0 = torch.rand(pg.n_slots, generator=torch.Generator().manual_seed(3))
+    m = m0.cuda()
+    cache = pg.cache(A, mass=m)
+    _, lse = ctx.tree(q.cuda(), cache, pg.starts, words, SCALE)
+    assert torch.isfinite(lse).all()
+    ctx.mass(q.cuda(), lse, cache, pg.starts, words, SCALE, decay=0.5)
+    at = pg.slots[0]
+    assert float(m[at[40]]) == 0.5 * float(m0[at[40]])
+    assert torch.isfinite(m[at.cuda()]).all()
