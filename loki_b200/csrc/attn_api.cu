@@ -138,11 +138,14 @@ void lk_attn_destroy(LkAttnCtx* c) {
 int lk_attn_get_error(LkAttnCtx* c, lk_stream_t stream) {
     if (!c) return LK_ERR_ARG;
     OnDevice on(c->device);
-    LK_CU(cudaStreamSynchronize((cudaStream_t)stream));
+    // all of it in the stream's own order: the default stream would wait for others, and its memset could run behind a later call
+    const cudaStream_t st = (cudaStream_t)stream;
     int e = 0;
-    LK_CU(cudaMemcpy(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost));
+    LK_CU(cudaMemcpyAsync(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost, st));
+    LK_CU(cudaStreamSynchronize(st));
     if (!e) return LK_OK;
-    LK_CU(cudaMemset(c->err, 0, sizeof(int)));
+    LK_CU(cudaMemsetAsync(c->err, 0, sizeof(int), st));
+    LK_CU(cudaStreamSynchronize(st));
     const char* what = e == ATT_ERR_PAGE ? "a page id outside the pool" : e == ATT_ERR_POS ? "a position outside the rope table"
                      : e == ATT_ERR_LEN ? "a length outside its pages" : e == ATT_ERR_TREE ? "token ranges out of order or too long"
                      : "a bounded wait ran out";

@@ -173,3 +173,27 @@ def test_mass_of_an_infinite_row(A, ctx, H):
     at = pg.slots[0]
     assert float(m[at[40]]) == 0.5 * float(m0[at[40]])
     assert torch.isfinite(m[at.cuda()]).all()
+
+
+def test_device_error_waits_for_its_stream_alone(A, ctx, native):
+    """device_error(stream) reads and clears the word in the order of that stream; work on another one is not waited for."""
+    s = torch.cuda.Stream()
+    bad = torch.tensor([16], dtype=torch.int32, device="cuda")
+    x, table = torch.zeros(1, 1, 64, device="cuda"), A.RopeTable(16, 64, device="cuda")
+    out = torch.empty_like(x)
+
+    def refused():
+        ctx.rope(x, bad, table, out=out, stream=s)
+        with pytest.raises(native.NativeError):
+            ctx.device_error(s)
+        ctx.device_error(s)
+    torch.cuda.synchronize()
+    refused()                                                            # what is loaded on first use is there
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_000_000_000)                                     # half a second on the default stream
+    busy = torch.cuda.Event()
+    busy.record()
+    for _ in range(20):
+        refused()
+    assert not busy.query()
+    torch.cuda.synchronize()
