@@ -23,8 +23,12 @@ static int set_err(LkAttnCtx* c, int code, const char* fmt, ...) {
     if (c) { va_list ap; va_start(ap, fmt); vsnprintf(c->msg, sizeof(c->msg), fmt, ap); va_end(ap); }
     return code;
 }
-#define LK_CU(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) \
-    return set_err(c, LK_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); } while (0)
+// a failed call is reported once: the runtime's last error would come out again of the next launch that asks for it
+static int cuda_err(LkAttnCtx* c, const char* call, cudaError_t e) {
+    cudaGetLastError();
+    return set_err(c, LK_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
+}
+#define LK_CU(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) return cuda_err(c, #call, e_); } while (0)
 
 namespace {
 // the context's device for the length of a call; the caller's is put back
@@ -121,7 +125,7 @@ int lk_attn_create(const LkAttnConfig* cfg, int device, LkAttnCtx** out) {
     if (e == cudaSuccess) e = evict_setup();
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     cudaSetDevice(prev);
-    if (e != cudaSuccess) { lk_attn_destroy(c); return LK_ERR_CUDA; }
+    if (e != cudaSuccess) { lk_attn_destroy(c); cudaGetLastError(); return LK_ERR_CUDA; }
     *out = c;
     return LK_OK;
 }

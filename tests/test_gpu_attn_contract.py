@@ -197,3 +197,13 @@ def test_device_error_waits_for_its_stream_alone(A, ctx, native):
         refused()
     assert not busy.query()
     torch.cuda.synchronize()
+
+
+def test_a_failed_call_leaves_no_error_for_the_next(A, native):
+    """A context for a device that is not there is refused, and that alone: the next call does not report it again."""
+    with pytest.raises(native.NativeError):
+        A.AttnContext(99)
+    A.RopeTable(16, 64, device="cuda")
+    c = A.AttnContext(0, 1, 1)
+    c.device_error()
+    c.close()
