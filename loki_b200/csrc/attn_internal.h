@@ -99,7 +99,7 @@ __device__ __forceinline__ int kv_len(const KvView& kv, int b, int* err) {
 // pool row of row i of sequence b; -1 (recorded) where its page id is not one of the pool's
 __device__ __forceinline__ int kv_slot(const KvView& kv, int b, int i, int* err) {
     const int pi = i >> kv.page_shift;
-    if (pi >= kv.table_stride) { att_error(err, ATT_ERR_LEN); return -1; }
+    if ((unsigned)pi >= (unsigned)kv.table_stride) { att_error(err, ATT_ERR_LEN); return -1; }
     const int page = kv.block_table[(int64_t)b * kv.table_stride + pi];
     if ((unsigned)page >= (unsigned)kv.n_pages) { att_error(err, ATT_ERR_PAGE); return -1; }
     return (page << kv.page_shift) + (i & (kv.page_size - 1));

@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p) {
     }
     const int i = t - p.starts[b];
     if (i < 0 || t >= p.starts[b + 1]) { if (u == 0) att_error(p.err, ATT_ERR_TREE); return; }
-    const int slot = kv_slot(p.kv, b, kv_len(p.kv, b, p.err) + i, p.err);
+    // a row beyond 2^31 wraps to a negative one, which no page holds
+    const int slot = kv_slot(p.kv, b, (int)((unsigned)kv_len(p.kv, b, p.err) + (unsigned)i), p.err);
     if (slot < 0) return;
     TO* row = (TO*)p.kv.rows + (int64_t)slot * p.kv.row_stride;
     float v[8];

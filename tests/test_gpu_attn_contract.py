@@ -207,3 +207,24 @@ def test_a_failed_call_leaves_no_error_for_the_next(A, native):
     c = A.AttnContext(0, 1, 1)
     c.device_error()
     c.close()
+
+
+def test_append_behind_the_longest_table(A, ctx, native):
+    """Rows that would come after 2^31 - 257 of context, the most that a table can hold, are refused like any beyond the pages."""
+    page, pages = 256, 0x7fffff00 // 256
+    rows = torch.zeros(2 * page, R.ROW, dtype=torch.bfloat16, device="cuda")
+    lens = torch.tensor([page * pages], dtype=torch.int32, device="cuda")
+    cache = A.KvCache(rows, page, torch.zeros(1, pages, dtype=torch.int32, device="cuda"), lens)
+    T = 600                                                              # from the 257th on the row number passes 2^31
+    starts, pos = torch.tensor([0, T], dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    table = A.RopeTable(16, 64, device="cuda")
+    ctx.append(cache, torch.ones(T, 512, dtype=torch.bfloat16, device="cuda"), torch.ones(T, 64, dtype=torch.bfloat16, device="cuda"), starts, pos, table)
+    with pytest.raises(native.NativeError, match="length"):
+        ctx.device_error()
+    assert (rows == 0).all()
+    cache.lens.fill_(page + 3)                                           # and the same table with rows that it holds
+    cache.block_table[0, 1] = 1
+    ctx.append(cache, torch.ones(4, 512, dtype=torch.bfloat16, device="cuda"), torch.ones(4, 64, dtype=torch.bfloat16, device="cuda"),
+               torch.tensor([0, 4], dtype=torch.int32, device="cuda"), pos[:4], table)
+    ctx.device_error()
+    assert (rows[page + 3:page + 7] == 1).all() and (rows[:page + 3] == 0).all() and (rows[page + 7:] == 0).all()
