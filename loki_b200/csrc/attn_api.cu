@@ -180,7 +180,8 @@ int lk_attn_rope(LkAttnCtx* c, int dtype, const void* x, int64_t x_token, int64_
     const int es = dtype == LK_DT_F32 ? 4 : 2;
     if (!x || !y || !pos || !table || ((uintptr_t)x | (uintptr_t)y) % es || ((uintptr_t)table & 7)) return set_err(c, LK_ERR_ARG, "null or misaligned pointer");
     if (x == y && (x_token != y_token || x_head != y_head)) return set_err(c, LK_ERR_ARG, "in place needs equal strides");
-    if ((int64_t)T * (((int64_t)H * head_dim + 31) / 32) > 0x7fffffff) return set_err(c, LK_ERR_CAPACITY, "T %d x H %d x %d", T, H, head_dim);
+    // a token's units are counted in 32 bits, as are the blocks
+    if ((int64_t)H * head_dim > (1 << 30) || (int64_t)T * (((int64_t)H * head_dim + 31) / 32) > 0x7fffffff) return set_err(c, LK_ERR_CAPACITY, "T %d x H %d x %d", T, H, head_dim);
     OnDevice on(c->device);
     RopeParams p{ x, x_token, x_head, y, y_token, y_head, T, H, head_dim, rot_offset, rot_dim, grad != 0, x != y, pos, (const float2*)table, max_pos, c->err };
     LK_CU(launch_rope(p, dtype, layout, (cudaStream_t)stream));

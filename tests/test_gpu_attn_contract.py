@@ -228,3 +228,11 @@ def test_append_behind_the_longest_table(A, ctx, native):
                torch.tensor([0, 4], dtype=torch.int32, device="cuda"), pos[:4], table)
     ctx.device_error()
     assert (rows[page + 3:page + 7] == 1).all() and (rows[:page + 3] == 0).all() and (rows[page + 7:] == 0).all()
+
+
+def test_rope_of_more_than_2_30_values_a_token_is_refused(A, ctx, native):
+    """Heads that a stride of 0 repeats need no memory, and 65 536 of 40 000 values are more than the kernel counts."""
+    x = torch.zeros(1, 1, 40000, dtype=torch.bfloat16, device="cuda").expand(1, 65536, 40000)
+    out, pos = torch.zeros(1, 1, 40000, dtype=torch.bfloat16, device="cuda").expand(1, 65536, 40000), torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(native.NativeError, match="40000"):
+        ctx.rope(x, pos, A.RopeTable(16, 64, device="cuda"), out=out)
