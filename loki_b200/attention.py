@@ -3,7 +3,8 @@ cache, attention of drafted token trees over it, the attention weight of each ca
 
 The cache holds the row that the reference's attention keeps (latent 512, rotated key part 64; src/fused_layer.cu:277-308);
 torch supplies device memory and streams, every computation runs in libloki_moe.so.  Calls are queued on the current
-stream (or `stream`) and do not synchronise; AttnContext.device_error() reports what a kernel refused.
+stream (or `stream`, whose pool then holds what the call returns) and do not synchronise; AttnContext.device_error()
+reports what a kernel refused.
 """
 import ctypes
 
@@ -54,9 +55,9 @@ class RopeTable:
         device = torch.device(device)
         self.device = torch.cuda.current_device() if device.index is None else device.index
         self.max_pos, self.rot_dim = max_pos, rot_dim
-        self.table = torch.empty(max(max_pos, 0), max(rot_dim, 0) // 2, 2, device="cuda:%d" % self.device)
         cfg = N.LkRopeConfig(rot_dim, base, factor, orig_ctx, beta_fast, beta_slow, mscale)
-        with torch.cuda.device(self.device):
+        with torch.cuda.device(self.device), torch.cuda.stream(stream):
+            self.table = torch.empty(max(max_pos, 0), max(rot_dim, 0) // 2, 2, device="cuda:%d" % self.device)
             check(lib().lk_attn_rope_table(None, ctypes.byref(cfg), max_pos, self.table.data_ptr(), _queue(stream, self.device)))
         self.address = self.table.data_ptr()
 
@@ -122,6 +123,9 @@ class AttnContext:
     def rope(self, x, pos, table, rot_offset=0, layout="interleaved", grad=False, out=None, stream=None):
         """x [T][H][head_dim] with [rot_offset, rot_offset + table.rot_dim) of each head rotated to pos [T]; grad: the
         transpose (x is the gradient of the rotated heads, the result that of the plain ones).  out=x works in place."""
+        if stream is not None:                           # memory of that stream's pool: another's may be in use until its queue ends
+            with torch.cuda.stream(stream):
+                return self.rope(x, pos, table, rot_offset, layout, grad, out)
         dev = self.device
         at, st = _rows(x, "x", dev, None)
         _need(x.dim() == 3 and x.dtype in _DTYPE, "x: [T][H][head_dim], fp32, fp16 or bf16")
@@ -135,7 +139,7 @@ class AttnContext:
             _need(out.shape == x.shape and out.dtype is x.dtype, "out: x's shape and dtype")
         rc = self._lib.lk_attn_rope(self.ctx, _DTYPE[x.dtype], at, st[0], st[1], to, so[0], so[1], T, H, D, rot_offset, table.rot_dim,
                                     _LAYOUT[layout], grad, _dense(pos, "pos", _I32, dev, T), table.address, table.max_pos,
-                                    _queue(stream, dev))
+                                    _queue(None, dev))
         if rc:
             self._check(rc)
         return out
@@ -166,6 +170,9 @@ class AttnContext:
     def tree(self, q, cache, starts, tree, scale, out=None, lse=None, stream=None):
         """out [T][H][512], lse [T][H]: the drafted tokens' attention over their sequence's context and over drafted row j
         where bit j of tree [T] (64-bit words) is set.  tree None: a chain (each token sees the drafts up to itself)."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.tree(q, cache, starts, tree, scale, out, lse)
         at, st, starts_at, tree_at = self._query(q, cache, starts, tree)
         T, H, _ = q.shape
         if out is None:
@@ -180,7 +187,7 @@ class AttnContext:
         else:
             lse_at = _dense(lse, "lse", _F32, self.device, T, H)
         rc = self._lib.lk_attn_tree(self.ctx, cache._ref, at, st[0], st[1], T, H, starts_at, tree_at, scale, to, so[0], so[1],
-                                    lse_at, _queue(stream, self.device))
+                                    lse_at, _queue(None, self.device))
         if rc:
             self._check(rc)
         return out, lse
@@ -199,9 +206,12 @@ class AttnContext:
         """Cut every sequence to its `budget` best rows (position < sinks or >= next_pos - recent first, then the largest
         mass, then row order); kept rows beyond the budget fill the holes before it.  Returns new_lens [n_seqs], which may
         be cache.lens itself."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.evict(cache, budget, next_pos, sinks, recent, new_lens)
         if new_lens is None:
             new_lens = next_pos.new_empty((cache.n_seqs,))
         self._check(self._lib.lk_attn_evict(self.ctx, cache._ref, budget, sinks, recent,
                                             _dense(next_pos, "next_pos", _I32, self.device, cache.n_seqs),
-                                            _dense(new_lens, "new_lens", _I32, self.device, cache.n_seqs), _queue(stream, self.device)))
+                                            _dense(new_lens, "new_lens", _I32, self.device, cache.n_seqs), _queue(None, self.device)))
         return new_lens

@@ -236,3 +236,63 @@ def test_rope_of_more_than_2_30_values_a_token_is_refused(A, ctx, native):
     out, pos = torch.zeros(1, 1, 40000, dtype=torch.bfloat16, device="cuda").expand(1, 65536, 40000), torch.zeros(1, dtype=torch.int32, device="cuda")
     with pytest.raises(native.NativeError, match="40000"):
         ctx.rope(x, pos, A.RopeTable(16, 64, device="cuda"), out=out)
+
+
+def _behind(make, value=7):
+    """Memory of `make` given back while the current stream still has a write to it in its queue."""
+    t = make()
+    torch.cuda._sleep(200_000_000)                                       # a tenth of a second
+    t.fill_(value)
+    del t
+
+
+def test_results_on_another_stream_have_memory_of_their_own(A, ctx):
+    """With stream=, what a call returns is not memory that the current stream still writes to, nor given to it while the call
+    runs: rope, a rope table, tree and evict against the same calls on the current stream."""
+    pg = R.Paged([200, 90], [3, 1], 64, torch.bfloat16, "cuda", seed=6)
+    q, words = torch.randn(4, 8, R.ROW, generator=torch.Generator().manual_seed(1)).bfloat16().cuda(), R.to_words([1, 3, 5, 1], "cuda")
+    x, pos, table = q.clone(), torch.arange(4, dtype=torch.int32, device="cuda"), A.RopeTable(300, 64, device="cuda")
+    mass, place = torch.rand(pg.n_slots, device="cuda"), torch.arange(pg.n_slots, dtype=torch.int32, device="cuda")
+    cache, nxt = pg.cache(A, mass=mass, pos=place), torch.tensor([1 << 20, 1 << 20], dtype=torch.int32, device="cuda")
+    state = [t.clone() for t in (pg.rows, mass, place)]
+
+    def calls(stream):
+        yield lambda: (ctx.rope(x, pos, table, rot_offset=512, stream=stream),)
+        yield lambda: (A.RopeTable(300, 64, device="cuda", stream=stream).table,)
+        yield lambda: ctx.tree(q, cache, pg.starts, words, SCALE, stream=stream)
+        yield lambda: (ctx.evict(cache, 100, nxt, stream=stream), pg.rows, mass, place)
+
+    def again():
+        for t, v in zip((pg.rows, mass, place), state):
+            t.copy_(v)
+        torch.cuda.synchronize()
+    want = []
+    for call in calls(None):
+        again()
+        want.append([t.clone() for t in call()])
+    s = torch.cuda.Stream()
+    for k, call in enumerate(calls(s)):
+        again()
+        call()                                                           # the stream's pool has seen such a call
+        again()
+        shapes = [(t.shape, t.dtype) for t in want[k]]
+        for shape, dt in shapes:
+            _behind(lambda: torch.empty(shape, dtype=dt, device="cuda"))
+        got = call()
+        torch.cuda.synchronize()
+        for g, w in zip(got, want[k]):
+            assert torch.equal(g.view(torch.uint8), w.view(torch.uint8))
+    ctx.device_error()
+
+
+def test_a_dropped_result_is_not_given_away_while_its_call_runs(A, ctx):
+    """The result of a call on `stream`, dropped at once, does not become a tensor of the current stream under the call."""
+    x, pos, table = torch.randn(8, 16, 64, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda"), A.RopeTable(4, 64, device="cuda")
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)
+    ctx.rope(x, pos, table, stream=s)                                    # its kernel comes after the sleep
+    mine = [torch.full_like(x, 3.0) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert all((m == 3.0).all() for m in mine)
