@@ -41,8 +41,21 @@ def _rows(t, name, device, last):
     return t.data_ptr(), st
 
 
+def _elsewhere(name, x, device):
+    raise ValueError("%s: on cuda:%d, the context on cuda:%d" % (name, x.device, device))
+
+
+def _on(stream, device):
+    """`stream` as the current one: what the call makes comes from its pool (another's memory may be in use until its queue ends)."""
+    _need(stream.device.index == device, "stream: one of cuda:%d", device)
+    return torch.cuda.stream(stream)
+
+
 def _queue(stream, device):
-    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device)
+    _need(stream.device.index == device, "stream: one of cuda:%d", device)
+    return stream.cuda_stream
 
 
 class RopeTable:
@@ -56,9 +69,9 @@ class RopeTable:
         self.device = torch.cuda.current_device() if device.index is None else device.index
         self.max_pos, self.rot_dim = max_pos, rot_dim
         cfg = N.LkRopeConfig(rot_dim, base, factor, orig_ctx, beta_fast, beta_slow, mscale)
-        with torch.cuda.device(self.device), torch.cuda.stream(stream):
+        with torch.cuda.device(self.device), torch.cuda.stream(None) if stream is None else _on(stream, self.device):
             self.table = torch.empty(max(max_pos, 0), max(rot_dim, 0) // 2, 2, device="cuda:%d" % self.device)
-            check(lib().lk_attn_rope_table(None, ctypes.byref(cfg), max_pos, self.table.data_ptr(), _queue(stream, self.device)))
+            check(lib().lk_attn_rope_table(None, ctypes.byref(cfg), max_pos, self.table.data_ptr(), _queue(None, self.device)))
         self.address = self.table.data_ptr()
 
 
@@ -123,10 +136,12 @@ class AttnContext:
     def rope(self, x, pos, table, rot_offset=0, layout="interleaved", grad=False, out=None, stream=None):
         """x [T][H][head_dim] with [rot_offset, rot_offset + table.rot_dim) of each head rotated to pos [T]; grad: the
         transpose (x is the gradient of the rotated heads, the result that of the plain ones).  out=x works in place."""
-        if stream is not None:                           # memory of that stream's pool: another's may be in use until its queue ends
-            with torch.cuda.stream(stream):
-                return self.rope(x, pos, table, rot_offset, layout, grad, out)
         dev = self.device
+        if stream is not None:
+            with _on(stream, dev):
+                return self.rope(x, pos, table, rot_offset, layout, grad, out)
+        if table.device != dev:
+            _elsewhere("table", table, dev)
         at, st = _rows(x, "x", dev, None)
         _need(x.dim() == 3 and x.dtype in _DTYPE, "x: [T][H][head_dim], fp32, fp16 or bf16")
         _need(layout in _LAYOUT, "layout: interleaved or half")
@@ -148,6 +163,10 @@ class AttnContext:
         """Tokens starts[b] .. starts[b+1]-1 of latent [T][512] and k_rope [T][64] (not yet rotated) become the rows after
         sequence b's lens[b]; cache.pos gets pos [T], cache.mass zeros.  lens stays as it is."""
         dev = self.device
+        if cache.device != dev:
+            _elsewhere("cache", cache, dev)
+        if table.device != dev:
+            _elsewhere("table", table, dev)
         at, st = _rows(latent, "latent", dev, ATTN_LATENT)
         kt, ks = _rows(k_rope, "k_rope", dev, ATTN_ROPE)
         _need(latent.dim() == 2 and k_rope.dim() == 2 and k_rope.shape[0] == latent.shape[0] and latent.dtype is k_rope.dtype and
@@ -160,6 +179,8 @@ class AttnContext:
                                              table.address, table.max_pos, _LAYOUT[layout], _queue(stream, dev)))
 
     def _query(self, q, cache, starts, tree):
+        if cache.device != self.device:
+            _elsewhere("cache", cache, self.device)
         at, st = _rows(q, "q", self.device, ATTN_ROW)
         _need(q.dim() == 3 and q.dtype is cache.dtype, "q: [T][H][576] of the cache's dtype")
         tree_at = None
@@ -171,7 +192,7 @@ class AttnContext:
         """out [T][H][512], lse [T][H]: the drafted tokens' attention over their sequence's context and over drafted row j
         where bit j of tree [T] (64-bit words) is set.  tree None: a chain (each token sees the drafts up to itself)."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with _on(stream, self.device):
                 return self.tree(q, cache, starts, tree, scale, out, lse)
         at, st, starts_at, tree_at = self._query(q, cache, starts, tree)
         T, H, _ = q.shape
@@ -207,8 +228,10 @@ class AttnContext:
         mass, then row order); kept rows beyond the budget fill the holes before it.  Returns new_lens [n_seqs], which may
         be cache.lens itself."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with _on(stream, self.device):
                 return self.evict(cache, budget, next_pos, sinks, recent, new_lens)
+        if cache.device != self.device:
+            _elsewhere("cache", cache, self.device)
         if new_lens is None:
             new_lens = next_pos.new_empty((cache.n_seqs,))
         self._check(self._lib.lk_attn_evict(self.ctx, cache._ref, budget, sinks, recent,
