@@ -36,7 +36,9 @@ def tree_words(parents):
 class DraftSession:
     """The paged latent cache of n_seqs sequences with everything its decode loop needs.  budget: rows that a sequence keeps
     after each accept() (None: all); sinks first positions and the `recent` last ones are always kept.  rope: a RopeTable
-    (default: unstretched, base 10000, max_positions of them, 2 max_len unless given)."""
+    (default: unstretched, base 10000, max_positions of them, 2 max_len unless given).  Positions grow with every accepted token,
+    evicted or not, so max_positions bounds the whole text; a step that would pass it, or the pages, is refused before it starts.
+    lens and next_pos are the session's to change: it keeps their values on the host too."""
 
     def __init__(self, n_seqs, heads, max_len, budget=None, sinks=4, recent=64, decay=1.0, dtype=torch.bfloat16, page=64,
                  scale=192 ** -0.5, rope=None, max_positions=None, layout="interleaved", device=0):
@@ -51,6 +53,7 @@ class DraftSession:
         self.cache = A.KvCache(new(n_seqs * per * page, ATTN_ROW, dt=dtype), page,
                                torch.arange(n_seqs * per, dtype=torch.int32, device=self.device).view(n_seqs, per), self.lens,
                                mass=new(n_seqs * per * page, dt=torch.float32), pos=new(n_seqs * per * page))
+        self._room, self._lens, self._next = per * page, [0] * n_seqs, [0] * n_seqs
         self._pending = None
 
     def slots(self, seq, index):
@@ -63,31 +66,52 @@ class DraftSession:
         counts = torch.as_tensor(counts, dtype=torch.int64)
         if len(counts) != self.n_seqs or bool((counts < 0).any()):
             raise ValueError("counts: one per sequence")
+        counts = counts.cpu()
         starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
         seq = torch.repeat_interleave(torch.arange(self.n_seqs), counts)
         at = torch.arange(int(starts[-1])) - starts[seq]
         return starts.int().to(self.device), seq.to(self.device), at.to(self.device)
 
+    def _fit(self, rows, positions):
+        """Refuses rows[b] more rows or positions[b] more positions of sequence b than there is room for."""
+        for b, (n, p) in enumerate(zip(rows, positions)):
+            if self._lens[b] + n > self._room:
+                raise ValueError("sequence %d: %d rows and %d more, its pages hold %d" % (b, self._lens[b], n, self._room))
+            if self._next[b] + p > self.rope.max_pos:
+                raise ValueError("sequence %d: %d positions and %d more, the rope table has %d" % (b, self._next[b], p, self.rope.max_pos))
+
+    def _grow(self, rows, keep=None):
+        """What the device's lens and next_pos become: rows[b] more, then at most `keep`."""
+        for b, n in enumerate(rows):
+            self._next[b] += n
+            self._lens[b] = self._lens[b] + n if keep is None else min(self._lens[b] + n, keep)
+
     def prefill(self, latent, k_rope, counts):
         """Append the prompts' rows: counts[b] tokens of sequence b, one sequence after another."""
         starts, seq, at = self._tokens(counts)
+        rows = torch.as_tensor(counts).tolist()
+        self._fit(rows, rows)
         self.ctx.append(self.cache, latent, k_rope, starts, (self.next_pos[seq] + at).int(), self.rope, layout=self.layout)
         n = starts.diff()
         self.lens += n
         self.next_pos += n
+        self._grow(rows)
 
     def verify(self, q, latent, k_rope, parents):
         """Attention of the drafted trees: q [T][heads][576] (its last 64 values not yet rotated; rotated in place), latent and
         k_rope the nodes' rows, parents[b] the tree of sequence b.  A node's position is its depth below the context.
         Returns out [T][heads][512] and lse [T][heads]; accept() follows."""
+        words = tree_words(parents)
         starts, seq, _ = self._tokens([len(p) for p in parents])
-        depths = []
+        depths, reach = [], []
         for p in parents:
             d = []
             for j, a in enumerate(p):
                 d.append(0 if a < 0 else d[a] + 1)
             depths += d
-        words = torch.tensor(tree_words(parents), dtype=torch.int64).to(self.device)
+            reach.append(max(d, default=-1) + 1)
+        self._fit([len(p) for p in parents], reach)
+        words = torch.tensor(words, dtype=torch.int64).to(self.device)
         pos = (self.next_pos[seq] + torch.tensor(depths, dtype=torch.int64).to(self.device)).int()
         self.ctx.rope(q, pos, self.rope, rot_offset=ATTN_LATENT, layout=self.layout, out=q)
         self.ctx.append(self.cache, latent, k_rope, starts, pos, self.rope, layout=self.layout)
@@ -121,6 +145,7 @@ class DraftSession:
         n = torch.tensor([len(p) for p in paths], dtype=torch.int32).to(self.device)
         self.lens += n
         self.next_pos += n
+        self._grow([len(p) for p in paths], self.budget)
         if self.budget is not None:
             self.ctx.evict(self.cache, self.budget, self.next_pos, sinks=self.sinks, recent=self.recent, new_lens=self.lens)
 
