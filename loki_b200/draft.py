@@ -116,25 +116,30 @@ class DraftSession:
         self.ctx.rope(q, pos, self.rope, rot_offset=ATTN_LATENT, layout=self.layout, out=q)
         self.ctx.append(self.cache, latent, k_rope, starts, pos, self.rope, layout=self.layout)
         out, lse = self.ctx.tree(q, self.cache, starts, words, self.scale)
-        self._pending = (q, lse, starts, words, [len(p) for p in parents])
+        self._pending = (q, lse, starts, words, [list(p) for p in parents])
         return out, lse
 
     def accept(self, paths):
-        """Keep node paths[b] (ascending indices of the accepted branch) of sequence b's tree: their queries' weights go to the
-        rows they attended to, their rows follow the context, and sequences over budget are cut."""
-        q, lse, starts, words, sizes = self._pending
+        """Keep node paths[b] (the accepted branch, from a root of sequence b's tree down) of every sequence: their queries'
+        weights go to the rows they attended to, their rows follow the context, and sequences over budget are cut."""
+        if self._pending is None:
+            raise ValueError("accept() follows verify()")
+        q, lse, starts, words, parents = self._pending
+        if len(paths) != self.n_seqs:
+            raise ValueError("paths: one per sequence")
+        for b, (path, tree) in enumerate(zip(paths, parents)):
+            if any(not 0 <= j < len(tree) for j in path) or any(tree[j] != a for j, a in zip(path, [-1, *path])):
+                raise ValueError("paths[%d]: each node's parent comes before it, the first has none" % b)
         self._pending = None
-        first, w = 0, torch.zeros(sum(sizes))
+        first, w = 0, torch.zeros(sum(len(tree) for tree in parents))
         src_seq, src_at, dst_at = [], [], []
-        for b, (path, n) in enumerate(zip(paths, sizes)):
-            if any(not 0 <= j < n for j in path) or any(a >= c for a, c in zip(path, path[1:])):
-                raise ValueError("paths[%d]: ascending nodes of its tree" % b)
+        for b, (path, tree) in enumerate(zip(paths, parents)):
             for k, j in enumerate(path):
                 w[first + j] = 1.0
                 src_seq.append(b)
                 src_at.append(j)
                 dst_at.append(k)
-            first += n
+            first += len(tree)
         self.ctx.mass(q, lse, self.cache, starts, words, self.scale, weight=w.to(self.device), decay=self.decay)
         seq = torch.tensor(src_seq, dtype=torch.int64, device=self.device)
         base = self.lens[seq].long()

@@ -102,3 +102,23 @@ def test_a_budget_makes_room(session):
     _verify(s, [list(range(-1, 27)), [-1]])
     s.accept([list(range(28)), [0]])
     assert s.lens.tolist() == [100, 3] and s.next_pos.tolist() == [156, 3]
+
+
+def test_paths_that_are_no_branches_are_refused(session):
+    """A refused accept() changes nothing, and the verified trees can still be accepted."""
+    s = session(budget=None)
+    _prefill(s, [3, 5])
+    with pytest.raises(ValueError, match="verify"):
+        s.accept([[], []])
+    _verify(s, [[-1, 0, 0, 2], [-1, -1]])
+    s.cache.rows[:, 0] = torch.arange(s.cache.rows.shape[0])
+    rows, mass = s.cache.rows.clone(), s.cache.mass.clone()
+    for paths in ([[0, 2]], [[0, 2], [], []], [[0, 3], []], [[2, 3], []], [[0, 1, 2], []], [[2, 0], []], [[0, 0], []], [[0], [0, 1]], [[4], []], [[-1], []]):
+        _kept(s, lambda: s.accept(paths), "paths")
+        assert torch.equal(s.cache.rows, rows) and torch.equal(s.cache.mass, mass)
+    s.accept([[0, 2, 3], [1]])
+    assert s.lens.tolist() == [6, 6] and s.next_pos.tolist() == [6, 6]
+    at = s.slots(torch.tensor([0, 0, 0, 1]), torch.tensor([3, 4, 5, 5]))
+    assert s.cache.rows[at, 0].tolist() == [rows[i, 0].item() for i in s.slots(torch.tensor([0, 0, 0, 1]), torch.tensor([3, 5, 6, 6]))]
+    with pytest.raises(ValueError, match="verify"):
+        s.accept([[], []])
