@@ -87,11 +87,13 @@ class DraftSession:
             self._lens[b] = self._lens[b] + n if keep is None else min(self._lens[b] + n, keep)
 
     def prefill(self, latent, k_rope, counts):
-        """Append the prompts' rows: counts[b] tokens of sequence b, one sequence after another."""
+        """Append the prompts' rows: counts[b] tokens of sequence b, one sequence after another.  Verified trees that were not
+        accepted are dropped: the rows take their place."""
         starts, seq, at = self._tokens(counts)
         rows = torch.as_tensor(counts).tolist()
         self._fit(rows, rows)
         self.ctx.append(self.cache, latent, k_rope, starts, (self.next_pos[seq] + at).int(), self.rope, layout=self.layout)
+        self._pending = None
         n = starts.diff()
         self.lens += n
         self.next_pos += n
@@ -111,10 +113,13 @@ class DraftSession:
             depths += d
             reach.append(max(d, default=-1) + 1)
         self._fit([len(p) for p in parents], reach)
+        if q.dim() != 3 or q.shape[0] != len(words) or q.shape[2] != ATTN_ROW or q.dtype is not self.cache.rows.dtype:
+            raise ValueError("q: [%d][heads][%d] of the cache's dtype" % (len(words), ATTN_ROW))
         words = torch.tensor(words, dtype=torch.int64).to(self.device)
         pos = (self.next_pos[seq] + torch.tensor(depths, dtype=torch.int64).to(self.device)).int()
+        self.ctx.append(self.cache, latent, k_rope, starts, pos, self.rope, layout=self.layout)      # first: it may refuse its rows
+        self._pending = None
         self.ctx.rope(q, pos, self.rope, rot_offset=ATTN_LATENT, layout=self.layout, out=q)
-        self.ctx.append(self.cache, latent, k_rope, starts, pos, self.rope, layout=self.layout)
         out, lse = self.ctx.tree(q, self.cache, starts, words, self.scale)
         self._pending = (q, lse, starts, words, [list(p) for p in parents])
         return out, lse

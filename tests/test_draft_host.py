@@ -122,3 +122,29 @@ def test_paths_that_are_no_branches_are_refused(session):
     assert s.cache.rows[at, 0].tolist() == [rows[i, 0].item() for i in s.slots(torch.tensor([0, 0, 0, 1]), torch.tensor([3, 5, 6, 6]))]
     with pytest.raises(ValueError, match="verify"):
         s.accept([[], []])
+
+
+def test_a_refused_verify_leaves_its_query_unrotated(session):
+    """What does not fit the trees is refused before q is rotated in place."""
+    s = session()
+    _prefill(s, [3, 5])
+    good = dict(q=torch.zeros(3, 1, 576), latent=torch.zeros(3, 512), k_rope=torch.zeros(3, 64), parents=[[-1, 0], [-1]])
+    for bad in (dict(q=torch.zeros(2, 1, 576)), dict(q=torch.zeros(3, 1, 512)), dict(q=torch.zeros(3, 1, 576).half()), dict(q=torch.zeros(3, 576))):
+        _kept(s, lambda: s.verify(**{**good, **bad}), "q")
+
+    def refuse(*_, **__):
+        raise ValueError("latent")
+    s.ctx.append = refuse
+    _kept(s, lambda: s.verify(**good), "latent")
+    del s.ctx.append
+    s.verify(**good)
+    assert s.ctx.calls[-3:] == ["append", "rope", "tree"]
+
+
+def test_prompts_drop_the_trees_whose_place_they_take(session):
+    s = session()
+    _verify(s, [[-1, 0], [-1]])
+    _prefill(s, [3, 0])
+    with pytest.raises(ValueError, match="verify"):
+        s.accept([[0], [0]])
+    assert s.lens.tolist() == [3, 0]
