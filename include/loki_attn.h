@@ -107,7 +107,8 @@ LK_API int lk_attn_tree(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, i
 /* cache->mass[row k] = decay * mass + sum_t weight[t] * sum_h exp(scale * q . row_k - lse[t][h]) for every row of every
  * sequence (context and drafted), over the tokens that see it: the attention weight that lk_attn_tree gave it (sequences
  * without tokens keep theirs).  weight [T] (null: all 1; 0 for rejected drafts: only tokens of positive weight count).
- * Each row's terms are added in a fixed order, so results repeat. */
+ * Each row's terms are added in a fixed order, so results repeat.  q's strides must be positive here (heads or tokens that a
+ * stride of 0 repeats are refused; lk_attn_tree takes them). */
 LK_API int lk_attn_mass(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H,
                         const int* starts, const uint64_t* tree, float scale, const float* lse, const float* weight,
                         float decay, lk_stream_t stream);

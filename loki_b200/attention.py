@@ -215,7 +215,8 @@ class AttnContext:
 
     def mass(self, q, lse, cache, starts, tree, scale, weight=None, decay=1.0, stream=None):
         """cache.mass = decay * cache.mass + the attention weight that tree() gave each row, summed over heads and over the
-        tokens with their weight [T] (0 for rejected drafts; None: 1).  Sequences without tokens keep theirs."""
+        tokens with their weight [T] (0 for rejected drafts; None: 1).  Sequences without tokens keep theirs.  An expanded q
+        (a stride of 0), which tree() takes, is refused here."""
         at, st, starts_at, tree_at = self._query(q, cache, starts, tree)
         T, H, _ = q.shape
         self._check(self._lib.lk_attn_mass(self.ctx, cache._ref, at, st[0], st[1], T, H, starts_at, tree_at, scale,

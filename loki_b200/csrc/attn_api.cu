@@ -42,8 +42,9 @@ struct OnDevice {
 static bool is16(const void* p) { return p && !((uintptr_t)p & 15); }
 
 // rows of 64-value columns as a tensor map: dims[0] values of a row, the outer strides in elements, boxes of 64 values x `rows` of
-// the next dimension, 128-byte swizzle, zeros outside
-static int encode_map(LkAttnCtx* c, CUtensorMap* map, int dtype, const void* base, int rank, const int64_t* dims, const int64_t* strides, int rows) {
+// dimension `along`, 128-byte swizzle, zeros outside
+static int encode_map(LkAttnCtx* c, CUtensorMap* map, int dtype, const void* base, int rank, const int64_t* dims, const int64_t* strides, int rows,
+                      int along = 1) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static const Encode encode = [] {
@@ -56,7 +57,7 @@ static int encode_map(LkAttnCtx* c, CUtensorMap* map, int dtype, const void* bas
     cuuint64_t d[3], s[2];
     for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i];
     for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)strides[i] * 2;
-    const cuuint32_t box[3] = { 64, (cuuint32_t)rows, 1 }, step[3] = { 1, 1, 1 };
+    const cuuint32_t box[3] = { 64, along == 1 ? (cuuint32_t)rows : 1, along == 2 ? (cuuint32_t)rows : 1 }, step[3] = { 1, 1, 1 };
     const CUresult r = encode(map, dtype == LK_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s,
                               box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -266,10 +267,12 @@ int lk_attn_mass(LkAttnCtx* c, const LkKvCache* cache, const void* q, int64_t q_
     p.lse = const_cast<float*>(lse); p.weight = weight; p.decay = decay;
     CUtensorMap map, q_map;
     if (int rc = kv_map(c, cache, &map)) return rc;
-    // a dimension of one has no stride of its own
-    const int64_t dims[3] = { AT_ROW, H, T }, strides[2] = { H > 1 ? q_head : AT_ROW, T > 1 ? q_token : AT_ROW };
-    if (strides[0] <= 0 || strides[1] <= 0) return set_err(c, LK_ERR_UNSUPPORTED, "q strides must be positive");
-    if (int rc = encode_map(c, &q_map, cache->dtype, q, 3, dims, strides, mass_q_box(H))) return rc;
+    // dimensions from the smaller stride to the larger; one of a single entry has no stride of its own
+    const int64_t head = H > 1 ? q_head : AT_ROW, token = T > 1 ? q_token : head * H;
+    if (head <= 0 || token <= 0) return set_err(c, LK_ERR_UNSUPPORTED, "q strides (%lld, %lld) must be positive", (long long)q_token, (long long)q_head);
+    p.q_head_major = token < head;
+    const int64_t dims[3] = { AT_ROW, p.q_head_major ? T : H, p.q_head_major ? H : T }, strides[2] = { p.q_head_major ? token : head, p.q_head_major ? head : token };
+    if (int rc = encode_map(c, &q_map, cache->dtype, q, 3, dims, strides, mass_q_box(H), p.q_head_major ? 2 : 1)) return rc;
     LK_CU(launch_mass(p, cache->dtype, map, q_map, c->mass, c->nsm / 2, (cudaStream_t)stream));
     return LK_OK;
 }

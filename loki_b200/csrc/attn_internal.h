@@ -54,6 +54,7 @@ struct TreeParams {
     float* lse;                                    // tree: out; mass: in
     const float* weight; float decay;              // mass
     int q_flat;                                    // tree: q's rows (t, h) lie at equal distances
+    int q_head_major;                              // mass: the dimensions of q's tensor map are (576, T, H), else (576, H, T)
     int* err;
 };
 // parts of items that more than one pair of CTAs works on (attn_tree.cu)

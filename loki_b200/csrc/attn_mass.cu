@@ -224,24 +224,29 @@ k_mass(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap
             // ---------------------------------------------------------------- Q: this CTA's half of a block's rows, 64 values a stage
             if (rows && elect_one()) {
                 const uint32_t full0 = peer_addr(smem_u32(&B.q_full[0]), 0);
-                while (ok && g.next(j, h0, h1)) {
-                    const int end = min(h1 * MS_HALF, rows);
-                    for (int r1 = h0 * MS_HALF; ok && r1 < end; r1 += MS_ROWS) {
-                        const int half = mass_cols(end - r1, hb) / 2, r0 = r1 + (int)rank * half;
-                        const int a0 = r0 / Hp, hd0 = r0 - a0 * Hp;
-                        for (int c = 0; c < 9; ++c, ++n_q) {
-                            const uint32_t st = n_q % MS_RING, bar = full0 + 8 * st;
-                            if (!(ok = wait_phase(&B.q_empty[st], ((n_q / MS_RING) & 1) ^ 1, gave_up, p.err))) break;
-                            arrive_expect_at(bar, half * 128);
-                            uint32_t to = smb + MS_Q + st * MS_CHUNK;
-                            for (int r = 0, a = a0, h = hd0; r < half; r += hb, to += hb * 128) {
-                                // rows beyond the last token's: that token's again (their c is infinite)
-                                tma_3d_pair(to, &q_map, c * 64, h, g.first + act[min(a, rows / Hp - 1)], bar);
-                                if ((h += hb) == Hp) { h = 0; ++a; }
+                auto load = [&](auto head_major) {            // the order of the map's dimensions, settled outside the loops
+                    while (ok && g.next(j, h0, h1)) {
+                        const int end = min(h1 * MS_HALF, rows);
+                        for (int r1 = h0 * MS_HALF; ok && r1 < end; r1 += MS_ROWS) {
+                            const int half = mass_cols(end - r1, hb) / 2, r0 = r1 + (int)rank * half;
+                            const int a0 = r0 / Hp, hd0 = r0 - a0 * Hp;
+                            for (int c = 0; c < 9; ++c, ++n_q) {
+                                const uint32_t st = n_q % MS_RING, bar = full0 + 8 * st;
+                                if (!(ok = wait_phase(&B.q_empty[st], ((n_q / MS_RING) & 1) ^ 1, gave_up, p.err))) break;
+                                arrive_expect_at(bar, half * 128);
+                                uint32_t to = smb + MS_Q + st * MS_CHUNK;
+                                for (int r = 0, a = a0, h = hd0; r < half; r += hb, to += hb * 128) {
+                                    // rows beyond the last token's: that token's again (their c is infinite)
+                                    const int t = g.first + act[min(a, rows / Hp - 1)];
+                                    if (decltype(head_major)::value) tma_3d_pair(to, &q_map, c * 64, t, h, bar);
+                                    else tma_3d_pair(to, &q_map, c * 64, h, t, bar);
+                                    if ((h += hb) == Hp) { h = 0; ++a; }
+                                }
                             }
                         }
                     }
-                }
+                };
+                if (p.q_head_major) load(std::true_type()); else load(std::false_type());
                 if (!ok) __nanosleep(1000000);
             }
         } else if (warp >= 4) {

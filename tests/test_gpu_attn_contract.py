@@ -296,3 +296,45 @@ def test_a_dropped_result_is_not_given_away_while_its_call_runs(A, ctx):
     mine = [torch.full_like(x, 3.0) for _ in range(8)]
     torch.cuda.synchronize()
     assert all((m == 3.0).all() for m in mine)
+
+
+@pytest.mark.parametrize("H", [1, 3, 20, 128])
+def test_mass_of_strided_queries(A, ctx, H):
+    """Head-major q, heads and tokens with space between them, every other token of a longer q: the bits of a dense q."""
+    lens, new = [300, 70], [5, 2]
+    pg = R.Paged(lens, new, 32, torch.bfloat16, "cuda", seed=H)
+    T = sum(new)
+    q = torch.randn(T, H, R.ROW, generator=torch.Generator().manual_seed(H)).bfloat16().cuda()
+    words = R.to_words(R.tree_masks(new, 4), "cuda")
+    m = torch.rand(pg.n_slots, device="cuda")
+    m0 = m.clone()
+    cache = pg.cache(A, mass=m)
+    _, lse = ctx.tree(q, cache, pg.starts, words, SCALE)
+    ctx.mass(q, lse, cache, pg.starts, words, SCALE, decay=0.5)
+    want = m.clone()
+    assert not torch.equal(want, m0)
+    nan = lambda *s: torch.full(s, float("nan"), dtype=torch.bfloat16, device="cuda")
+    forms = {"heads first": nan(H, T, 576).transpose(0, 1), "heads first, spaced": nan(H, T, 584)[:, :, :576].transpose(0, 1),
+             "spaced heads": nan(T, H, 640)[:, :, :576], "every other token": nan(2 * T, H, 576)[::2], "part of the heads": nan(T, H + 5, 576)[:, 2:H + 2]}
+    for name, qs in forms.items():
+        qs.copy_(q)
+        m.copy_(m0)
+        ctx.mass(qs, lse, cache, pg.starts, words, SCALE, decay=0.5)
+        assert torch.equal(m, want), name
+    ctx.device_error()
+
+
+def test_repeated_queries(A, ctx, native):
+    """A stride of 0: attention takes it, mass says that it does not."""
+    pg = R.Paged([100], [3], 16, torch.bfloat16, "cuda", seed=1)
+    m = torch.zeros(pg.n_slots, device="cuda")
+    cache = pg.cache(A, mass=m)
+    one = torch.randn(1, 1, R.ROW, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    for q in (one.expand(3, 6, R.ROW), one.expand(3, 1, R.ROW).contiguous().expand(3, 6, R.ROW), one.expand(1, 6, R.ROW).contiguous().expand(3, 6, R.ROW)):
+        out, lse = ctx.tree(q, cache, pg.starts, None, SCALE)
+        o2, l2 = ctx.tree(q.contiguous(), cache, pg.starts, None, SCALE)
+        assert torch.equal(out, o2) and torch.equal(lse, l2)
+        with pytest.raises(native.NativeError, match="strides"):
+            ctx.mass(q, lse, cache, pg.starts, None, SCALE)
+    ctx.mass(q.contiguous(), lse, cache, pg.starts, None, SCALE)
+    ctx.device_error()
