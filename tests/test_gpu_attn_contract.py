@@ -338,3 +338,51 @@ def test_repeated_queries(A, ctx, native):
             ctx.mass(q, lse, cache, pg.starts, None, SCALE)
     ctx.mass(q.contiguous(), lse, cache, pg.starts, None, SCALE)
     ctx.device_error()
+
+
+def test_a_captured_step_follows_its_inputs(A, ctx):
+    """Rotate, append, attend, add the weights and evict in one graph: replayed on new inputs, lengths and weights it gives the
+    bits of the same calls outside a graph."""
+    H, page = 8, 16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    table = A.RopeTable(2000, 64, device="cuda")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    starts, words = i32([0, 3, 5]), R.to_words([1, 3, 5, 1, 3], "cuda")
+
+    def fresh():
+        return dict(rows=torch.zeros(32 * page, R.ROW, dtype=torch.bfloat16, device="cuda"), mass=torch.zeros(32 * page, device="cuda"),
+                    pos=torch.zeros(32 * page, dtype=torch.int32, device="cuda"), lens=i32([0, 0]), q=torch.zeros(5, H, R.ROW, dtype=torch.bfloat16, device="cuda"),
+                    latent=torch.zeros(5, 512, dtype=torch.bfloat16, device="cuda"), k=torch.zeros(5, 64, dtype=torch.bfloat16, device="cuda"),
+                    at=i32([0] * 5), w=torch.zeros(5, device="cuda"), next=i32([0, 0]), new=i32([0, 0]),
+                    out=torch.zeros(5, H, 512, dtype=torch.bfloat16, device="cuda"), lse=torch.zeros(5, H, device="cuda"))
+
+    def step(s, cache):
+        ctx.rope(s["q"], s["at"], table, rot_offset=512, out=s["q"])
+        ctx.append(cache, s["latent"], s["k"], starts, s["at"], table)
+        ctx.tree(s["q"], cache, starts, words, SCALE, out=s["out"], lse=s["lse"])
+        ctx.mass(s["q"], s["lse"], cache, starts, words, SCALE, weight=s["w"], decay=0.9)
+        ctx.evict(cache, 100, s["next"], sinks=2, recent=4, new_lens=s["new"])
+    block = torch.randperm(32, generator=g, device="cuda").int().view(2, 16).contiguous()
+    held, plain = fresh(), fresh()
+    caches = [A.KvCache(s["rows"], page, block, s["lens"], mass=s["mass"], pos=s["pos"]) for s in (held, plain)]
+    step(held, caches[0])                                                # makes the workspaces
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(held, caches[0])
+    for lens in ([140, 3], [0, 250], [101, 100]):
+        new = dict(rows=rand(32 * page, R.ROW), mass=torch.rand(32 * page, generator=g, device="cuda"),
+                   pos=torch.randint(0, 1500, (32 * page,), generator=g, device="cuda").int(), lens=i32(lens), q=rand(5, H, R.ROW),
+                   latent=rand(5, 512), k=rand(5, 64), at=i32([lens[0]] * 3 + [lens[1]] * 2), w=(torch.rand(5, generator=g, device="cuda") * 2 - 0.5),
+                   next=i32([l + 1000 for l in lens]))
+        for s in (held, plain):
+            for name, v in new.items():
+                s[name].copy_(v)
+        graph.replay()
+        step(plain, caches[1])
+        torch.cuda.synchronize()
+        for name in held:
+            assert torch.equal(held[name].view(torch.uint8), plain[name].view(torch.uint8)), (lens, name)
+        assert plain["new"].tolist() == [min(l, 100) for l in lens]
+    ctx.device_error()
