@@ -74,7 +74,8 @@ __device__ __forceinline__ void rotate(float (&a)[V], float (&b)[V], const float
 // ---------------------------------------------------------------- rope
 // A unit is V pairs of the rotated part, or V copied elements; V elements are one 16-byte access (V = 1 where the
 // head's geometry, a stride or a pointer is not a multiple of that).  A thread takes N units a block apart and loads them all
-// before it stores: 805 MB (fp32, 4096 tokens x 128 heads x 192) take 130 us (6.2 TB/s, 95 % of a copy's rate), at N = 1 162 us.
+// before it stores: 805 MB (fp32, 4096 tokens x 128 heads x 192, half pairs) take 130 us a call among others (6.2 TB/s, 95 % of a
+// copy's rate), 124 in a graph.
 template <class T, int V, int LAYOUT, int N>
 __global__ void __launch_bounds__(256) k_rope(RopeParams p, int units, int blocks_per_token) {
     const int t = blockIdx.x / blocks_per_token, rot_units = p.rot / 2 / V;
@@ -129,10 +130,14 @@ static cudaError_t rope_n(const RopeParams& p, int layout, cudaStream_t st) {
     return launch_pdl_n(k_rope<T, V, LK_ROPE_INTERLEAVED, N>, dim3(p.T * bpt), dim3(threads), 0, st, p, units, bpt);
 }
 
-// few tokens: a unit a thread fills more SMs; many: four in flight
+// Units a thread, both sides measured (interleaved / half pairs, 192-wide heads of which 64 rotate, a call in a graph):
+// 16-byte units of 16-bit types: one, at every size (4096 x 128 heads 98 / 109 us, with four 175 / 179; 64 x 128 3.7 / 3.3, 5.5 / 5.6).
+// Others: four from 64 tokens on.  fp32 142 / 124 us for 4096 x 128 (one: 146 / 147), 12.3 / 11.3 for 1024 x 32 (10.3 / 10.3), 4.2 / 4.3 for
+// 64 x 128 (3.9 / 3.9); single elements (heads of 193) 277 / 272 for 4096 x 128 in bf16 (375 / 383), 6.2 / 6.3 for 64 x 128 (7.3 / 7.4).
 template <class T, int V>
 static cudaError_t rope_go(const RopeParams& p, int layout, cudaStream_t st) {
-    return p.T < 64 ? rope_n<T, V, 1>(p, layout, st) : rope_n<T, V, 4>(p, layout, st);
+    if constexpr (V == 8) return rope_n<T, V, 1>(p, layout, st);
+    else return p.T < 64 ? rope_n<T, V, 1>(p, layout, st) : rope_n<T, V, 4>(p, layout, st);
 }
 
 template <class T>
