@@ -4,8 +4,10 @@
  *
  * Every pointer argument is a device pointer unless stated otherwise; work is queued on the caller's stream and
  * the calls do not synchronise (lk_attn_get_error does).  Return values are the LK_* status codes of loki_moe.h;
- * no call exits the process.  A context belongs to one device and holds the workspaces of its calls, so calls on
- * one context are issued to one stream at a time (or ordered by events); contexts are independent.
+ * no call exits the process.  A context belongs to one device, as do all pointers of its calls, and holds the workspaces of
+ * its calls, so calls on one context are issued to one stream at a time (or ordered by events); contexts are independent.
+ * A captured call keeps the workspaces that it was captured with: the context outlives the graph, and later calls of any size
+ * leave them as they are.
  *
  * One cached row is 576 values: the 512-wide latent c, which is the key's first part and the value, and 64
  * rotated key values.  The query of one (token, head) row has the same 576 values (the head's query already
@@ -51,7 +53,9 @@ typedef struct LkRopeConfig {
 
 /* The paged cache of n_seqs sequences.  Row i of sequence b is pool row
  * block_table[b * table_stride + i / page_size] * page_size + i % page_size.  Sequences may share pages where a call only
- * reads rows (lk_attn_tree); lk_attn_append, lk_attn_mass and lk_attn_evict write what their sequences' pages hold. */
+ * reads rows (lk_attn_tree); lk_attn_append, lk_attn_mass and lk_attn_evict write what their sequences' pages hold.  With the
+ * heads shared out over GPUs, lk_attn_mass gives a GPU the share of its heads: sum mass over the GPUs before lk_attn_evict, or
+ * each keeps other rows. */
 typedef struct LkKvCache {
     void* rows;                        /* [n_pages * page_size] rows, 16-byte aligned */
     int64_t row_stride;                /* elements from one row to the next: >= 576 and a multiple of 8 */
@@ -98,6 +102,7 @@ LK_API int lk_attn_append(LkAttnCtx* ctx, const LkKvCache* cache, int in_dtype, 
  * rows and to drafted row j where bit j of tree[t] is set.
  *   out[t][h] = sum_k p_k c_k,  p = softmax(scale * q . row_k),  lse[t][h] = ln sum_k exp(scale * q . row_k)
  * A row that sees nothing gives out = 0, lse = -inf; a row that it does not see never reaches it, whatever it holds.
+ * Tokens that are in no sequence's range (before starts[0], or from starts[n_seqs] on) have their out and lse left as they are.
  * tree null: every token sees the drafted rows up to its own (a plain chain).  One token per sequence and tree null is
  * ordinary decoding.  out [T][H][512] in cache->dtype, lse [T][H] fp32 (optional).  Strides in elements, multiples of 8. */
 LK_API int lk_attn_tree(LkAttnCtx* ctx, const LkKvCache* cache, const void* q, int64_t q_token, int64_t q_head, int T, int H,

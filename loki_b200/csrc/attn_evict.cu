@@ -10,9 +10,11 @@
 // memory (sequences of up to 8 x EV_KEYS rows; beyond, it computes them again in each pass).  Per digit the CTAs' histograms
 // are added over distributed shared memory by each CTA alike, so one cluster barrier a digit is all they exchange; ranks come
 // from ordered block scans and the CTAs' totals.  It reads 8 bytes a row once and is bound by its ~10 barriers and scans
-// (one CTA per sequence took 170 us of a 16-sequence call).  1200 rows cut to 1024: 12.9 us a call, nearly all of it this.
-// k_evict_move: 72 threads copy a row's 1152 bytes; memory-bound.  16 sequences of 6000 to 40 000 rows cut to 8192: both 22.5 us,
-// 168 MB at 7.5 TB/s, which L2 gives in part (the plain forms 377 and 470).
+// (one CTA per sequence took 170 us of a 16-sequence call).
+// k_evict_move: 72 threads copy a row's 1152 bytes, two rows in flight; rows lie anywhere in the pool.
+// Times a call with mass and pos put back before each (a call leaves nothing for the next on the same cache to move): 1200 rows
+// cut to 1024, 167 of them moved, 14.3 us, nearly all of it the selection; 16 sequences of 6000 to 40 000 rows cut to 8192, 74 135
+// rows moved, 66: the selection 22, the moves 42 (171 MB read and written, 4.1 TB/s).  The plain forms 305 and 665.
 #include "attn_tc.cuh"
 #include "moe_internal.h"
 

@@ -11,7 +11,8 @@
 // each SM's; Q is re-read per key tile (16 KB per 512 cycles and SM, from L2).  Measured 531 cycles a chunk of 512.  With one
 // block (a decoded token) the cache's 1152 bytes a key from HBM are the bound, and below a tile a pair the set-up of 3 us.
 // Times a call: 4 sequences x 12 nodes, 128 heads, 10 000 to 30 000 rows, 60 % of the weights positive: 81 to 93 us by the clock
-// that the power allows (53 to 61 of products; the plain form 6620); one token over 8191 rows 9.7 (824).
+// that the power allows (53 to 61 of products; the plain form 6600); one token over 8191 rows 11.5 with the cache from HBM, 9.7 where it
+// is in L2 from the attention before it (819).
 //
 // The key tile stays in shared memory (9 chunks of 64 values, 144 KB); each chunk is replaced as soon as the last row block has
 // read it, so the next tile's loads run under the rest.  Q chunks go through a ring of 4 (16 KB: the CTA's half of the rows x 64

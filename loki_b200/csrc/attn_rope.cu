@@ -157,8 +157,9 @@ cudaError_t launch_rope(const RopeParams& p, int dtype, int layout, cudaStream_t
 }
 
 // ---------------------------------------------------------------- append
-// One thread per 8 latent values (64 of them) or 8 rotated pairs (4): 68 units a token.  8 x 1024 fp32 rows take 7.1 us a call,
+// One thread per 8 latent values (64 of them) or 8 rotated pairs (4): 68 units a token.  8 x 1024 bf16 rows take 7.2 us a call,
 // 3.2 of them the bytes: the launch and the chain of loads from starts to page are the rest (8.3 with the values loaded after it).
+// fp32 rows 9.5, 4.6 of them the bytes; up to 64 rows 2.7 in a graph.
 constexpr int AP_UNITS = AT_LATENT / 8 + AT_ROPE / 16;
 
 template <class T> __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {

@@ -15,10 +15,15 @@
 // Measured on a B200, 2-CTA M = 128 runs at the full 4096 products per cycle and SM for N = 128 and 256 (one CTA with
 // M = 128, N = 128 reaches 2925), so a unit costs 2176 cycles of tensor pipe.  A unit takes about 3000: the thread that issues S
 // waits at five stages of K a tile.  L2 is not what bounds it (136 KB a CTA; leaving V's loads out gains under 5 %).
-// Times a call: 64 nodes over 65 000 rows 1055 us (1.10 PFLOP/s at the 1.2 to 1.4 GHz that the power allows), 8 nodes over 16 384
-// rows 49.7, one token over 30 011 rows 27.6 (of them 8 the tiles and 10 the parts and their merge), 16 sequences of 3 to 17
-// nodes on 32 heads 95, one tile 11.6 (14 where the pages could hold more and the merge is launched); the plain forms: 24 960, 1472,
-// 836, 6247, 694.
+// Times a call: 64 nodes over 65 000 rows 1050 us in a long run (1.10 PFLOP/s at the 1.49 GHz that 1 kW allows; 915 to 920 in the first
+// ten calls after a rest), 8 nodes over 16 384 rows 49.7, one token over 30 011 rows 27.6 (of them 8 the tiles and 10 the parts and
+// their merge; the same whether the cache lies in L2 or not), 16 sequences of 3 to 17 nodes on 32 heads 95, one tile 12 (14 where the
+// pages could hold more and the merge is launched); the plain forms: 25 000, 1470, 837, 6250, 699.
+//
+// P is rounded to the cache's type before its product, because an MMA takes 16-bit operands of one type (in tf32 it would run at half
+// the rate or less, on a copy of C in 32 bits).  The rounding is relative, 2^-9 (bf16) or 2^-12 (fp16) of each weight at most, and the sum l
+// takes the weights unrounded: against 64 bits out is off by 1.7 to 2.0e-3 in bf16, where the rounding of out alone gives 1.66e-3, and
+// by 2.2 to 2.6e-4 in fp16 (2.07e-4); lse by 1 to 4e-7.
 //
 // Roles (384 threads a CTA): warp 0 loads (TMA, ring of 8 x 16 KB), warps 1 and 2 of CTA 0 issue the MMAs of S and of O,
 // warp 3 repairs tail tiles, warps 4-11 do softmax, O's scaling and the output (two threads per tensor-memory lane, four per
@@ -30,7 +35,8 @@
 //
 // Rows that must not matter: a tile's rows beyond the drafts, and drafted rows that a token does not see, get P = 0; but
 // 0 * NaN is NaN, so the former are loaded as zeros from outside the pool (the last 16 rows' rest is zeroed by warp 3), and warp 3
-// zeroes every drafted row of the O operand that holds a non-finite value (a token that does see it gets its NaN through S and P).
+// zeroes every drafted row of the O operand that holds a non-finite value (a token that does see it gets its NaN through S and P; where
+// its score is -infinity, the row has no weight).
 #include <type_traits>
 #include "attn_tc.cuh"
 #include "attn_sched.cuh"
