@@ -130,7 +130,11 @@ class MoeLayer:
         return check(rc, self.ctx)
 
     def forward(self, W, x, resid, logits_override=None, h=None, moe=None, sel=None, w=None, stream=None):
-        """h, moe, sel, w = layer(x, resid): all CUDA tensors; outputs allocated when not given."""
+        """h, moe, sel, w = layer(x, resid): all CUDA tensors; outputs allocated when not given (with stream, from its pool:
+        memory of the current stream's may be in use until that one's queue ends).  So in the calls below."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.forward(W, x, resid, logits_override, h, moe, sel, w)
         T = x.shape[0]
         dev = x.device
         h = torch.empty(T, HIDDEN, device=dev) if h is None else h
@@ -139,35 +143,44 @@ class MoeLayer:
         w = torch.empty(T, self.keep, device=dev) if w is None else w
         ws = W.struct() if hasattr(W, "struct") else W
         self._check(lib().lk_moe_forward(self.ctx, ctypes.byref(ws), _ptr(x), _ptr(resid), T, _ptr(logits_override),
-                                         _ptr(h), _ptr(moe), _ptr(sel), _ptr(w), _stream(stream)))
+                                         _ptr(h), _ptr(moe), _ptr(sel), _ptr(w), _stream()))
         return h, moe, sel, w
 
     def route(self, W, x, logits_override=None, stream=None):
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.route(W, x, logits_override)
         T = x.shape[0]
         sel = torch.empty(T, self.keep, dtype=torch.int32, device=x.device)
         w = torch.empty(T, self.keep, device=x.device)
         probs = torch.empty(T, N_EXPERTS, device=x.device)
         ws = W.struct() if hasattr(W, "struct") else W
         self._check(lib().lk_moe_route(self.ctx, ctypes.byref(ws), _ptr(x), T, _ptr(logits_override), _ptr(sel), _ptr(w),
-                                       _ptr(probs), _stream(stream)))
+                                       _ptr(probs), _stream()))
         return probs, sel, w
 
     def dispatch(self, sel, w, stream=None):
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.dispatch(sel, w)
         T, keep = sel.shape
         counts = torch.empty(N_EXPERTS, dtype=torch.int32, device=sel.device)
         offsets = torch.empty(N_EXPERTS + 1, dtype=torch.int32, device=sel.device)
         perm = torch.empty(T * keep, dtype=torch.int32, device=sel.device)
         self._check(lib().lk_moe_dispatch(self.ctx, _ptr(sel), _ptr(w), T, keep, _ptr(counts), _ptr(offsets), _ptr(perm),
-                                          _stream(stream)))
+                                          _stream()))
         return counts, offsets, perm
 
     def experts(self, W, x, resid, sel, w, h=None, moe=None, stream=None):
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.experts(W, x, resid, sel, w, h, moe)
         T, keep = sel.shape
         h = torch.empty(T, HIDDEN, device=x.device) if h is None else h
         moe = torch.empty(T, HIDDEN, device=x.device) if moe is None else moe
         ws = W.struct() if hasattr(W, "struct") else W
         self._check(lib().lk_moe_experts(self.ctx, ctypes.byref(ws), _ptr(x), _ptr(resid), T, _ptr(sel), _ptr(w), keep,
-                                         _ptr(h), _ptr(moe), _stream(stream)))
+                                         _ptr(h), _ptr(moe), _stream()))
         return h, moe
 
     def set_gemm_threshold(self, min_tokens):
